@@ -350,6 +350,97 @@ QTTS_API int qtts_w8a16_head_argmax(const void* x, int64_t ldx, int x_dtype, con
                                     int vocab, void* embed_out, int64_t ldeo, int E, uint64_t* state, int M, int N,
                                     int K, unsigned flags, void* stream);
 
+/* ---- residual + RMSNorm -> 8 bits ----------------------------------------------
+ * What stands between two W8A8 linears of a decoder layer, in one launch:
+ *   h        = x + residual                       (fp32; x alone when residual is NULL)
+ *   residual_out = cast(h)
+ *   y        = weight * (h * (1 / sqrt(mean(h^2) + eps)))
+ *   scale[m] = max(max_k |y[m,k]|, 1e-6) * fl32(1 / 448)   (e4m3; 1 / 127 for int8)
+ *   q[m,k]   = e4m3_rne(y / scale), or clamp(rne(y / scale), -127, 127)
+ * in fp32 from the inputs to the codes (neither h nor y is rounded to x's type
+ * on the way, unlike the separate kernels). x, residual, residual_out, weight:
+ * BF16, FP16 or FP32 (dtype); residual_out may be residual or x (in place; same
+ * leading dimension). q: [rows, width] of q_dtype (QTTS_E4M3 or QTTS_INT8), ready
+ * for qtts_fp8_gemm / qtts_i8_gemm with scale [rows]. width <= 65536. residual
+ * and residual_out are both given or both NULL. A row with a NaN or an infinity
+ * gets a NaN scale. Replaces: residual add, RMSNorm.forward (qtts/layers/norm.py:
+ * 102-137) and the activation quantization of Fp8Method / Int8Method
+ * (qtts/quant/fp8.py:77-78, int8.py:138-140). */
+QTTS_API int qtts_add_rms_norm_quant(const void* x, int64_t ldx, const void* residual, int64_t ldr,
+                                     const void* weight, float eps, void* residual_out, int64_t ldro, int dtype,
+                                     void* q, int64_t ldq, int q_dtype, float* scale, int rows, int width,
+                                     unsigned flags, void* stream);
+
+/* ---- 4-bit key/value cache -------------------------------------------------------
+ * A paged cache: keys and values apart, each as
+ *   codes  [pages, kv_heads, page_size, head_dim / 2] bytes, two 4-bit codes each
+ *   params [pages, kv_heads, page_size, head_dim / 32, 2] bf16: scale, minimum
+ * (contiguous, 16-byte aligned). 32 neighbouring channels of one token and head
+ * form a group: scale = bf16((max - min) / 15), minimum = bf16(min), code =
+ * clamp(rne((x - minimum) / scale), 0, 15), standing for code * scale + minimum.
+ * Nibble order, n = head_dim / 32: a key's channel 32j + 8c + i is nibble i (from
+ * the low end) of 32-bit word c * n + j of its row, a value's channel 32j + 4g + i
+ * is nibble i of 16-bit word g * n + j. A token's place is its slot: page *
+ * page_size + row. One page of `slots` rows a request is a slot cache, as
+ * TalkerKVCache (qtts/models/talker.py:47-91) has it in 16 bits. head_dim is 64
+ * or 128. */
+
+/* Per-head RMSNorm, rotary positions with up to four axes and the cache write
+ * of a fused projection's output, in one launch.
+ *   qkv       [tokens, (q_heads + 2 * kv_heads) * head_dim], BF16 or FP16, leading
+ *             dimension ldqkv: the q heads, then the k heads, then the v heads
+ *   q_norm, k_norm  [head_dim] of qkv's type, or NULL: no norm of that part
+ *   cos, sin  [table_len, head_dim / 2] fp32 tables, or both NULL: no rotation.
+ *             Pair (j, j + head_dim / 2) of a q or k head is turned by the tables'
+ *             row positions[axis(j), token], column j
+ *   positions [axes, tokens] int64, leading dimension ldpos
+ *   sections  host array of `axes` (1..4) counts of pairs that sum to head_dim / 2:
+ *             the first sections[0] pairs belong to axis 0, the next to axis 1, ...;
+ *             with `interleaved`, pair j belongs to axis j % axes while j < axes *
+ *             sections[that axis], and to axis 0 otherwise
+ *   slots     [tokens] int64; a negative slot is not stored. Slots are distinct.
+ *   q_out     [tokens, q_heads * head_dim] of qkv's type, leading dimension ldq
+ *   k_values, v_values  [tokens, kv_heads, head_dim] of qkv's type, or both NULL:
+ *             what the cache will give back for these tokens
+ * fp32 from the load to the one rounding of each output. A position outside the
+ * tables or a slot outside the cache records QTTS_ERR_SHAPE on the device; such a
+ * token is not stored (and with a bad position its outputs are zeros). 16-byte
+ * aligned rows. Replaces: q/k norm, apply_rope and the cache write of
+ * TalkerAttention (qtts/models/talker.py:94-136, qtts/layers/rope.py:23-72). */
+QTTS_API int qtts_rope_kv4_append(const void* qkv, int64_t ldqkv, int dtype, int tokens, int q_heads, int kv_heads,
+                                  int head_dim, const void* q_norm, const void* k_norm, float eps,
+                                  const float* cos, const float* sin, int64_t table_len, const int64_t* positions,
+                                  int64_t ldpos, int axes, const int* sections, int interleaved,
+                                  const int64_t* slots, void* q_out, int64_t ldq, uint8_t* k_codes, void* k_params,
+                                  uint8_t* v_codes, void* v_params, int64_t pages, int page_size, void* k_values,
+                                  void* v_values, unsigned flags, void* stream);
+
+/* Attention of one or many new tokens a request over the 4-bit cache:
+ *   out[i, h] = sum_t softmax_t(scale * q[i, h] . k[t, h']) v[t, h'],
+ *   h' = h / (q_heads / kv_heads)
+ * The new tokens of a request are the last n of its lengths[b] cached tokens (they
+ * are in the cache already). With `causal`, new token i sees the cached tokens
+ * t <= lengths[b] - n + i, without it all lengths[b]. A row that sees nothing
+ * gives zeros. What lies in the cache beyond a row's tokens is never used, be it
+ * NaN.
+ *   q           token and head strides in elements (multiples of 8), BF16 or FP16
+ *   block_table [batch, table_cols] int32 page numbers, leading dimension ld_table
+ *   lengths     [batch] int32, at most table_cols * page_size
+ *   q_starts    [batch + 1] int32 first rows of q; NULL: max_q rows a request
+ *   max_q       the most new tokens of any request (bounds the launch)
+ *   out         [total_q, q_heads, head_dim] of q's type, token stride given
+ * page_size is a multiple of 16. Scores, softmax statistics and sums are fp32. A
+ * length, row range or page number out of its bounds records QTTS_ERR_SHAPE on the
+ * device and the tokens concerned are left out. Replaces: the SDPA backend over the
+ * slot cache (qtts/attention/backends/torch_sdpa.py:16-69). */
+QTTS_API int qtts_kv4_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, int dtype,
+                                const uint8_t* k_codes, const void* k_params, const uint8_t* v_codes,
+                                const void* v_params, int64_t pages, int page_size, const int32_t* block_table,
+                                int64_t ld_table, int table_cols, const int32_t* lengths, const int32_t* q_starts,
+                                int total_q, int max_q, int batch, int q_heads, int kv_heads, int head_dim,
+                                float scale, int causal, void* out, int64_t out_token_stride, unsigned flags,
+                                void* stream);
+
 /* ---- int8 W8A8 (Int8Method) --------------------------------------------------
  * Per-token int8 quantization of the activations of Int8Method.apply
  * (qtts/quant/int8.py:138-140), each step in the activation dtype as torch

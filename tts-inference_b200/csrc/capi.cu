@@ -33,6 +33,8 @@ size_t dtype_size(int d) {
 }
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+}  // namespace
+
 // ---- device capability ------------------------------------------------------------
 int check_device() {
   int dev = 0;
@@ -46,6 +48,8 @@ int check_device() {
   }
   return cc_major[dev] == 10 ? QTTS_OK : QTTS_ERR_ARCH;
 }
+
+namespace {
 
 // ---- driver entry point for tensor-map encoding -------------------------------------
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,

@@ -429,6 +429,18 @@ __device__ __forceinline__ float to_float<float>(float v) {
   return v;
 }
 
+// Minimum and maximum that keep a NaN (fminf / fmaxf drop it).
+__device__ __forceinline__ float nan_min(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float nan_max(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
 // Timeline probe, compiled in only with -DQTTS_TRACE (never in the shipped
 // library): globaltimer stamps per CTA at each phase of a kernel, read back by
 // qtts_trace_read(). `a` must be the kernel's argument block (trace_slot).

@@ -162,6 +162,81 @@ int make_tmap_16b_2d(CUtensorMap* map, const void* base, int dtype, uint64_t row
 
 uint64_t current_wait_limit_ns();
 
+// QTTS_OK when the current device is an sm_100 part, QTTS_ERR_ARCH otherwise.
+int check_device();
+
+// ---- residual + RMSNorm -> 8 bits (csrc/add_norm_quant.cu) -----------------------
+struct AddNormQuantArgs {
+  const void* x;
+  int64_t ldx;
+  const void* residual;  // or nullptr
+  int64_t ldr;
+  const void* weight;  // [width], of x's type
+  float eps;
+  void* residual_out;  // nullptr exactly when residual is
+  int64_t ldro;
+  void* q;  // e4m3 or int8, leading dimension ldq
+  int64_t ldq;
+  float* scale;  // [rows]
+  int rows, width;
+  bool vec;  // rows, weight and outputs allow 16-byte loads and 8-byte code stores; width % 8 == 0
+};
+int launch_add_norm_quant(const AddNormQuantArgs& a, int dtype, int q_dtype, bool pdl, cudaStream_t stream);
+
+// ---- 4-bit cache (csrc/kv4.cuh, rope_kv4.cu, kv4_attention.cu) --------------------
+struct Kv4Cache {
+  uint8_t* k_codes;    // [pages, kv_heads, page_size, head_dim / 2]
+  uint32_t* k_params;  // [pages, kv_heads, page_size, head_dim / 32]: scale (low half), minimum (high half), bf16
+  uint8_t* v_codes;
+  uint32_t* v_params;
+  int64_t pages;
+  int page_size;
+  int kv_heads;
+};
+
+constexpr int kMaxRopeAxes = 4;
+constexpr int kKv4MaxPairs = 64;  // head_dim <= 128
+
+struct RopeKv4Args {
+  const void* qkv;
+  int64_t ldqkv;
+  int tokens, q_heads;
+  const void* q_norm;  // [head_dim] of qkv's type, or nullptr
+  const void* k_norm;
+  float eps;
+  const float* cos;  // [table_len, head_dim / 2], or nullptr: no rotation
+  const float* sin;
+  int64_t table_len;
+  const int64_t* positions;  // [axes, tokens], leading dimension ldpos
+  int64_t ldpos;
+  int axes;
+  uint64_t axis_of[2];  // two bits for each pair of channels: its axis
+  const int64_t* slots;  // [tokens]: page * page_size + row; negative: not stored
+  void* q_out;           // [tokens, q_heads * head_dim], leading dimension ldq
+  int64_t ldq;
+  Kv4Cache cache;
+  void* k_values;  // [tokens, kv_heads, head_dim] as stored, or nullptr
+  void* v_values;
+};
+int launch_rope_kv4(const RopeKv4Args& a, int dtype, int head_dim, bool pdl, cudaStream_t stream);
+
+struct Kv4AttnArgs {
+  const void* q;
+  int64_t q_token_stride, q_head_stride;
+  Kv4Cache cache;
+  const int32_t* table;  // [batch, table_cols], leading dimension ld_table
+  int64_t ld_table;
+  int table_cols;
+  const int32_t* lengths;   // [batch]
+  const int32_t* q_starts;  // [batch + 1], or nullptr: max_q tokens a request
+  int total_q, max_q, batch, q_heads;
+  float scale;
+  int causal;
+  void* out;  // [total_q, q_heads, head_dim]
+  int64_t out_token_stride;
+};
+int launch_kv4_attention(const Kv4AttnArgs& a, int dtype, int head_dim, bool pdl, cudaStream_t stream);
+
 #ifdef QTTS_TRACE
 int qtts_trace_next_slot();
 #endif

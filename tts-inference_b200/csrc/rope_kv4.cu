@@ -1,0 +1,265 @@
+// Per-head RMSNorm, rotary positions with several axes and the 4-bit cache write
+// of a fused projection's output, in one launch (qtts_rope_kv4_append).
+//
+// Input row of a token: [q heads | k heads | v heads], D channels each
+// (MergedLinear's qkv order). Per head of q and k:
+//   y = w * (x * (1 / sqrt(mean(x^2) + eps)))          (skipped without a weight)
+//   (y[j], y[j + D/2]) turned by the angle of pair j    (skipped without tables)
+// where the angle is the table's row for the position of the token along the axis
+// that pair j belongs to (time, height, width for images and video; one axis for
+// text). q is written in its own type, k and v as 4-bit groups (kv4.cuh). All of
+// it in fp32 between the load and the one rounding of each output.
+//
+// D / 8 lanes hold one head row, eight neighbouring channels each: one 16-byte
+// load, a pair's partner D / 16 lanes away, a group of 32 channels on four
+// neighbouring lanes, and a lane's eight codes are exactly one 32-bit word of a
+// key row or two 16-bit words of a value row.
+#include "kernels.h"
+#include "kv4.cuh"
+#include "prologue.cuh"
+
+namespace qtts {
+namespace {
+
+constexpr int kRkThreads = 256;
+
+// The eight codes of a lane's channels; returns them one a nibble and gives the
+// values that they stand for. lo/hi: minimum and maximum of the group.
+__device__ __forceinline__ uint32_t quantize_group(const float (&y)[8], float lo, float hi, uint32_t& params,
+                                                   float (&held)[8]) {
+  const __nv_bfloat16 sb = __float2bfloat16_rn(__fdiv_rn(hi - lo, 15.0f));
+  const __nv_bfloat16 zb = __float2bfloat16_rn(lo);
+  params = static_cast<uint32_t>(__bfloat16_as_ushort(sb)) | (static_cast<uint32_t>(__bfloat16_as_ushort(zb)) << 16);
+  const float s = __bfloat162float(sb), z = __bfloat162float(zb);
+  uint32_t word = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    float c = s > 0.f ? rintf(__fdiv_rn(y[i] - z, s)) : 0.f;
+    c = fminf(fmaxf(c, 0.f), 15.f);
+    word |= static_cast<uint32_t>(c) << (4 * i);
+    held[i] = __fadd_rn(__fmul_rn(c, s), z);
+  }
+  return word;
+}
+
+template <typename T>
+__device__ __forceinline__ uint4 pack8(const float (&y)[8]) {
+  uint4 o;
+  T* r = reinterpret_cast<T*>(&o);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) r[i] = from_float<T>(y[i]);
+  return o;
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kRkThreads) rope_kv4_kernel(const RopeKv4Args a) {
+  constexpr int kLanes = D / 8;      // lanes a head row
+  constexpr int kGroups = D / kKv4Group;
+  pdl_launch_dependents();
+  pdl_wait();
+  const int heads = a.q_heads + 2 * a.cache.kv_heads;
+  const int64_t item = (static_cast<int64_t>(blockIdx.x) * kRkThreads + threadIdx.x) / kLanes;
+  const int l = threadIdx.x % kLanes;
+  const bool live = item < static_cast<int64_t>(a.tokens) * heads;
+  const int64_t t = live ? item / heads : 0;
+  const int head = live ? static_cast<int>(item - t * heads) : 0;
+  const int kv = head - a.q_heads;  // key head, or kv_heads + value head
+  const bool is_q = kv < 0;
+  const bool is_v = kv >= a.cache.kv_heads;
+
+  const uint4 raw = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.qkv) + t * a.ldqkv + head * D + 8 * l);
+  const T* e = reinterpret_cast<const T*>(&raw);
+  float y[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) y[i] = to_float(e[i]);
+
+  const T* w = static_cast<const T*>(is_q ? a.q_norm : a.k_norm);
+  if (w != nullptr) {
+    float ss = leaf_sumsq(y);
+#pragma unroll
+    for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    if (!is_v) {
+      const float inv = rms_inv(ss, D, a.eps);
+      const uint4 wr = __ldg(reinterpret_cast<const uint4*>(w + 8 * l));
+      const T* we = reinterpret_cast<const T*>(&wr);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = rms_apply(y[i], inv, to_float(we[i]));
+    }
+  }
+  // A token with a position outside the tables gives zeros and is not stored.
+  bool ok = true;
+  if (a.cos != nullptr) {
+    int64_t pos[kMaxRopeAxes];
+#pragma unroll
+    for (int x = 0; x < kMaxRopeAxes; ++x) {
+      pos[x] = x < a.axes ? a.positions[x * a.ldpos + t] : 0;
+      if (pos[x] < 0 || pos[x] >= a.table_len) {
+        pos[x] = 0;
+        ok = false;
+      }
+    }
+    if (!ok) record_status(QTTS_ERR_SHAPE);
+    const int j0 = 8 * (l % (kLanes / 2));  // first of this lane's pairs
+    const float sign = l < kLanes / 2 ? -1.f : 1.f;
+    float other[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) other[i] = __shfl_xor_sync(0xffffffffu, y[i], kLanes / 2);
+    if (!is_v) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int j = j0 + i;
+        const int axis = static_cast<int>(a.axis_of[j >> 5] >> (2 * (j & 31))) & 3;
+        const int64_t at = (axis == 0 ? pos[0] : axis == 1 ? pos[1] : axis == 2 ? pos[2] : pos[3]) * (D / 2) + j;
+        y[i] = __fadd_rn(__fmul_rn(y[i], a.cos[at]), sign * __fmul_rn(other[i], a.sin[at]));
+      }
+    }
+  }
+  if (!ok) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = 0.f;
+  }
+  float lo = y[0], hi = y[0];
+#pragma unroll
+  for (int i = 1; i < 8; ++i) lo = nan_min(lo, y[i]), hi = nan_max(hi, y[i]);
+#pragma unroll
+  for (int o = 2; o > 0; o >>= 1) {
+    lo = nan_min(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+    hi = nan_max(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+  }
+  if (!live) return;
+  if (is_q) {
+    *reinterpret_cast<uint4*>(static_cast<T*>(a.q_out) + t * a.ldq + head * D + 8 * l) = pack8<T>(y);
+    return;
+  }
+  uint32_t params;
+  float held[8];
+  const uint32_t word = quantize_group(y, lo, hi, params, held);
+  const int h = is_v ? kv - a.cache.kv_heads : kv;
+  T* values = static_cast<T*>(is_v ? a.v_values : a.k_values);
+  if (values != nullptr) {
+    *reinterpret_cast<uint4*>(values + (t * a.cache.kv_heads + h) * D + 8 * l) = pack8<T>(held);
+  }
+  const int64_t slot = a.slots[t];
+  if (slot < 0 || !ok) return;
+  if (slot >= a.cache.pages * a.cache.page_size) {
+    record_status(QTTS_ERR_SHAPE);
+    return;
+  }
+  const int64_t page = slot / a.cache.page_size;
+  const int64_t row = kv4_row(a.cache, page, h, static_cast<int>(slot - page * a.cache.page_size));
+  const int j = l / 4, c = l % 4;
+  if (is_v) {
+    uint16_t* dst = reinterpret_cast<uint16_t*>(a.cache.v_codes + row * (D / 2));
+    dst[(2 * c) * kGroups + j] = static_cast<uint16_t>(word & 0xffffu);
+    dst[(2 * c + 1) * kGroups + j] = static_cast<uint16_t>(word >> 16);
+    if (c == 0) a.cache.v_params[row * kGroups + j] = params;
+  } else {
+    reinterpret_cast<uint32_t*>(a.cache.k_codes + row * (D / 2))[c * kGroups + j] = word;
+    if (c == 0) a.cache.k_params[row * kGroups + j] = params;
+  }
+}
+
+template <typename T, int D>
+int launch_rk(const RopeKv4Args& a, bool pdl, cudaStream_t stream) {
+  const int64_t lanes = static_cast<int64_t>(a.tokens) * (a.q_heads + 2 * a.cache.kv_heads) * (D / 8);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>((lanes + kRkThreads - 1) / kRkThreads));
+  cfg.blockDim = dim3(kRkThreads);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  if (pdl) {
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+  }
+  return cudaLaunchKernelEx(&cfg, rope_kv4_kernel<T, D>, a) == cudaSuccess ? QTTS_OK : QTTS_ERR_LAUNCH;
+}
+
+}  // namespace
+
+int launch_rope_kv4(const RopeKv4Args& a, int dtype, int head_dim, bool pdl, cudaStream_t stream) {
+  if (dtype == QTTS_BF16) {
+    return head_dim == 128 ? launch_rk<__nv_bfloat16, 128>(a, pdl, stream)
+                           : launch_rk<__nv_bfloat16, 64>(a, pdl, stream);
+  }
+  return head_dim == 128 ? launch_rk<__half, 128>(a, pdl, stream) : launch_rk<__half, 64>(a, pdl, stream);
+}
+
+}  // namespace qtts
+
+extern "C" int qtts_rope_kv4_append(const void* qkv, int64_t ldqkv, int dtype, int tokens, int q_heads, int kv_heads,
+                                    int head_dim, const void* q_norm, const void* k_norm, float eps,
+                                    const float* cos, const float* sin, int64_t table_len, const int64_t* positions,
+                                    int64_t ldpos, int axes, const int* sections, int interleaved,
+                                    const int64_t* slots, void* q_out, int64_t ldq, uint8_t* k_codes, void* k_params,
+                                    uint8_t* v_codes, void* v_params, int64_t pages, int page_size, void* k_values,
+                                    void* v_values, unsigned flags, void* stream) {
+  using namespace qtts;
+  if (tokens < 0 || q_heads < 0 || kv_heads < 1 || q_heads > 4096 || kv_heads > 4096) return QTTS_ERR_SHAPE;
+  if (head_dim != 64 && head_dim != 128) return QTTS_ERR_SHAPE;
+  if (pages < 0 || page_size < 1) return QTTS_ERR_SHAPE;
+  if (dtype != QTTS_BF16 && dtype != QTTS_FP16) return QTTS_ERR_DTYPE;
+  if (tokens == 0) return QTTS_OK;
+  if (qkv == nullptr || slots == nullptr || (q_heads > 0 && q_out == nullptr)) return QTTS_ERR_NULL;
+  if (pages > 0 && (k_codes == nullptr || k_params == nullptr || v_codes == nullptr || v_params == nullptr)) {
+    return QTTS_ERR_NULL;
+  }
+  if ((cos == nullptr) != (sin == nullptr) || (cos != nullptr && (positions == nullptr || sections == nullptr))) {
+    return QTTS_ERR_NULL;
+  }
+  if ((k_values == nullptr) != (v_values == nullptr)) return QTTS_ERR_NULL;
+  const int64_t width = static_cast<int64_t>(q_heads + 2 * kv_heads) * head_dim;
+  if (ldqkv < width || ldq < static_cast<int64_t>(q_heads) * head_dim) return QTTS_ERR_SHAPE;
+  if (static_cast<int64_t>(tokens) * width / 8 > (static_cast<int64_t>(1) << 38)) return QTTS_ERR_SHAPE;
+  const auto al = [](const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; };
+  if (!al(qkv, 16) || !al(q_out, 16) || !al(q_norm, 16) || !al(k_norm, 16) || !al(k_values, 16) ||
+      !al(v_values, 16) || !al(k_codes, 16) || !al(v_codes, 16) || !al(k_params, 16) || !al(v_params, 16) ||
+      ldqkv % 8 != 0 || ldq % 8 != 0 || !al(cos, 4) || !al(sin, 4) || !al(positions, 8) || !al(slots, 8)) {
+    return QTTS_ERR_ALIGN;
+  }
+  RopeKv4Args a{};
+  if (cos != nullptr) {
+    if (axes < 1 || axes > kMaxRopeAxes || table_len < 1 || ldpos < tokens) return QTTS_ERR_SHAPE;
+    int sum = 0;
+    for (int x = 0; x < axes; ++x) {
+      if (sections[x] < 0 || sections[x] > head_dim / 2) return QTTS_ERR_SHAPE;
+      sum += sections[x];
+    }
+    if (sum != head_dim / 2) return QTTS_ERR_SHAPE;
+    for (int j = 0; j < head_dim / 2; ++j) {
+      int axis = 0;
+      if (interleaved) {
+        // 0 1 2 0 1 2 ...; an axis that has had its share leaves its turns to axis 0.
+        axis = j % axes;
+        if (j >= axes * sections[axis]) axis = 0;
+      } else {
+        for (int end = sections[0]; j >= end; end += sections[axis]) ++axis;
+      }
+      a.axis_of[j >> 5] |= static_cast<uint64_t>(axis) << (2 * (j & 31));
+    }
+  }
+  const int dev_ok = check_device();
+  if (dev_ok != QTTS_OK) return dev_ok;
+  a.qkv = qkv;
+  a.ldqkv = ldqkv;
+  a.tokens = tokens;
+  a.q_heads = q_heads;
+  a.q_norm = q_norm;
+  a.k_norm = k_norm;
+  a.eps = eps;
+  a.cos = cos;
+  a.sin = sin;
+  a.table_len = table_len;
+  a.positions = positions;
+  a.ldpos = ldpos;
+  a.axes = axes;
+  a.slots = slots;
+  a.q_out = q_out;
+  a.ldq = ldq;
+  a.cache = Kv4Cache{k_codes, static_cast<uint32_t*>(k_params), v_codes, static_cast<uint32_t*>(v_params), pages,
+                     page_size, kv_heads};
+  a.k_values = k_values;
+  a.v_values = v_values;
+  return launch_rope_kv4(a, dtype, head_dim, (flags & QTTS_FLAG_PDL) != 0, static_cast<cudaStream_t>(stream));
+}

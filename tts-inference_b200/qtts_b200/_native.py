@@ -109,6 +109,23 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         [_c_vp, _c_i64, _c_int, _c_int, _c_vp, ctypes.c_float, _c_vp, _c_i64, _c_vp, _c_int, _c_vp, _c_vp, _c_i64,
          _c_int, _c_int, _c_int, _c_vp, _c_int, _c_uint, _c_vp],
     ),
+    "qtts_add_rms_norm_quant": (
+        _c_int,
+        [_c_vp, _c_i64, _c_vp, _c_i64, _c_vp, ctypes.c_float, _c_vp, _c_i64, _c_int, _c_vp, _c_i64, _c_int, _c_vp,
+         _c_int, _c_int, _c_uint, _c_vp],
+    ),
+    "qtts_rope_kv4_append": (
+        _c_int,
+        [_c_vp, _c_i64, _c_int, _c_int, _c_int, _c_int, _c_int, _c_vp, _c_vp, ctypes.c_float, _c_vp, _c_vp, _c_i64,
+         _c_vp, _c_i64, _c_int, _c_vp, _c_int, _c_vp, _c_vp, _c_i64, _c_vp, _c_vp, _c_vp, _c_vp, _c_i64, _c_int,
+         _c_vp, _c_vp, _c_uint, _c_vp],
+    ),
+    "qtts_kv4_attention": (
+        _c_int,
+        [_c_vp, _c_i64, _c_i64, _c_int, _c_vp, _c_vp, _c_vp, _c_vp, _c_i64, _c_int, _c_vp, _c_i64, _c_int, _c_vp,
+         _c_vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, ctypes.c_float, _c_int, _c_vp, _c_i64, _c_uint,
+         _c_vp],
+    ),
     "qtts_w8a16_gemm_prologue_fused": (_c_int, [_c_int, _c_int, _c_int, _c_int, _c_int]),
     "qtts_fp8_linear_noalloc": (
         _c_int,

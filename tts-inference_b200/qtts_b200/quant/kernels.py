@@ -165,6 +165,62 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, *,
     return out.reshape(*x.shape)
 
 
+def add_rms_norm_quant(
+    x: torch.Tensor,
+    residual: torch.Tensor | None,
+    weight: torch.Tensor,
+    eps: float = 1e-6,
+    *,
+    dtype: torch.dtype = torch.float8_e4m3fn,
+    residual_out: torch.Tensor | None = None,
+) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor | None]:
+    """``h = x + residual``, RMSNorm of h over the last dimension, and its 8-bit codes, in one
+    launch (``qtts_add_rms_norm_quant``): ``(q [M, W], scale [M, 1] fp32, h in x's shape)``.
+
+    ``dtype`` is ``torch.float8_e4m3fn`` (for :func:`fp8_scaled_mm`) or ``torch.int8`` (for
+    :func:`i8_scaled_mm`); ``scale`` is the row's largest magnitude, at least 1e-6, over 448
+    or 127. x, residual and weight share one type (bf16, fp16 or fp32). ``residual_out``
+    receives h and may be ``residual`` itself; with ``residual`` None there is no addition
+    and h is None. fp32 throughout: the norm reads the unrounded sum and the quantizer the
+    unrounded norm."""
+    width = x.shape[-1]
+    if weight.dim() != 1 or weight.shape[0] != width:
+        raise ValueError(f"weight is {tuple(weight.shape)}, expected [{width}]")
+    if dtype not in (torch.float8_e4m3fn, torch.int8):
+        raise TypeError(f"codes are float8_e4m3fn or int8, not {dtype}")
+    device = _require_cuda(x, weight, residual, residual_out)
+    a = _rows_view(x, width)
+    rows = a.shape[0]
+    if weight.dtype != x.dtype or weight.stride(0) != 1:
+        weight = weight.to(x.dtype).contiguous()
+    r_ptr = ro_ptr = None
+    ldr = ldro = width
+    if residual is not None:
+        if residual.shape != x.shape or residual.dtype != x.dtype:
+            raise ValueError(f"residual must be {x.dtype} {tuple(x.shape)}")
+        r = _rows_view(residual, width)
+        if residual_out is None:
+            residual_out = torch.empty(x.shape, device=device, dtype=x.dtype)
+            ro = residual_out.view(rows, width)
+        else:
+            ro = _rows_view(residual_out, width)
+            if residual_out.shape != x.shape or ro.dtype != x.dtype or ro.data_ptr() != residual_out.data_ptr():
+                raise ValueError(f"residual_out must be {x.dtype} {tuple(x.shape)} with unit column stride")
+        if rows > 1:
+            ldr, ldro = r.stride(0), ro.stride(0)
+        r_ptr, ro_ptr = r.data_ptr(), ro.data_ptr()
+    elif residual_out is not None:
+        raise ValueError("residual_out needs a residual")
+    q = torch.empty((rows, width), device=device, dtype=dtype)
+    scale = torch.empty((rows, 1), device=device, dtype=torch.float32)
+    code = nat.lib().qtts_add_rms_norm_quant(
+        a.data_ptr(), a.stride(0) if rows > 1 else width, r_ptr, ldr, weight.data_ptr(), eps, ro_ptr, ldro,
+        nat.dtype_code(x.dtype), q.data_ptr(), width, nat.dtype_code(dtype), scale.data_ptr(), rows, width, _flags(),
+        nat.stream_ptr(device))
+    nat.check(code, "qtts_add_rms_norm_quant")
+    return q, scale, residual_out
+
+
 def silu_mul(gate_up: torch.Tensor, *, out: torch.Tensor | None = None) -> torch.Tensor:
     """``F.silu(gate) * up`` of ``gate_up = [gate | up]`` (``[..., 2W]`` -> ``[..., W]``;
     qtts/layers/activation.py:143-147), bit for bit torch's two CUDA kernels."""
