@@ -428,10 +428,12 @@ QTTS_API int qtts_rope_kv4_append(const void* qkv, int64_t ldqkv, int dtype, int
  *   lengths     [batch] int32, at most table_cols * page_size
  *   q_starts    [batch + 1] int32 first rows of q; NULL: max_q rows a request
  *   max_q       the most new tokens of any request (bounds the launch)
+ *   scale       positive and finite
  *   out         [total_q, q_heads, head_dim] of q's type, token stride given
  * page_size is a multiple of 16. Scores, softmax statistics and sums are fp32. A
  * length, row range or page number out of its bounds records QTTS_ERR_SHAPE on the
- * device and the tokens concerned are left out. Replaces: the SDPA backend over the
+ * device; nothing outside the arrays is read, and that request's output means
+ * nothing. Replaces: the SDPA backend over the
  * slot cache (qtts/attention/backends/torch_sdpa.py:16-69). */
 QTTS_API int qtts_kv4_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, int dtype,
                                 const uint8_t* k_codes, const void* k_params, const uint8_t* v_codes,

@@ -66,9 +66,9 @@ def test_write_refuses(lib, want, kw):
 
 def attend(lib, q=16, qt=16 * 128, qh=128, dtype=nat.BF16, kc=16, kp=16, vc=16, vp=16, pages=4, page=16, table=16,
            ld=2, cols=2, lengths=16, starts=None, total=3, max_q=1, batch=3, heads=16, kv_heads=8, d=128, out=16,
-           ot=16 * 128):
+           ot=16 * 128, scale=0.1):
     return lib.qtts_kv4_attention(q, qt, qh, dtype, kc, kp, vc, vp, pages, page, table, ld, cols, lengths, starts, total,
-                                  max_q, batch, heads, kv_heads, d, 0.1, 1, out, ot, 0, None)
+                                  max_q, batch, heads, kv_heads, d, scale, 1, out, ot, 0, None)
 
 
 @pytest.mark.parametrize("want,kw", [
@@ -79,7 +79,8 @@ def attend(lib, q=16, qt=16 * 128, qh=128, dtype=nat.BF16, kc=16, kp=16, vc=16, 
     (NULL, dict(q=None)), (NULL, dict(out=None)), (NULL, dict(lengths=None)), (NULL, dict(table=None)),
     (NULL, dict(kc=None)), (NULL, dict(vp=None)), (SHAPE, dict(qh=64)), (SHAPE, dict(ot=15 * 128)), (ALIGN, dict(q=24)),
     (ALIGN, dict(qt=16 * 128 + 4)), (ALIGN, dict(out=8)), (ALIGN, dict(table=2)), (ALIGN, dict(starts=2)),
-    (ALIGN, dict(vc=8)),
+    (ALIGN, dict(vc=8)), (SHAPE, dict(scale=0.0)), (SHAPE, dict(scale=-1.0)), (SHAPE, dict(scale=float("nan"))),
+    (SHAPE, dict(scale=float("inf"))),
 ])
 def test_attention_refuses(lib, want, kw):
     assert attend(lib, **kw) == want

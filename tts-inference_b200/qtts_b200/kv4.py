@@ -222,6 +222,10 @@ def kv4_attention(
         if max_q is None:
             raise ValueError("max_q is needed with q_starts")
         max_q = min(max_q, total)
+    if scale is None:
+        scale = 1.0 / math.sqrt(d)
+    elif not 0.0 < scale < math.inf:
+        raise ValueError(f"scale {scale} is not positive and finite")
     device = _require_cuda(q, cache.k_codes, block_table, lengths, q_starts, out)
     if q.stride(2) != 1 or q.stride(0) % 8 or q.stride(1) % 8 or q.stride(1) < d or q.data_ptr() % 16:
         q = q.clone(memory_format=torch.contiguous_format)
@@ -234,7 +238,7 @@ def kv4_attention(
         q.data_ptr(), q.stride(0), q.stride(1), nat.dtype_code(q.dtype), *cache._ptrs, cache.pages, cache.page_size,
         block_table.data_ptr(), block_table.stride(0) if batch > 1 else columns, columns, lengths.data_ptr(),
         q_starts.data_ptr() if q_starts is not None else None, total, max_q, batch, heads, cache.kv_heads, d,
-        1.0 / math.sqrt(d) if scale is None else scale, int(causal), out.data_ptr(), heads * d, _flags(),
+        scale, int(causal), out.data_ptr(), heads * d, _flags(),
         nat.stream_ptr(device))
     nat.check(code, "qtts_kv4_attention")
     return out
