@@ -430,6 +430,7 @@ QTTS_API int qtts_rope_kv4_append(const void* qkv, int64_t ldqkv, int dtype, int
  *   max_q       the most new tokens of any request (bounds the launch)
  *   scale       positive and finite
  *   out         [total_q, q_heads, head_dim] of q's type, token stride given
+ *   workspace   qtts_kv4_attention_workspace() bytes, 16-byte aligned; NULL when 0
  * page_size is a multiple of 16. Scores, softmax statistics and sums are fp32. A
  * length, row range or page number out of its bounds records QTTS_ERR_SHAPE on the
  * device; nothing outside the arrays is read, and that request's output means
@@ -440,8 +441,15 @@ QTTS_API int qtts_kv4_attention(const void* q, int64_t q_token_stride, int64_t q
                                 const void* v_params, int64_t pages, int page_size, const int32_t* block_table,
                                 int64_t ld_table, int table_cols, const int32_t* lengths, const int32_t* q_starts,
                                 int total_q, int max_q, int batch, int q_heads, int kv_heads, int head_dim,
-                                float scale, int causal, void* out, int64_t out_token_stride, unsigned flags,
-                                void* stream);
+                                float scale, int causal, void* out, int64_t out_token_stride, void* workspace,
+                                unsigned flags, void* stream);
+
+/* Bytes of workspace that qtts_kv4_attention needs for these arguments (max_tokens =
+ * table_cols * page_size): 0 for most; where few (request, head) pairs share a long
+ * cache, the parts of its split. Host-only. The call needs nothing of it to start
+ * at any value, and calls that may run at the same time need separate ones. */
+QTTS_API int64_t qtts_kv4_attention_workspace(int total_q, int max_q, int batch, int q_heads, int kv_heads,
+                                              int head_dim, int64_t max_tokens);
 
 /* ---- int8 W8A8 (Int8Method) --------------------------------------------------
  * Per-token int8 quantization of the activations of Int8Method.apply

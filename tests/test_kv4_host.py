@@ -66,9 +66,9 @@ def test_write_refuses(lib, want, kw):
 
 def attend(lib, q=16, qt=16 * 128, qh=128, dtype=nat.BF16, kc=16, kp=16, vc=16, vp=16, pages=4, page=16, table=16,
            ld=2, cols=2, lengths=16, starts=None, total=3, max_q=1, batch=3, heads=16, kv_heads=8, d=128, out=16,
-           ot=16 * 128, scale=0.1):
+           ot=16 * 128, scale=0.1, workspace=None):
     return lib.qtts_kv4_attention(q, qt, qh, dtype, kc, kp, vc, vp, pages, page, table, ld, cols, lengths, starts, total,
-                                  max_q, batch, heads, kv_heads, d, scale, 1, out, ot, 0, None)
+                                  max_q, batch, heads, kv_heads, d, scale, 1, out, ot, workspace, 0, None)
 
 
 @pytest.mark.parametrize("want,kw", [
@@ -93,6 +93,18 @@ def test_valid_arguments_reach_the_device_check(lib):
     assert write(lib) == write(lib, cos=None, sin=None) == write(lib, sections=(24, 20, 20)) == ARCH
     assert write(lib, heads=0, q=None) == ARCH
     assert attend(lib) == attend(lib, starts=16, total=7, max_q=5) == ARCH
+
+
+def test_workspace(lib):
+    def need(total=1, max_q=1, batch=1, heads=16, kv_heads=8, d=128, tokens=64):
+        return lib.qtts_kv4_attention_workspace(total, max_q, batch, heads, kv_heads, d, tokens)
+
+    assert need() == need(total=0) == need(batch=0) == need(heads=12) == 0
+    assert need(total=64, batch=64, tokens=1 << 20) == 0  # many requests: no split across the workspace
+    long = need(tokens=1 << 20)
+    assert long > 0 and long % (16 * (128 + 2) * 4) == 0
+    kw = dict(total=1, batch=1, cols=1 << 16, ld=1 << 16)
+    assert attend(lib, **kw) == NULL and attend(lib, workspace=8, **kw) == ALIGN
 
 
 def cache(**kw):

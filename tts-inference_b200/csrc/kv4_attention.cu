@@ -34,6 +34,8 @@ namespace {
 
 constexpr int kTile = 32;   // tokens a warp takes at a time
 constexpr int kStages = 2;  // tiles in flight a warp
+constexpr int kWarps = 4;   // a CTA
+constexpr int kMaxCluster = 8;
 
 __device__ __forceinline__ uint32_t nib_pair(uint32_t w, int n, uint32_t magic) {
   return ((w >> (4 * n)) & 0x000F000Fu) | magic;
@@ -57,9 +59,9 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
   return r;
 }
 
-__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
   asm volatile(
-      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)),
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
       "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(smem_u32(bar))
       : "memory");
 }
@@ -92,7 +94,7 @@ struct RowsSmem {
 };
 
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(256, NT == 1 ? 2 : 1) kv4_rows_kernel(const Kv4AttnArgs a, int row_blocks,
+__global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 4 : 2) kv4_rows_kernel(const Kv4AttnArgs a, int row_blocks,
                                                                         uint64_t wait_ns) {
   using S = RowsSmem<D>;
   constexpr int NG = D / kKv4Group;
@@ -102,11 +104,11 @@ __global__ void __launch_bounds__(256, NT == 1 ? 2 : 1) kv4_rows_kernel(const Kv
   constexpr float kBaseK = kBf16 ? 128.f : 1024.f;
   constexpr uint32_t kMagicV = 0x43004300u;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ uint64_t full[8][kStages];
-  __shared__ float stat_m[8][kRows], stat_l[8][kRows];  // of each warp
+  __shared__ uint64_t full[kWarps][kStages];
+  __shared__ float stat_m[kWarps][kRows], stat_l[kWarps][kRows];  // of each warp
   __shared__ float part_m[kRows], part_l[kRows];        // of the CTA
 
-  const int warps = blockDim.x >> 5;
+  constexpr int warps = kWarps;
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   const int g = lane >> 2, c = lane & 3;
@@ -140,48 +142,48 @@ __global__ void __launch_bounds__(256, NT == 1 ? 2 : 1) kv4_rows_kernel(const Kv
   const int kmax = r0 >= rows ? 0 : max(0, a.causal ? len - n + last + 1 : len);
   const int tiles = (kmax + kTile - 1) / kTile;
 
-  // This warp's tiles: every (splits * warps)-th one.
+  // This warp's tiles: every (splits * warps)-th one. A tile is one or two runs of tokens that
+  // lie in one page; lane 4 h + x copies run h of array x (key codes, key params, value codes,
+  // value params). Column and row within the page advance without a division, and the page of
+  // the next copy is fetched one copy ahead.
   uint8_t* ring = smem + warp * S::kWarpRing;
   const int step = splits * warps;
   const int t_first = rank * warps + warp;
+  const int run = a.run;                      // 32 or 16 tokens
+  const int per_page = a.cache.page_size / run;
+  const int runs_a_tile = kTile / run;
+  const int xarr = lane & 3, xrun = lane >> 2;
+  const bool copier = xrun < runs_a_tile;
+  const uint8_t* xbase = xarr == 0   ? a.cache.k_codes
+                         : xarr == 1 ? reinterpret_cast<const uint8_t*>(a.cache.k_params)
+                         : xarr == 2 ? a.cache.v_codes
+                                     : reinterpret_cast<const uint8_t*>(a.cache.v_params);
+  const int xrow = (xarr & 1) ? NG * 4 : D / 2;  // bytes a token
+  const uint32_t xdst = smem_u32(ring) + (xarr >= 1 ? S::kCodes : 0) + (xarr >= 2 ? S::kParams : 0) +
+                        (xarr == 3 ? S::kCodes : 0) + xrun * run * xrow;
   const int32_t* table = a.table + b * a.ld_table;
-  auto issue = [&](int tile, int stage) {  // lane 0: the tile's rows, in 16-token runs that lie in one page
-    uint8_t* dst = ring + stage * S::kStage;
-    const int t0 = tile * kTile;
-    const int runs = t0 + 16 < kmax ? 2 : 1;
-    mbar_arrive_expect_tx(&full[warp][stage], static_cast<uint32_t>(runs * (S::kStage / 2)));
-    int64_t row[2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      row[h] = 0;
-      if (h < runs) {
-        const int t = t0 + 16 * h;
-        const int col = t / a.cache.page_size;
-        int64_t page = table[col];
-        if (page < 0 || page >= a.cache.pages) {
-          record_status(QTTS_ERR_SHAPE);
-          page = 0;
-        }
-        row[h] = kv4_row(a.cache, page, kvh, t - col * a.cache.page_size);
+  int at = t_first * runs_a_tile + xrun;  // run number within the request
+  int col = at / per_page, off = at - col * per_page;
+  const int dat = step * runs_a_tile, dcol = dat / per_page, doff = dat - dcol * per_page;
+  int next_page = copier && at * run < kmax ? table[col] : 0;
+  auto issue = [&](int stage) {
+    const bool there = copier && at * run < kmax;
+    const uint32_t parts = __popc(__ballot_sync(0xffffffffu, there && xarr == 0));
+    if (lane == 0) mbar_arrive_expect_tx(&full[warp][stage], parts * static_cast<uint32_t>(run * (S::kStage / kTile)));
+    if (there) {
+      int64_t page = next_page;
+      if (page < 0 || page >= a.cache.pages) {
+        record_status(QTTS_ERR_SHAPE);
+        page = 0;
       }
+      bulk_load(xdst + stage * S::kStage, xbase + kv4_row(a.cache, page, kvh, off * run) * xrow,
+                static_cast<uint32_t>(run * xrow), &full[warp][stage]);
     }
-    const bool joined = runs == 2 && row[1] == row[0] + 16;
-    const int copies = joined ? 1 : runs;
-    for (int h = 0; h < copies; ++h) {
-      const int m = joined ? 2 : 1;
-      const int64_t r = row[h];
-      bulk_load(dst + h * (S::kCodes / 2), a.cache.k_codes + r * (D / 2), m * S::kCodes / 2, &full[warp][stage]);
-      bulk_load(dst + S::kCodes + h * (S::kParams / 2), a.cache.k_params + r * NG, m * S::kParams / 2,
-                &full[warp][stage]);
-      bulk_load(dst + S::kCodes + S::kParams + h * (S::kCodes / 2), a.cache.v_codes + r * (D / 2), m * S::kCodes / 2,
-                &full[warp][stage]);
-      bulk_load(dst + 2 * S::kCodes + S::kParams + h * (S::kParams / 2), a.cache.v_params + r * NG,
-                m * S::kParams / 2, &full[warp][stage]);
-    }
+    at += dat, col += dcol, off += doff;
+    if (off >= per_page) off -= per_page, ++col;
+    if (copier && at * run < kmax) next_page = table[col];
   };
-  if (lane == 0) {
-    for (int s = 0; s < kStages && t_first + s * step < tiles; ++s) issue(t_first + s * step, s);
-  }
+  for (int s = 0; s < kStages && t_first + s * step < tiles; ++s) issue(s);
 
   // q as the B operand: row 8 nt + g, channels 32j + 8c .. + 7 as pairs (i, i + 4); and the
   // sums over each group of the rows 8 nt + 2c, + 1, whose scores this lane holds.
@@ -420,7 +422,7 @@ __global__ void __launch_bounds__(256, NT == 1 ? 2 : 1) kv4_rows_kernel(const Kv
       }
     }
     __syncwarp();
-    if (lane == 0 && tile + kStages * step < tiles) issue(tile + kStages * step, stage);
+    if (tile + kStages * step < tiles) issue(stage);
   }
   if (tile_failed) {  // copies still in flight must land before their memory is used again
     for (int s = 0; s < kStages; ++s) (void)mbar_wait_bounded(&full[warp][(it + s) % kStages], ((it + s) / kStages) & 1, wait_ns);
@@ -458,55 +460,77 @@ __global__ void __launch_bounds__(256, NT == 1 ? 2 : 1) kv4_rows_kernel(const Kv
   }
   __syncthreads();
 
-  // The CTA's warps together; with one CTA that is the answer, else it goes to the cluster.
-  const bool alone = splits == 1;
+  // The CTA's warps together; with one CTA that is the answer, else its part goes to the
+  // cluster or, where more CTAs share a unit than a cluster holds, to the workspace.
+  const int mode = a.parts != nullptr ? 2 : splits > 1 ? 1 : 0;
   float* whole = reinterpret_cast<float*>(smem);  // [kRows][kPitch], in place of warp 0's
-  for (int i = threadIdx.x; i < kRows * (D / 4); i += blockDim.x) {
+  for (int i = threadIdx.x; i < kRows * (D / 4); i += 32 * kWarps) {
     const int r = i / (D / 4), ch = 4 * (i % (D / 4));
+    const int rr = r0 + r;
+    if (rr >= rows) continue;
     float top = -INFINITY;
-    for (int w = 0; w < warps; ++w) top = fmaxf(top, stat_m[w][r]);
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, stat_m[w][r]);
     const float safe = top == -INFINITY ? 0.f : top;
     float lsum = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int w = 0; w < warps; ++w) {
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
       const float f = ex2(stat_m[w][r] - safe);
       const float4 x = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(smem) +
                                                         (w * kRows + r) * S::kPitch + ch);
       lsum += f * stat_l[w][r];
       o.x = fmaf(f, x.x, o.x), o.y = fmaf(f, x.y, o.y), o.z = fmaf(f, x.z, o.z), o.w = fmaf(f, x.w, o.w);
     }
-    if (alone) {
-      const int rr = r0 + r;
-      if (rr < rows) {
-        const float inv = lsum == 0.f ? 0.f : 1.f / lsum;
-        T* dst = static_cast<T*>(a.out) + static_cast<int64_t>(start + rr / share) * a.out_token_stride +
-                 static_cast<int64_t>(kvh * share + rr % share) * D + ch;
-        T v[4] = {from_float<T>(o.x * inv), from_float<T>(o.y * inv), from_float<T>(o.z * inv),
-                  from_float<T>(o.w * inv)};
-        *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<uint2*>(v);
-      }
+    const int64_t orow = static_cast<int64_t>(start + rr / share);
+    const int head = kvh * share + rr % share;
+    if (mode == 0) {
+      const float inv = lsum == 0.f ? 0.f : 1.f / lsum;
+      T v[4] = {from_float<T>(o.x * inv), from_float<T>(o.y * inv), from_float<T>(o.z * inv),
+                from_float<T>(o.w * inv)};
+      *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + orow * a.out_token_stride + head * D + ch) =
+          *reinterpret_cast<uint2*>(v);
+    } else if (mode == 2) {
+      const int64_t at_row = (orow * a.q_heads + head) * splits + rank;
+      *reinterpret_cast<float4*>(a.parts + at_row * D + ch) = o;
+      if (ch == 0) a.stats[at_row] = make_float2(top, lsum);
     } else {
       // Each thread reads exactly the elements of every warp's part that it then overwrites.
       *reinterpret_cast<float4*>(whole + r * S::kPitch + ch) = o;
       if (ch == 0) part_m[r] = top, part_l[r] = lsum;
     }
   }
-  if (alone) return;
+  if (mode != 1) return;
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-  for (int i = rank * blockDim.x + threadIdx.x; i < kRows * D; i += splits * blockDim.x) {
+  for (int i = rank * 32 * kWarps + threadIdx.x; i < kRows * D; i += splits * 32 * kWarps) {
     const int r = i / D, ch = i % D;
     const int rr = r0 + r;
     if (rr < rows) {
       const uint32_t am = smem_u32(&part_m[r]), al = smem_u32(&part_l[r]), ao = smem_u32(&whole[r * S::kPitch + ch]);
+      float pm[kMaxCluster], pl[kMaxCluster], po[kMaxCluster];
       float top = -INFINITY;
-      for (int q = 0; q < splits; ++q) top = fmaxf(top, ld_cluster_f32(mapa_shared(am, q)));
+#pragma unroll
+      for (int q = 0; q < kMaxCluster; ++q) {
+        if (q < splits) {
+          pm[q] = ld_cluster_f32(mapa_shared(am, q));
+          pl[q] = ld_cluster_f32(mapa_shared(al, q));
+          po[q] = ld_cluster_f32(mapa_shared(ao, q));
+        }
+      }
+#pragma unroll
+      for (int q = 0; q < kMaxCluster; ++q) {
+        if (q < splits) top = fmaxf(top, pm[q]);
+      }
       const float safe = top == -INFINITY ? 0.f : top;
       float lsum = 0.f, o = 0.f;
-      for (int q = 0; q < splits; ++q) {
-        const float f = ex2(ld_cluster_f32(mapa_shared(am, q)) - safe);
-        lsum = fmaf(f, ld_cluster_f32(mapa_shared(al, q)), lsum);
-        o = fmaf(f, ld_cluster_f32(mapa_shared(ao, q)), o);
+#pragma unroll
+      for (int q = 0; q < kMaxCluster; ++q) {
+        if (q < splits) {
+          const float f = ex2(pm[q] - safe);
+          lsum = fmaf(f, pl[q], lsum);
+          o = fmaf(f, po[q], o);
+        }
       }
       static_cast<T*>(a.out)[static_cast<int64_t>(start + rr / share) * a.out_token_stride +
                              static_cast<int64_t>(kvh * share + rr % share) * D + ch] =
@@ -518,53 +542,116 @@ __global__ void __launch_bounds__(256, NT == 1 ? 2 : 1) kv4_rows_kernel(const Kv
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-template <typename T, int D, int NT>
-int launch_rows(const Kv4AttnArgs& a, bool pdl, cudaStream_t stream) {
-  const int share = a.q_heads / a.cache.kv_heads;
-  const int64_t rows = static_cast<int64_t>(a.max_q) * share;
-  const int64_t row_blocks = (rows + 8 * NT - 1) / (8 * NT);
-  const int64_t units = row_blocks * a.cache.kv_heads * a.batch;
-  if (row_blocks * a.cache.kv_heads > 65535) return QTTS_ERR_SHAPE;
-  // Warps and CTAs for one unit: as many as give each SM some 16 warps in all, at least
-  // one tile a warp.
-  const int64_t most = static_cast<int64_t>(a.table_cols) * a.cache.page_size;
-  const int64_t tiles = (most + kTile - 1) / kTile;
-  const int warps = tiles > 4 ? 8 : 4;
-  int splits = 1;
-  while (splits < 16 && 2 * splits * warps <= tiles && units * splits * warps < 16 * kNumSMs) splits *= 2;
-  using S = RowsSmem<D>;
-  const size_t ring = static_cast<size_t>(warps) * S::kWarpRing;
-  const size_t part = static_cast<size_t>(warps) * 8 * NT * S::kPitch * 4;
-  const size_t smem = ring > part ? ring : part;
-  auto kern = kv4_rows_kernel<T, D, NT>;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) != cudaSuccess ||
-      (splits > 8 && cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)) {
+// The parts of each (token, head) row from the workspace, one warp a row.
+template <typename T, int D>
+__global__ void __launch_bounds__(128) kv4_join_kernel(const Kv4AttnArgs a, int splits) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int lane = threadIdx.x & 31;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
+  if (row >= static_cast<int64_t>(a.total_q) * a.q_heads) return;
+  const float2* st = a.stats + row * splits;
+  float top = -INFINITY;
+  for (int q = lane; q < splits; q += 32) top = fmaxf(top, st[q].x);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  const float safe = top == -INFINITY ? 0.f : top;
+  float lsum = 0.f, out[D / 32] = {};
+  const float* part = a.parts + row * splits * D + lane * (D / 32);
+#pragma unroll 4
+  for (int q = 0; q < splits; ++q) {
+    const float2 s = st[q];
+    const float f = ex2(s.x - safe);
+    lsum = fmaf(f, s.y, lsum);
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) out[i] = fmaf(f, part[static_cast<int64_t>(q) * D + i], out[i]);
+  }
+  const float inv = lsum == 0.f ? 0.f : 1.f / lsum;
+  T* dst = static_cast<T*>(a.out) + row / a.q_heads * a.out_token_stride + row % a.q_heads * D + lane * (D / 32);
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) dst[i] = from_float<T>(out[i] * inv);
+}
+
+// How a call is laid out: rows a CTA, and CTAs that share the tokens of one (request, key
+// head, row block).
+struct RowsPlan {
+  int nt;
+  int64_t row_blocks;
+  int splits;
+};
+
+RowsPlan plan_rows(int64_t max_q, int share, int kv_heads, int batch, int64_t most_tokens) {
+  RowsPlan p;
+  const int64_t rows = max_q * share;
+  p.nt = rows <= 8 ? 1 : 2;
+  p.row_blocks = (rows + 8 * p.nt - 1) / (8 * p.nt);
+  const int64_t units = p.row_blocks * kv_heads * batch;
+  // One wave of CTAs (four of 128 threads an SM; two with 16 rows, for their registers), at
+  // least one tile a warp.
+  const int64_t wave = static_cast<int64_t>(kNumSMs) * (p.nt == 1 ? 4 : 2);
+  const int64_t tiles = (most_tokens + kTile - 1) / kTile;
+  const int64_t want = wave / (units > 0 ? units : 1);
+  const int64_t can = (tiles + kWarps - 1) / kWarps;
+  int64_t s = want < can ? want : can;
+  p.splits = static_cast<int>(s < 1 ? 1 : s > 256 ? 256 : s);
+  return p;
+}
+
+template <typename KernT, typename... Args>
+int launch(KernT kern, dim3 grid, int threads, size_t smem, int cluster, bool pdl, cudaStream_t stream, Args... args) {
+  if (smem > 48 * 1024 &&
+      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) != cudaSuccess) {
     (void)cudaGetLastError();
     return QTTS_ERR_LAUNCH;
   }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(splits, static_cast<unsigned>(row_blocks * a.cache.kv_heads), a.batch);
-  cfg.blockDim = dim3(32 * warps);
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = splits;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  int n = 0;
+  if (cluster > 1) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = cluster;
+    attr[n].val.clusterDim.y = 1;
+    attr[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  if (pdl) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n].val.programmaticStreamSerializationAllowed = 1;
+    ++n;
+  }
   cfg.attrs = attr;
-  cfg.numAttrs = pdl ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, kern, a, static_cast<int>(row_blocks), current_wait_limit_ns()) == cudaSuccess
-             ? QTTS_OK
-             : QTTS_ERR_LAUNCH;
+  cfg.numAttrs = n;
+  return cudaLaunchKernelEx(&cfg, kern, args...) == cudaSuccess ? QTTS_OK : QTTS_ERR_LAUNCH;
+}
+
+template <typename T, int D, int NT>
+int launch_rows(Kv4AttnArgs a, const RowsPlan& p, bool pdl, cudaStream_t stream) {
+  using S = RowsSmem<D>;
+  constexpr size_t kRing = static_cast<size_t>(kWarps) * S::kWarpRing;
+  constexpr size_t kPart = static_cast<size_t>(kWarps) * 8 * NT * S::kPitch * 4;
+  constexpr size_t kSmem = kRing > kPart ? kRing : kPart;
+  const bool workspace = p.splits > kMaxCluster;
+  if (!workspace) a.parts = nullptr, a.stats = nullptr;
+  const int r = launch(kv4_rows_kernel<T, D, NT>,
+                       dim3(p.splits, static_cast<unsigned>(p.row_blocks * a.cache.kv_heads), a.batch), 32 * kWarps,
+                       kSmem, workspace ? 1 : p.splits, pdl, stream, a, static_cast<int>(p.row_blocks),
+                       current_wait_limit_ns());
+  if (r != QTTS_OK || !workspace) return r;
+  const int64_t rows = static_cast<int64_t>(a.total_q) * a.q_heads;
+  return launch(kv4_join_kernel<T, D>, dim3(static_cast<unsigned>((rows + 3) / 4)), 128, 0, 1, true, stream, a,
+                p.splits);
 }
 
 template <typename T, int D>
 int launch_ka(const Kv4AttnArgs& a, bool pdl, cudaStream_t stream) {
-  const int64_t rows = static_cast<int64_t>(a.max_q) * (a.q_heads / a.cache.kv_heads);
-  return rows <= 8 ? launch_rows<T, D, 1>(a, pdl, stream) : launch_rows<T, D, 2>(a, pdl, stream);
+  const RowsPlan p = plan_rows(a.max_q, a.q_heads / a.cache.kv_heads, a.cache.kv_heads, a.batch,
+                               static_cast<int64_t>(a.table_cols) * a.cache.page_size);
+  if (p.row_blocks * a.cache.kv_heads > 65535) return QTTS_ERR_SHAPE;
+  return p.nt == 1 ? launch_rows<T, D, 1>(a, p, pdl, stream) : launch_rows<T, D, 2>(a, p, pdl, stream);
 }
 
 }  // namespace
@@ -579,13 +666,22 @@ int launch_kv4_attention(const Kv4AttnArgs& a, int dtype, int head_dim, bool pdl
 
 }  // namespace qtts
 
+extern "C" int64_t qtts_kv4_attention_workspace(int total_q, int max_q, int batch, int q_heads, int kv_heads,
+                                                int head_dim, int64_t max_tokens) {
+  using namespace qtts;
+  if (total_q < 1 || max_q < 1 || batch < 1 || kv_heads < 1 || q_heads < 1 || q_heads % kv_heads != 0) return 0;
+  const RowsPlan p = plan_rows(max_q, q_heads / kv_heads, kv_heads, batch, max_tokens);
+  if (p.splits <= kMaxCluster) return 0;
+  return static_cast<int64_t>(total_q) * q_heads * p.splits * (head_dim + 2) * 4;
+}
+
 extern "C" int qtts_kv4_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, int dtype,
                                   const uint8_t* k_codes, const void* k_params, const uint8_t* v_codes,
                                   const void* v_params, int64_t pages, int page_size, const int32_t* block_table,
                                   int64_t ld_table, int table_cols, const int32_t* lengths, const int32_t* q_starts,
                                   int total_q, int max_q, int batch, int q_heads, int kv_heads, int head_dim,
-                                  float scale, int causal, void* out, int64_t out_token_stride, unsigned flags,
-                                  void* stream) {
+                                  float scale, int causal, void* out, int64_t out_token_stride, void* workspace,
+                                  unsigned flags, void* stream) {
   using namespace qtts;
   if (batch < 0 || batch > 65535 || total_q < 0 || max_q < 0 || max_q > total_q) return QTTS_ERR_SHAPE;
   if (q_heads < 1 || kv_heads < 1 || q_heads % kv_heads != 0 || q_heads > 4096) return QTTS_ERR_SHAPE;
@@ -613,6 +709,10 @@ extern "C" int qtts_kv4_attention(const void* q, int64_t q_token_stride, int64_t
       !al(lengths, 4) || !al(q_starts, 4)) {
     return QTTS_ERR_ALIGN;
   }
+  const int64_t need = qtts_kv4_attention_workspace(total_q, max_q, batch, q_heads, kv_heads, head_dim,
+                                                    static_cast<int64_t>(table_cols) * page_size);
+  if (need > 0 && workspace == nullptr) return QTTS_ERR_NULL;
+  if (need > 0 && !al(workspace, 16)) return QTTS_ERR_ALIGN;
   const int dev_ok = check_device();
   if (dev_ok != QTTS_OK) return dev_ok;
   Kv4AttnArgs a{};
@@ -635,5 +735,10 @@ extern "C" int qtts_kv4_attention(const void* q, int64_t q_token_stride, int64_t
   a.causal = causal;
   a.out = out;
   a.out_token_stride = out_token_stride;
+  a.run = page_size % kTile == 0 ? kTile : 16;
+  if (need > 0) {
+    a.parts = static_cast<float*>(workspace);
+    a.stats = reinterpret_cast<float2*>(a.parts + need / ((head_dim + 2) * 4) * head_dim);
+  }
   return launch_kv4_attention(a, dtype, head_dim, (flags & QTTS_FLAG_PDL) != 0, static_cast<cudaStream_t>(stream));
 }

@@ -123,9 +123,10 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "qtts_kv4_attention": (
         _c_int,
         [_c_vp, _c_i64, _c_i64, _c_int, _c_vp, _c_vp, _c_vp, _c_vp, _c_i64, _c_int, _c_vp, _c_i64, _c_int, _c_vp,
-         _c_vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, ctypes.c_float, _c_int, _c_vp, _c_i64, _c_uint,
-         _c_vp],
+         _c_vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, ctypes.c_float, _c_int, _c_vp, _c_i64, _c_vp,
+         _c_uint, _c_vp],
     ),
+    "qtts_kv4_attention_workspace": (_c_i64, [_c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_i64]),
     "qtts_w8a16_gemm_prologue_fused": (_c_int, [_c_int, _c_int, _c_int, _c_int, _c_int]),
     "qtts_fp8_linear_noalloc": (
         _c_int,

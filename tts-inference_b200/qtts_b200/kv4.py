@@ -234,11 +234,14 @@ def kv4_attention(
     elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
         raise ValueError(f"out must be a contiguous {q.dtype} {tuple(q.shape)}")
     columns = block_table.shape[1]
+    need = nat.lib().qtts_kv4_attention_workspace(total, max_q, batch, heads, cache.kv_heads, d,
+                                                  columns * cache.page_size)
+    workspace = torch.empty(need, device=device, dtype=torch.uint8) if need else None
     code = nat.lib().qtts_kv4_attention(
         q.data_ptr(), q.stride(0), q.stride(1), nat.dtype_code(q.dtype), *cache._ptrs, cache.pages, cache.page_size,
         block_table.data_ptr(), block_table.stride(0) if batch > 1 else columns, columns, lengths.data_ptr(),
         q_starts.data_ptr() if q_starts is not None else None, total, max_q, batch, heads, cache.kv_heads, d,
-        scale, int(causal), out.data_ptr(), heads * d, _flags(),
-        nat.stream_ptr(device))
+        scale, int(causal), out.data_ptr(), heads * d,
+        workspace.data_ptr() if need else None, _flags(), nat.stream_ptr(device))
     nat.check(code, "qtts_kv4_attention")
     return out
