@@ -8,17 +8,21 @@
 // cache once, 0.625 bytes an element, and almost as much the instructions that
 // turn nibbles into matrix operands, so those are kept few:
 //   * scores as S^T = K q^T with mma.sync m16n8k16: 16 tokens by 8 rows, a row
-//     being a (new token, query head) pair that shares the key head. A nibble is
-//     ORed into the mantissa of a power of two (128 + code in bf16, 1024 + code in
-//     fp16: exact); the accumulator starts at minus that power times the sum of
-//     the row's q over the group, so it ends as sum(q * code), and the group's
-//     scale and minimum enter once per (token, row, group), in fp32;
+//     being a (new token, query head) pair that shares the key head. A nibble
+//     masked out of a word is an fp16 subnormal as it stands, code * 2^-24 in bits
+//     0..3 and code * 2^-20 in bits 4..7, both exact: four masks and one shift
+//     make four operand pairs. q is brought to fp16 by a power of two per row
+//     (largest magnitude in [2^14, 2^15): exact for bf16 down to 2^-24 of it) and
+//     the channels of the higher nibbles by 2^-4 more. The group's scale and
+//     minimum enter once per (token, row, group), in fp32;
 //   * out^T = V^T P^T: two tokens' half-words are interleaved by a byte permute, so
-//     a nibble mask again gives operand pairs. The probability times the value's
-//     scale is what is rounded to bf16; sum p (code - 8) scale + p (minimum + 8 scale)
-//     keeps the rounded part as small as the values themselves. The 128 + 8 is
-//     taken out with one more product per group by a constant row of -136 with the
-//     same rounded probabilities, exactly as it went in;
+//     the same masks again give operand pairs, and one fp16 fused multiply-add
+//     makes a pair the value itself, rounded once: code * scale + minimum, in units
+//     of a power of two that follows the largest scale the warp has met (that scale
+//     becomes 2^14..2^15 against the code's 2^-24, so a value keeps 11 bits, or 2^-15
+//     of that scale where it is smaller). Scale and minimum of a tile are
+//     brought to those units once, a word a lane, through shared memory.
+//     Probabilities are fp16 too, times 2^15 so that the small ones stay normal;
 //   * every warp streams its own tiles of 32 tokens through a ring of bulk copies
 //     and keeps its own running maximum and sum; the warps of a CTA meet in shared
 //     memory, and where there are few (request, head) pairs a cluster of up to 16
@@ -37,9 +41,9 @@ constexpr int kStages = 2;  // tiles in flight a warp
 constexpr int kWarps = 4;   // a CTA
 constexpr int kMaxCluster = 8;
 
-__device__ __forceinline__ uint32_t nib_pair(uint32_t w, int n, uint32_t magic) {
-  return ((w >> (4 * n)) & 0x000F000Fu) | magic;
-}
+// Nibbles n and n + 4 (n = 0, 1) of a word as a pair of fp16 subnormals: code * 2^-24 for
+// n = 0, code * 2^-20 for n = 1; nibbles n + 2 and n + 6 from the word shifted by eight.
+__device__ __forceinline__ uint32_t nib_pair(uint32_t w, int n) { return w & (n ? 0x00F000F0u : 0x000F000Fu); }
 
 __device__ __forceinline__ float ex2(float x) {
   float r;
@@ -47,11 +51,22 @@ __device__ __forceinline__ float ex2(float x) {
   return r;
 }
 
-__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   uint32_t r;
-  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
+__device__ __forceinline__ uint32_t fma_f16x2(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t r;
+  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+  return r;
+}
+__device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ float exp2_int(int e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
 
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
   uint32_t r;
@@ -99,12 +114,9 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 4 : 2) kv4_rows_kernel(
   using S = RowsSmem<D>;
   constexpr int NG = D / kKv4Group;
   constexpr int kRows = 8 * NT;
-  constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
-  constexpr uint32_t kMagicK = kBf16 ? 0x43004300u : 0x64006400u;
-  constexpr float kBaseK = kBf16 ? 128.f : 1024.f;
-  constexpr uint32_t kMagicV = 0x43004300u;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint64_t full[kWarps][kStages];
+  __shared__ __align__(16) uint32_t vparam[kWarps][kTile * NG];  // value scales and minima of a tile, fp16
   __shared__ float stat_m[kWarps][kRows], stat_l[kWarps][kRows];  // of each warp
   __shared__ float part_m[kRows], part_l[kRows];        // of the CTA
 
@@ -186,31 +198,47 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 4 : 2) kv4_rows_kernel(
   for (int s = 0; s < kStages && t_first + s * step < tiles; ++s) issue(s);
 
   // q as the B operand: row 8 nt + g, channels 32j + 8c .. + 7 as pairs (i, i + 4); and the
-  // sums over each group of the rows 8 nt + 2c, + 1, whose scores this lane holds.
+  // sums over each group of the rows 8 nt + 2c, + 1, whose scores this lane holds, in the
+  // same units. to_log2: from those units to the exponent of two.
   uint32_t qf[NT][NG][4];
-  float qsum[NT][NG][2];
+  float qsum[NT][NG][2], to_log2[NT][2];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     const int r = r0 + 8 * nt + g;
     const T* qr = static_cast<const T*>(a.q) + static_cast<int64_t>(start + r / share) * a.q_token_stride +
                   (kvh * share + r % share) * a.q_head_stride + 8 * c;
+    float x[NG][8];
+    float top = 0.f;
 #pragma unroll
     for (int j = 0; j < NG; ++j) {
       uint4 u = make_uint4(0u, 0u, 0u, 0u);
       if (r < rows) u = *reinterpret_cast<const uint4*>(qr + 32 * j);
-      qf[nt][j][0] = __byte_perm(u.x, u.z, 0x5410);
-      qf[nt][j][1] = __byte_perm(u.x, u.z, 0x7632);
-      qf[nt][j][2] = __byte_perm(u.y, u.w, 0x5410);
-      qf[nt][j][3] = __byte_perm(u.y, u.w, 0x7632);
       const T* e = reinterpret_cast<const T*>(&u);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[j][i] = to_float(e[i]), top = fmaxf(top, fabsf(x[j][i]));
+    }
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    const int e = min(100, max(-100, 14 + 127 - static_cast<int>(__float_as_uint(top) >> 23)));
+    const float up = exp2_int(e);
+#pragma unroll
+    for (int j = 0; j < NG; ++j) {
       float sum = 0.f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) sum += to_float(e[i]);
+      for (int i = 0; i < 8; ++i) x[j][i] *= up, sum += x[j][i];
+      qf[nt][j][0] = pack_f16(x[j][0], x[j][4]);
+      qf[nt][j][1] = pack_f16(0.0625f * x[j][1], 0.0625f * x[j][5]);
+      qf[nt][j][2] = pack_f16(x[j][2], x[j][6]);
+      qf[nt][j][3] = pack_f16(0.0625f * x[j][3], 0.0625f * x[j][7]);
       sum += __shfl_xor_sync(0xffffffffu, sum, 1);
       sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+      sum *= 0x1p-24f;
       qsum[nt][j][0] = __shfl_sync(0xffffffffu, sum, (2 * c) * 4);
       qsum[nt][j][1] = __shfl_sync(0xffffffffu, sum, (2 * c + 1) * 4);
     }
+    const float back = a.scale * 1.4426950408889634f * exp2_int(24 - e);
+    to_log2[nt][0] = __shfl_sync(0xffffffffu, back, (2 * c) * 4);
+    to_log2[nt][1] = __shfl_sync(0xffffffffu, back, (2 * c + 1) * 4);
   }
   int lim[NT][2];
 #pragma unroll
@@ -221,21 +249,15 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 4 : 2) kv4_rows_kernel(
       lim[nt][e] = a.causal ? min(len - n + i + 1, kmax) : len;
     }
   }
-  const float to_log2 = a.scale * 1.4426950408889634f;
 
-  float m[NT][2], l[NT][2], zacc[NT][NG][2];
-  float acc[NT][NG][2][4];  // [group][channel pair] of out^T, fp32
-  float csum[NT][4];        // row j: -136 * sum of the rounded probabilities * scale of group j
+  float m[NT][2], l[NT][2];
+  float acc[NT][NG][2][4];  // [group][channel pair] of out^T, fp32, in units of 2^(vexp - 127 + 10)
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
     for (int e = 0; e < 2; ++e) m[nt][e] = -INFINITY, l[nt][e] = 0.f;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) csum[nt][e] = 0.f;
-#pragma unroll
     for (int j = 0; j < NG; ++j) {
-#pragma unroll
-      for (int e = 0; e < 2; ++e) zacc[nt][j][e] = 0.f;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
 #pragma unroll
@@ -243,29 +265,93 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 4 : 2) kv4_rows_kernel(
       }
     }
   }
+  // Unit of the values: 2^(vexp - 127 + 10), vexp the exponent field of the largest value scale
+  // so far (or of the largest minimum / 2^20, where that is more: both have to stay in fp16's
+  // range). What reaches vlimit moves it.
+  int vexp = 0;
+  float vlimit = 0.f;
+  float vunit = 0.f;  // 2^(127 - vexp)
 
   // Token of row slot s of a 16-token operand: s with the last bit turned in every other
   // pair, so that neither the key nor the value loads below hit one bank with more than two rows.
   const int kslot = g ^ ((g >> 1) & 1);
   const int v0 = (2 * c) ^ (c & 1), v1 = (2 * c + 1) ^ (c & 1);
 
-  int it = 0;
-  bool tile_failed = false;
-  for (int tile = t_first; tile < tiles; tile += step, ++it) {
-    const int stage = it % kStages;
-    const bool got = mbar_wait_bounded(&full[warp][stage], (it / kStages) & 1, wait_ns);
-    if (!__all_sync(0xffffffffu, got)) {
-      if (lane == 0) record_status(QTTS_ERR_TIMEOUT);
-      tile_failed = true;
-      break;
+  auto load_params = [&](const void* p, int t, uint32_t(&w)[NG]) {
+    if constexpr (NG == 4) {
+      *reinterpret_cast<uint4*>(w) = static_cast<const uint4*>(p)[t];
+    } else {
+      *reinterpret_cast<uint2*>(w) = static_cast<const uint2*>(p)[t];
     }
-    const uint8_t* kc = ring + stage * S::kStage;
+  };
+
+  // One tile. kMasked: some row of the block does not see all of it.
+  auto attend = [&](const uint8_t* kc, int t0, auto masked) {
+    constexpr bool kMasked = decltype(masked)::value;
     const uint8_t* kp = kc + S::kCodes;
     const uint8_t* vc = kp + S::kParams;
     const uint8_t* vp = vc + S::kCodes;
-    const int t0 = tile * kTile;
 
-    // Scores of 2 x 16 tokens: s[nt][mt][token half][row of the pair].
+    // This tile's value scales and minima to fp16, NG words a lane.
+    float vs[NG], vz[NG];
+    float top = 0.f;
+    uint32_t bad = 0;  // masked tiles: tokens with a non-finite scale or minimum
+#pragma unroll
+    for (int k = 0; k < NG; ++k) {
+      const int i = lane + 32 * k;
+      uint32_t w = reinterpret_cast<const uint32_t*>(vp)[i];
+      if constexpr (kMasked) {  // beyond the request's tokens the cache holds anything
+        if (t0 + i / NG >= kmax) w = 0u;
+        const bool nf = (w & 0x7F80u) == 0x7F80u || (w & 0x7F800000u) == 0x7F800000u;
+        const uint32_t who = __ballot_sync(0xffffffffu, nf);
+        if (who != 0) {
+          for (int t = 0; t < 32 / NG; ++t) {
+            if (who >> (t * NG) & ((1u << NG) - 1u)) bad |= 1u << (k * (32 / NG) + t);
+          }
+        }
+      }
+      vs[k] = kv4_scale(w), vz[k] = kv4_min(w);
+    }
+    if constexpr (kMasked) {
+      // Rows that do not see such a token must not meet it (0 * NaN): its values become
+      // zeros here and its score NaN below, for the rows that do see it.
+#pragma unroll
+      for (int k = 0; k < NG; ++k) {
+        if (bad >> ((lane + 32 * k) / NG) & 1u) vs[k] = vz[k] = 0.f;
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < NG; ++k) top = fmaxf(top, fmaxf(vs[k], fabsf(vz[k]) * 0x1p-20f));
+    if (__any_sync(0xffffffffu, !(top < vlimit))) {
+      float most = 0.f;  // of the finite ones; others reach the output as they are
+#pragma unroll
+      for (int k = 0; k < NG; ++k) {
+        const float x = fmaxf(vs[k], fabsf(vz[k]) * 0x1p-20f);
+        most = fmaxf(most, x < INFINITY ? x : 0.f);
+      }
+      most = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most)));
+      if (!(most < vlimit)) {
+        const int to = min(253, max(16, static_cast<int>(__float_as_uint(most) >> 23)));
+        const float f = vlimit == 0.f ? 1.f : exp2_int(max(-126, vexp - to));
+        vexp = to;
+        vlimit = exp2_int(to - 126);
+        vunit = exp2_int(127 - to);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+          for (int j = 0; j < NG; ++j) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[nt][j][0][e] *= f, acc[nt][j][1][e] *= f;
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < NG; ++k) {
+      vparam[warp][lane + 32 * k] = pack_f16(vs[k] * vunit * 0x1p14f, vz[k] * vunit * 0x1p-10f);
+    }
+
+    // Scores of 2 x 16 tokens: s[nt][mt][2 * token half + row of the pair].
     float s[NT][2][4];
 #pragma unroll
     for (int mt = 0; mt < 2; ++mt) {
@@ -275,11 +361,10 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 4 : 2) kv4_rows_kernel(
         const int t = 16 * mt + 8 * h + kslot;
         if constexpr (NG == 4) {
           *reinterpret_cast<uint4*>(kw[h]) = *reinterpret_cast<const uint4*>(kc + t * 64 + 16 * c);
-          *reinterpret_cast<uint4*>(pw[h]) = *reinterpret_cast<const uint4*>(kp + t * 16);
         } else {
           *reinterpret_cast<uint2*>(kw[h]) = *reinterpret_cast<const uint2*>(kc + t * 32 + 8 * c);
-          *reinterpret_cast<uint2*>(pw[h]) = *reinterpret_cast<const uint2*>(kp + t * 8);
         }
+        load_params(kp, t, pw[h]);
       }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
@@ -288,20 +373,17 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 4 : 2) kv4_rows_kernel(
       }
 #pragma unroll
       for (int j = 0; j < NG; ++j) {
-        uint32_t a0[4], a1[4];
-        a0[0] = nib_pair(kw[0][j], 0, kMagicK), a0[1] = nib_pair(kw[1][j], 0, kMagicK);
-        a0[2] = nib_pair(kw[0][j], 1, kMagicK), a0[3] = nib_pair(kw[1][j], 1, kMagicK);
-        a1[0] = nib_pair(kw[0][j], 2, kMagicK), a1[1] = nib_pair(kw[1][j], 2, kMagicK);
-        a1[2] = nib_pair(kw[0][j], 3, kMagicK), a1[3] = nib_pair(kw[1][j], 3, kMagicK);
+        const uint32_t h0 = kw[0][j] >> 8, h1 = kw[1][j] >> 8;
+        const uint32_t a0[4] = {nib_pair(kw[0][j], 0), nib_pair(kw[1][j], 0), nib_pair(kw[0][j], 1),
+                                nib_pair(kw[1][j], 1)};
+        const uint32_t a1[4] = {nib_pair(h0, 0), nib_pair(h1, 0), nib_pair(h0, 1), nib_pair(h1, 1)};
         const float sc0 = kv4_scale(pw[0][j]), sc1 = kv4_scale(pw[1][j]);
         const float z0 = kv4_min(pw[0][j]), z1 = kv4_min(pw[1][j]);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          float d[4];
-          d[0] = d[2] = -kBaseK * qsum[nt][j][0];
-          d[1] = d[3] = -kBaseK * qsum[nt][j][1];
-          Mma16816<T>::run(d, a0, qf[nt][j][0], qf[nt][j][1]);
-          Mma16816<T>::run(d, a1, qf[nt][j][2], qf[nt][j][3]);
+          float d[4] = {0.f, 0.f, 0.f, 0.f};
+          Mma16816<__half>::run(d, a0, qf[nt][j][0], qf[nt][j][1]);
+          Mma16816<__half>::run(d, a1, qf[nt][j][2], qf[nt][j][3]);
           s[nt][mt][0] = fmaf(sc0, d[0], fmaf(z0, qsum[nt][j][0], s[nt][mt][0]));
           s[nt][mt][1] = fmaf(sc0, d[1], fmaf(z0, qsum[nt][j][1], s[nt][mt][1]));
           s[nt][mt][2] = fmaf(sc1, d[2], fmaf(z1, qsum[nt][j][0], s[nt][mt][2]));
@@ -309,8 +391,7 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 4 : 2) kv4_rows_kernel(
         }
       }
     }
-    const bool masked = t0 + kTile > first_lim;  // some row does not see all of the tile
-    if (masked) {
+    if constexpr (kMasked) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -318,13 +399,14 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 4 : 2) kv4_rows_kernel(
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int t = t0 + 16 * mt + 8 * (e >> 1) + kslot;
+            if (bad >> (t - t0) & 1u) s[nt][mt][e] = NAN;
             if (t >= lim[nt][e & 1]) s[nt][mt][e] = -INFINITY;
           }
         }
       }
     }
 
-    // Running maximum (in units of log2) and sum; p replaces s.
+    // Running maximum (exponent of two) and sum; p replaces s.
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       float mx[2];
@@ -337,89 +419,92 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 4 : 2) kv4_rows_kernel(
         mx[0] = fmaxf(mx[0], __shfl_xor_sync(0xffffffffu, mx[0], o));
         mx[1] = fmaxf(mx[1], __shfl_xor_sync(0xffffffffu, mx[1], o));
       }
-      // scale > 0: the largest score stays the largest.
-      mx[0] = fmaxf(m[nt][0], mx[0] * to_log2);
-      mx[1] = fmaxf(m[nt][1], mx[1] * to_log2);
-      const bool moved = mx[0] > m[nt][0] || mx[1] > m[nt][1];
-      if (__any_sync(0xffffffffu, moved)) {
+      // to_log2 > 0: the largest score stays the largest.
+      mx[0] = fmaxf(m[nt][0], mx[0] * to_log2[nt][0]);
+      mx[1] = fmaxf(m[nt][1], mx[1] * to_log2[nt][1]);
+      if (__any_sync(0xffffffffu, mx[0] > m[nt][0] || mx[1] > m[nt][1])) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const float f = mx[e] > m[nt][e] ? ex2(m[nt][e] - mx[e]) : 1.f;
           m[nt][e] = mx[e];
           l[nt][e] *= f;
-          csum[nt][e] *= f;
 #pragma unroll
           for (int j = 0; j < NG; ++j) {
-            zacc[nt][j][e] *= f;
             acc[nt][j][0][e] *= f, acc[nt][j][0][e + 2] *= f;
             acc[nt][j][1][e] *= f, acc[nt][j][1][e + 2] *= f;
           }
         }
       }
-      const float m0 = m[nt][0] == -INFINITY ? 0.f : m[nt][0];
-      const float m1 = m[nt][1] == -INFINITY ? 0.f : m[nt][1];
+      const float m0 = 15.f - (kMasked && m[nt][0] == -INFINITY ? 0.f : m[nt][0]);
+      const float m1 = 15.f - (kMasked && m[nt][1] == -INFINITY ? 0.f : m[nt][1]);
 #pragma unroll
       for (int mt = 0; mt < 2; ++mt) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          s[nt][mt][e] = ex2(fmaf(s[nt][mt][e], to_log2, -((e & 1) ? m1 : m0)));
+          s[nt][mt][e] = ex2(fmaf(s[nt][mt][e], to_log2[nt][e & 1], (e & 1) ? m1 : m0));
           l[nt][e & 1] += s[nt][mt][e];
         }
       }
     }
 
     // Weighted values.
+    __syncwarp();  // vparam
 #pragma unroll
     for (int mt = 0; mt < 2; ++mt) {
-      uint32_t vw[4][NG / 2], pw[2][NG];
+      uint32_t vw[4][NG / 2], pw[4][NG];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int ta = 16 * mt + 8 * h + v0, tb = 16 * mt + 8 * h + v1, tp = 16 * mt + 8 * h + kslot;
+      for (int h = 0; h < 4; ++h) {
+        const int t = 16 * mt + 8 * (h >> 1) + ((h & 1) ? v1 : v0);
         if constexpr (NG == 4) {
-          *reinterpret_cast<uint2*>(vw[2 * h]) = *reinterpret_cast<const uint2*>(vc + ta * 64 + 8 * g);
-          *reinterpret_cast<uint2*>(vw[2 * h + 1]) = *reinterpret_cast<const uint2*>(vc + tb * 64 + 8 * g);
-          *reinterpret_cast<uint4*>(pw[h]) = *reinterpret_cast<const uint4*>(vp + tp * 16);
+          *reinterpret_cast<uint2*>(vw[h]) = *reinterpret_cast<const uint2*>(vc + t * 64 + 8 * g);
         } else {
-          vw[2 * h][0] = *reinterpret_cast<const uint32_t*>(vc + ta * 32 + 4 * g);
-          vw[2 * h + 1][0] = *reinterpret_cast<const uint32_t*>(vc + tb * 32 + 4 * g);
-          *reinterpret_cast<uint2*>(pw[h]) = *reinterpret_cast<const uint2*>(vp + tp * 8);
+          vw[h][0] = *reinterpret_cast<const uint32_t*>(vc + t * 32 + 4 * g);
         }
+        load_params(vparam[warp], t, pw[h]);
+      }
+      uint32_t b0[NT], b1[NT];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        b0[nt] = transpose8x8(pack_f16(s[nt][mt][0], s[nt][mt][1]));
+        b1[nt] = transpose8x8(pack_f16(s[nt][mt][2], s[nt][mt][3]));
       }
 #pragma unroll
       for (int j = 0; j < NG; ++j) {
         // Tokens (2c, 2c + 1) and (2c + 8, 2c + 9) of group j, interleaved by half-words.
         const uint32_t xa = __byte_perm(vw[0][j / 2], vw[1][j / 2], (j & 1) ? 0x7632 : 0x5410);
         const uint32_t xb = __byte_perm(vw[2][j / 2], vw[3][j / 2], (j & 1) ? 0x7632 : 0x5410);
-        uint32_t a0[4], a1[4];
-        a0[0] = nib_pair(xa, 0, kMagicV), a0[1] = nib_pair(xa, 1, kMagicV);
-        a0[2] = nib_pair(xb, 0, kMagicV), a0[3] = nib_pair(xb, 1, kMagicV);
-        a1[0] = nib_pair(xa, 2, kMagicV), a1[1] = nib_pair(xa, 3, kMagicV);
-        a1[2] = nib_pair(xb, 2, kMagicV), a1[3] = nib_pair(xb, 3, kMagicV);
-        const uint32_t bias = g == j ? 0xC308C308u : 0u;  // (-136, -136)
-        const uint32_t ab[4] = {bias, 0u, bias, 0u};
-        const float sc0 = kv4_scale(pw[0][j]), sc1 = kv4_scale(pw[1][j]);
-        const float z0 = fmaf(8.f, sc0, kv4_min(pw[0][j])), z1 = fmaf(8.f, sc1, kv4_min(pw[1][j]));
+        const uint32_t ya = xa >> 8, yb = xb >> 8;
+        const uint32_t sa = __byte_perm(pw[0][j], pw[1][j], 0x5410), za = __byte_perm(pw[0][j], pw[1][j], 0x7632);
+        const uint32_t sb = __byte_perm(pw[2][j], pw[3][j], 0x5410), zb = __byte_perm(pw[2][j], pw[3][j], 0x7632);
+        const uint32_t sa4 = mul_f16x2(sa, 0x2C002C00u), sb4 = mul_f16x2(sb, 0x2C002C00u);  // / 16
+        const uint32_t a0[4] = {fma_f16x2(nib_pair(xa, 0), sa, za), fma_f16x2(nib_pair(xa, 1), sa4, za),
+                                fma_f16x2(nib_pair(xb, 0), sb, zb), fma_f16x2(nib_pair(xb, 1), sb4, zb)};
+        const uint32_t a1[4] = {fma_f16x2(nib_pair(ya, 0), sa, za), fma_f16x2(nib_pair(ya, 1), sa4, za),
+                                fma_f16x2(nib_pair(yb, 0), sb, zb), fma_f16x2(nib_pair(yb, 1), sb4, zb)};
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          const float* p = s[nt][mt];
-          float w[4] = {p[0] * sc0, p[1] * sc0, p[2] * sc1, p[3] * sc1};
-          float y[4] = {p[0] * z0, p[1] * z0, p[2] * z1, p[3] * z1};
-          if (masked) {  // what a row does not see stays out even where it is NaN
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              w[e] = p[e] == 0.f ? 0.f : w[e];
-              y[e] = p[e] == 0.f ? 0.f : y[e];
-            }
-          }
-          zacc[nt][j][0] += y[0] + y[2];
-          zacc[nt][j][1] += y[1] + y[3];
-          const uint32_t b0 = transpose8x8(pack_bf16(w[0], w[1]));
-          const uint32_t b1 = transpose8x8(pack_bf16(w[2], w[3]));
-          Mma16816<__nv_bfloat16>::run(acc[nt][j][0], a0, b0, b1);
-          Mma16816<__nv_bfloat16>::run(acc[nt][j][1], a1, b0, b1);
-          Mma16816<__nv_bfloat16>::run(csum[nt], ab, b0, b1);
+          Mma16816<__half>::run(acc[nt][j][0], a0, b0[nt], b1[nt]);
+          Mma16816<__half>::run(acc[nt][j][1], a1, b0[nt], b1[nt]);
         }
       }
+    }
+  };
+
+  int it = 0;
+  bool tile_failed = false;
+  for (int tile = t_first; tile < tiles; tile += step, ++it) {
+    const int stage = it % kStages;
+    const bool got = mbar_wait_bounded(&full[warp][stage], (it / kStages) & 1, wait_ns);
+    if (!__all_sync(0xffffffffu, got)) {
+      if (lane == 0) record_status(QTTS_ERR_TIMEOUT);
+      tile_failed = true;
+      break;
+    }
+    const int t0 = tile * kTile;
+    if (t0 + kTile > first_lim) {
+      attend(ring + stage * S::kStage, t0, std::true_type{});
+    } else {
+      attend(ring + stage * S::kStage, t0, std::false_type{});
     }
     __syncwarp();
     if (tile + kStages * step < tiles) issue(stage);
@@ -434,15 +519,12 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 4 : 2) kv4_rows_kernel(
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
 #pragma unroll
-      for (int o = 4; o < 32; o <<= 1) {
-        l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], o);
-#pragma unroll
-        for (int j = 0; j < NG; ++j) zacc[nt][j][e] += __shfl_xor_sync(0xffffffffu, zacc[nt][j][e], o);
-      }
+      for (int o = 4; o < 32; o <<= 1) l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], o);
     }
   }
   __syncthreads();  // every warp is done with its ring: the partial outputs take its place
   float* part = reinterpret_cast<float*>(smem) + warp * kRows * S::kPitch;
+  const float vref = vlimit == 0.f ? 0.f : exp2_int(vexp - 127);  // no tile: no values
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -450,10 +532,9 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 4 : 2) kv4_rows_kernel(
       const int r = 8 * nt + 2 * c + e;
 #pragma unroll
       for (int j = 0; j < NG; ++j) {
-        const float add = zacc[nt][j][e] + __shfl_sync(0xffffffffu, csum[nt][e], 4 * j + c);
-        *reinterpret_cast<float4*>(part + r * S::kPitch + 32 * j + 4 * g) =
-            make_float4(acc[nt][j][0][e] + add, acc[nt][j][0][e + 2] + add, acc[nt][j][1][e] + add,
-                        acc[nt][j][1][e + 2] + add);
+        *reinterpret_cast<float4*>(part + r * S::kPitch + 32 * j + 4 * g) = make_float4(
+            acc[nt][j][0][e] * 0x1p10f * vref, acc[nt][j][0][e + 2] * 0x1p10f * vref,
+            acc[nt][j][1][e] * 0x1p10f * vref, acc[nt][j][1][e + 2] * 0x1p10f * vref);
       }
       if (g == 0) stat_m[warp][r] = m[nt][e], stat_l[warp][r] = l[nt][e];
     }
