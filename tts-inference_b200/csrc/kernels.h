@@ -234,7 +234,6 @@ struct Kv4AttnArgs {
   int causal;
   void* out;  // [total_q, q_heads, head_dim]
   int64_t out_token_stride;
-  int run;        // tokens a bulk copy: 32 where pages are whole tiles, else 16
   float* parts;   // workspace [total_q, q_heads, splits, head_dim] and its statistics
   float2* stats;  // [total_q, q_heads, splits]: running maximum (log2) and sum
 };

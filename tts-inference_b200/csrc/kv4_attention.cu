@@ -22,8 +22,9 @@
 //     becomes 2^14..2^15 against the code's 2^-24, so a value keeps 11 bits, or 2^-15
 //     of that scale where it is smaller). Scale and minimum of a tile are
 //     brought to those units once, a word a lane, through shared memory.
-//     Probabilities are fp16 too, times 2^15 so that the small ones stay normal;
-//   * every warp streams its own tiles of 32 tokens through a ring of bulk copies
+//     Probabilities are fp16 too, times 2^7: up to 2^15 while the running maximum
+//     may lag by 2^8, and the small ones normal down to 2^-21;
+//   * every warp streams its own tiles of 32 tokens through a ring of asynchronous copies
 //     and keeps its own running maximum and sum; the warps of a CTA meet in shared
 //     memory, and where there are few (request, head) pairs a cluster of up to 16
 //     CTAs splits one of them and meets in distributed shared memory: one launch,
@@ -66,6 +67,14 @@ __device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
   asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
+// D = A x B (no accumulator to be zeroed first), m16n8k16 fp16 -> fp32.
+__device__ __forceinline__ void mma_f16_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
+      "{%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
 __device__ __forceinline__ float exp2_int(int e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
 
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
@@ -74,11 +83,13 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
   return r;
 }
 
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(smem_u32(bar))
-      : "memory");
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
 __device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
@@ -109,14 +120,13 @@ struct RowsSmem {
 };
 
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 4 : 2) kv4_rows_kernel(const Kv4AttnArgs a, int row_blocks,
-                                                                        uint64_t wait_ns) {
+__global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 4 : 2) kv4_rows_kernel(const Kv4AttnArgs a, int row_blocks) {
   using S = RowsSmem<D>;
   constexpr int NG = D / kKv4Group;
   constexpr int kRows = 8 * NT;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ uint64_t full[kWarps][kStages];
-  __shared__ __align__(16) uint32_t vparam[kWarps][kTile * NG];  // value scales and minima of a tile, fp16
+  // Value scales and minima of a tile in fp16: word p * NG + j holds the two tokens of pair p.
+  __shared__ __align__(16) uint32_t vscale[kWarps][kTile / 2 * NG], vmin[kWarps][kTile / 2 * NG];
   __shared__ float stat_m[kWarps][kRows], stat_l[kWarps][kRows];  // of each warp
   __shared__ float part_m[kRows], part_l[kRows];        // of the CTA
 
@@ -129,9 +139,6 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 4 : 2) kv4_rows_kernel(
   const int rb = blockIdx.y % row_blocks;
   const int kvh = blockIdx.y / row_blocks;
   const int b = blockIdx.z;
-  if (lane < kStages) mbar_init(&full[warp][lane], 1);
-  fence_mbarrier_init();
-  __syncwarp();
   pdl_launch_dependents();
   pdl_wait();
 
@@ -154,48 +161,82 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 4 : 2) kv4_rows_kernel(
   const int kmax = r0 >= rows ? 0 : max(0, a.causal ? len - n + last + 1 : len);
   const int tiles = (kmax + kTile - 1) / kTile;
 
-  // This warp's tiles: every (splits * warps)-th one. A tile is one or two runs of tokens that
-  // lie in one page; lane 4 h + x copies run h of array x (key codes, key params, value codes,
-  // value params). Column and row within the page advance without a division, and the page of
-  // the next copy is fetched one copy ahead.
+  // This warp's tiles: every (splits * warps)-th one, 16 bytes a lane and copy into a ring. A
+  // tile is two runs of 16 tokens, each within one page. Column and row within the page advance
+  // without a division, and the pages of the next tile are fetched one tile ahead.
   uint8_t* ring = smem + warp * S::kWarpRing;
   const int step = splits * warps;
   const int t_first = rank * warps + warp;
-  const int run = a.run;                      // 32 or 16 tokens
-  const int per_page = a.cache.page_size / run;
-  const int runs_a_tile = kTile / run;
-  const int xarr = lane & 3, xrun = lane >> 2;
-  const bool copier = xrun < runs_a_tile;
-  const uint8_t* xbase = xarr == 0   ? a.cache.k_codes
-                         : xarr == 1 ? reinterpret_cast<const uint8_t*>(a.cache.k_params)
-                         : xarr == 2 ? a.cache.v_codes
-                                     : reinterpret_cast<const uint8_t*>(a.cache.v_params);
-  const int xrow = (xarr & 1) ? NG * 4 : D / 2;  // bytes a token
-  const uint32_t xdst = smem_u32(ring) + (xarr >= 1 ? S::kCodes : 0) + (xarr >= 2 ? S::kParams : 0) +
-                        (xarr == 3 ? S::kCodes : 0) + xrun * run * xrow;
+  const int per_page = a.cache.page_size / 16;
   const int32_t* table = a.table + b * a.ld_table;
-  int at = t_first * runs_a_tile + xrun;  // run number within the request
+  const int dcol = 2 * step / per_page, doff = 2 * step - dcol * per_page;
+  int at = 2 * t_first;  // number of the tile's first run within the request
   int col = at / per_page, off = at - col * per_page;
-  const int dat = step * runs_a_tile, dcol = dat / per_page, doff = dat - dcol * per_page;
-  int next_page = copier && at * run < kmax ? table[col] : 0;
-  auto issue = [&](int stage) {
-    const bool there = copier && at * run < kmax;
-    const uint32_t parts = __popc(__ballot_sync(0xffffffffu, there && xarr == 0));
-    if (lane == 0) mbar_arrive_expect_tx(&full[warp][stage], parts * static_cast<uint32_t>(run * (S::kStage / kTile)));
-    if (there) {
-      int64_t page = next_page;
-      if (page < 0 || page >= a.cache.pages) {
-        record_status(QTTS_ERR_SHAPE);
-        page = 0;
-      }
-      bulk_load(xdst + stage * S::kStage, xbase + kv4_row(a.cache, page, kvh, off * run) * xrow,
-                static_cast<uint32_t>(run * xrow), &full[warp][stage]);
-    }
-    at += dat, col += dcol, off += doff;
-    if (off >= per_page) off -= per_page, ++col;
-    if (copier && at * run < kmax) next_page = table[col];
+  const bool whole_tiles = per_page % 2 == 0;
+  int page[2];
+  auto find_pages = [&]() {
+    page[0] = at * 16 < kmax ? table[col] : 0;
+    if (!whole_tiles) page[1] = off + 1 < per_page ? page[0] : at * 16 + 16 < kmax ? table[col + 1] : 0;
   };
-  for (int s = 0; s < kStages && t_first + s * step < tiles; ++s) issue(s);
+  find_pages();
+  auto issue = [&](int stage) {
+    const uint32_t dst = smem_u32(ring) + stage * S::kStage + 16 * lane;
+    if (page[0] < 0 || page[0] >= a.cache.pages) {
+      record_status(QTTS_ERR_SHAPE);
+      page[0] = 0;
+    }
+    constexpr int kLanes = S::kParams / 16;  // lanes that copy params: 32 or 16
+    const int64_t row = kv4_row(a.cache, page[0], kvh, 16 * off);
+    if (whole_tiles) {
+      // The tile lies in one page (to its end: what is beyond kmax is there and is masked).
+      const uint8_t* k = a.cache.k_codes + row * (D / 2) + 16 * lane;
+      const uint8_t* v = a.cache.v_codes + row * (D / 2) + 16 * lane;
+#pragma unroll
+      for (int i = 0; i < NG; ++i) {
+        copy16(dst + 512 * i, k + 512 * i);
+        copy16(dst + S::kCodes + S::kParams + 512 * i, v + 512 * i);
+      }
+      if (lane < kLanes) {
+        copy16(dst + S::kCodes, a.cache.k_params + row * NG + 4 * lane);
+        copy16(dst + 2 * S::kCodes + S::kParams, a.cache.v_params + row * NG + 4 * lane);
+      }
+    } else {
+      if (page[1] < 0 || page[1] >= a.cache.pages) {
+        record_status(QTTS_ERR_SHAPE);
+        page[1] = 0;
+      }
+      const int64_t row1 = off + 1 == per_page ? kv4_row(a.cache, page[1], kvh, 0) : row + 16;
+      const bool second = at * 16 + 16 < kmax;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        if (h == 0 || second) {
+          const int64_t r = h ? row1 : row;
+#pragma unroll
+          for (int i = 0; i < NG / 2; ++i) {  // 16 tokens' codes: NG / 2 copies of 512 bytes
+            const int o = 512 * i;
+            copy16(dst + (S::kCodes / 2) * h + o, a.cache.k_codes + r * (D / 2) + 16 * lane + o);
+            copy16(dst + S::kCodes + S::kParams + (S::kCodes / 2) * h + o,
+                   a.cache.v_codes + r * (D / 2) + 16 * lane + o);
+          }
+        }
+      }
+      const bool upper = lane >= kLanes / 2;
+      if (lane < kLanes && (!upper || second)) {
+        const int64_t prow = (upper ? row1 : row) * NG + 4 * (lane - (upper ? kLanes / 2 : 0));
+        copy16(dst + S::kCodes, a.cache.k_params + prow);
+        copy16(dst + 2 * S::kCodes + S::kParams, a.cache.v_params + prow);
+      }
+    }
+    at += 2 * step, col += dcol, off += doff;
+    if (off >= per_page) off -= per_page, ++col;
+    find_pages();
+  };
+  // One group a tile, empty ones too, so that waiting counts tiles.
+#pragma unroll
+  for (int s = 0; s < kStages; ++s) {
+    if (t_first + s * step < tiles) issue(s);
+    copy_commit();
+  }
 
   // q as the B operand: row 8 nt + g, channels 32j + 8c .. + 7 as pairs (i, i + 4); and the
   // sums over each group of the rows 8 nt + 2c, + 1, whose scores this lane holds, in the
@@ -270,7 +311,7 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 4 : 2) kv4_rows_kernel(
   // range). What reaches vlimit moves it.
   int vexp = 0;
   float vlimit = 0.f;
-  float vunit = 0.f;  // 2^(127 - vexp)
+  float vs_to = 0.f, vz_to = 0.f;  // 2^14 and 2^-10 in units of 2^(vexp - 127)
 
   // Token of row slot s of a 16-token operand: s with the last bit turned in every other
   // pair, so that neither the key nor the value loads below hit one bank with more than two rows.
@@ -331,11 +372,12 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 4 : 2) kv4_rows_kernel(
       }
       most = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most)));
       if (!(most < vlimit)) {
-        const int to = min(253, max(16, static_cast<int>(__float_as_uint(most) >> 23)));
+        const int to = min(243, max(16, static_cast<int>(__float_as_uint(most) >> 23)));
         const float f = vlimit == 0.f ? 1.f : exp2_int(max(-126, vexp - to));
         vexp = to;
         vlimit = exp2_int(to - 126);
-        vunit = exp2_int(127 - to);
+        vs_to = exp2_int(127 - to) * 0x1p14f;
+        vz_to = exp2_int(127 - to) * 0x1p-10f;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -348,7 +390,11 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 4 : 2) kv4_rows_kernel(
     }
 #pragma unroll
     for (int k = 0; k < NG; ++k) {
-      vparam[warp][lane + 32 * k] = pack_f16(vs[k] * vunit * 0x1p14f, vz[k] * vunit * 0x1p-10f);
+      const int i = lane + 32 * k, t = i / NG;
+      // Token t is the first or second of its operand pair as the row slots below have it.
+      const int half = 2 * ((t >> 1) * NG + i % NG) + ((t ^ (t >> 1)) & 1);
+      reinterpret_cast<__half*>(vscale[warp])[half] = __float2half_rn(vs[k] * vs_to);
+      reinterpret_cast<__half*>(vmin[warp])[half] = __float2half_rn(vz[k] * vz_to);
     }
 
     // Scores of 2 x 16 tokens: s[nt][mt][2 * token half + row of the pair].
@@ -381,8 +427,8 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 4 : 2) kv4_rows_kernel(
         const float z0 = kv4_min(pw[0][j]), z1 = kv4_min(pw[1][j]);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          float d[4] = {0.f, 0.f, 0.f, 0.f};
-          Mma16816<__half>::run(d, a0, qf[nt][j][0], qf[nt][j][1]);
+          float d[4];
+          mma_f16_first(d, a0, qf[nt][j][0], qf[nt][j][1]);
           Mma16816<__half>::run(d, a1, qf[nt][j][2], qf[nt][j][3]);
           s[nt][mt][0] = fmaf(sc0, d[0], fmaf(z0, qsum[nt][j][0], s[nt][mt][0]));
           s[nt][mt][1] = fmaf(sc0, d[1], fmaf(z0, qsum[nt][j][1], s[nt][mt][1]));
@@ -419,14 +465,16 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 4 : 2) kv4_rows_kernel(
         mx[0] = fmaxf(mx[0], __shfl_xor_sync(0xffffffffu, mx[0], o));
         mx[1] = fmaxf(mx[1], __shfl_xor_sync(0xffffffffu, mx[1], o));
       }
-      // to_log2 > 0: the largest score stays the largest.
-      mx[0] = fmaxf(m[nt][0], mx[0] * to_log2[nt][0]);
-      mx[1] = fmaxf(m[nt][1], mx[1] * to_log2[nt][1]);
-      if (__any_sync(0xffffffffu, mx[0] > m[nt][0] || mx[1] > m[nt][1])) {
+      // to_log2 > 0: the largest score stays the largest. The reference m follows the maximum
+      // only when that has grown by more than 2^8: probabilities stay below 2^15.
+      mx[0] *= to_log2[nt][0];
+      mx[1] *= to_log2[nt][1];
+      if (__any_sync(0xffffffffu, mx[0] > m[nt][0] + 8.f || mx[1] > m[nt][1] + 8.f)) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const float f = mx[e] > m[nt][e] ? ex2(m[nt][e] - mx[e]) : 1.f;
-          m[nt][e] = mx[e];
+          const float to = fmaxf(m[nt][e], mx[e]);
+          const float f = to > m[nt][e] ? ex2(m[nt][e] - to) : 1.f;
+          m[nt][e] = to;
           l[nt][e] *= f;
 #pragma unroll
           for (int j = 0; j < NG; ++j) {
@@ -435,8 +483,8 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 4 : 2) kv4_rows_kernel(
           }
         }
       }
-      const float m0 = 15.f - (kMasked && m[nt][0] == -INFINITY ? 0.f : m[nt][0]);
-      const float m1 = 15.f - (kMasked && m[nt][1] == -INFINITY ? 0.f : m[nt][1]);
+      const float m0 = 7.f - (kMasked && m[nt][0] == -INFINITY ? 0.f : m[nt][0]);
+      const float m1 = 7.f - (kMasked && m[nt][1] == -INFINITY ? 0.f : m[nt][1]);
 #pragma unroll
       for (int mt = 0; mt < 2; ++mt) {
 #pragma unroll
@@ -448,10 +496,10 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 4 : 2) kv4_rows_kernel(
     }
 
     // Weighted values.
-    __syncwarp();  // vparam
+    __syncwarp();  // vscale, vmin
 #pragma unroll
     for (int mt = 0; mt < 2; ++mt) {
-      uint32_t vw[4][NG / 2], pw[4][NG];
+      uint32_t vw[4][NG / 2], sw[2][NG], zw[2][NG];
 #pragma unroll
       for (int h = 0; h < 4; ++h) {
         const int t = 16 * mt + 8 * (h >> 1) + ((h & 1) ? v1 : v0);
@@ -460,7 +508,11 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 4 : 2) kv4_rows_kernel(
         } else {
           vw[h][0] = *reinterpret_cast<const uint32_t*>(vc + t * 32 + 4 * g);
         }
-        load_params(vparam[warp], t, pw[h]);
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        load_params(vscale[warp], 8 * mt + 4 * h + c, sw[h]);
+        load_params(vmin[warp], 8 * mt + 4 * h + c, zw[h]);
       }
       uint32_t b0[NT], b1[NT];
 #pragma unroll
@@ -474,8 +526,7 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 4 : 2) kv4_rows_kernel(
         const uint32_t xa = __byte_perm(vw[0][j / 2], vw[1][j / 2], (j & 1) ? 0x7632 : 0x5410);
         const uint32_t xb = __byte_perm(vw[2][j / 2], vw[3][j / 2], (j & 1) ? 0x7632 : 0x5410);
         const uint32_t ya = xa >> 8, yb = xb >> 8;
-        const uint32_t sa = __byte_perm(pw[0][j], pw[1][j], 0x5410), za = __byte_perm(pw[0][j], pw[1][j], 0x7632);
-        const uint32_t sb = __byte_perm(pw[2][j], pw[3][j], 0x5410), zb = __byte_perm(pw[2][j], pw[3][j], 0x7632);
+        const uint32_t sa = sw[0][j], za = zw[0][j], sb = sw[1][j], zb = zw[1][j];
         const uint32_t sa4 = mul_f16x2(sa, 0x2C002C00u), sb4 = mul_f16x2(sb, 0x2C002C00u);  // / 16
         const uint32_t a0[4] = {fma_f16x2(nib_pair(xa, 0), sa, za), fma_f16x2(nib_pair(xa, 1), sa4, za),
                                 fma_f16x2(nib_pair(xb, 0), sb, zb), fma_f16x2(nib_pair(xb, 1), sb4, zb)};
@@ -490,16 +541,10 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 4 : 2) kv4_rows_kernel(
     }
   };
 
-  int it = 0;
-  bool tile_failed = false;
-  for (int tile = t_first; tile < tiles; tile += step, ++it) {
-    const int stage = it % kStages;
-    const bool got = mbar_wait_bounded(&full[warp][stage], (it / kStages) & 1, wait_ns);
-    if (!__all_sync(0xffffffffu, got)) {
-      if (lane == 0) record_status(QTTS_ERR_TIMEOUT);
-      tile_failed = true;
-      break;
-    }
+  int stage = 0;
+  for (int tile = t_first; tile < tiles; tile += step) {
+    copy_wait<kStages - 1>();
+    __syncwarp();
     const int t0 = tile * kTile;
     if (t0 + kTile > first_lim) {
       attend(ring + stage * S::kStage, t0, std::true_type{});
@@ -508,9 +553,8 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 4 : 2) kv4_rows_kernel(
     }
     __syncwarp();
     if (tile + kStages * step < tiles) issue(stage);
-  }
-  if (tile_failed) {  // copies still in flight must land before their memory is used again
-    for (int s = 0; s < kStages; ++s) (void)mbar_wait_bounded(&full[warp][(it + s) % kStages], ((it + s) / kStages) & 1, wait_ns);
+    copy_commit();
+    stage = stage + 1 == kStages ? 0 : stage + 1;
   }
 
   // Finish the warp: the rest of the sums over its lanes, then its partial outputs.
@@ -573,7 +617,7 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 4 : 2) kv4_rows_kernel(
           *reinterpret_cast<uint2*>(v);
     } else if (mode == 2) {
       const int64_t at_row = (orow * a.q_heads + head) * splits + rank;
-      *reinterpret_cast<float4*>(a.parts + at_row * D + ch) = o;
+      if (top != -INFINITY) *reinterpret_cast<float4*>(a.parts + at_row * D + ch) = o;
       if (ch == 0) a.stats[at_row] = make_float2(top, lsum);
     } else {
       // Each thread reads exactly the elements of every warp's part that it then overwrites.
@@ -642,6 +686,7 @@ __global__ void __launch_bounds__(128) kv4_join_kernel(const Kv4AttnArgs a, int 
 #pragma unroll 4
   for (int q = 0; q < splits; ++q) {
     const float2 s = st[q];
+    if (s.x == -INFINITY) continue;  // saw nothing: its part was not written
     const float f = ex2(s.x - safe);
     lsum = fmaf(f, s.y, lsum);
 #pragma unroll
@@ -668,12 +713,18 @@ RowsPlan plan_rows(int64_t max_q, int share, int kv_heads, int batch, int64_t mo
   p.row_blocks = (rows + 8 * p.nt - 1) / (8 * p.nt);
   const int64_t units = p.row_blocks * kv_heads * batch;
   // One wave of CTAs (four of 128 threads an SM; two with 16 rows, for their registers), at
-  // least one tile a warp.
+  // least one tile a warp; and, as far as a cluster goes, no more than 8 tiles a warp, so that
+  // one long request among short ones does not hold the call up (many units even out by
+  // themselves).
   const int64_t wave = static_cast<int64_t>(kNumSMs) * (p.nt == 1 ? 4 : 2);
   const int64_t tiles = (most_tokens + kTile - 1) / kTile;
   const int64_t want = wave / (units > 0 ? units : 1);
   const int64_t can = (tiles + kWarps - 1) / kWarps;
-  int64_t s = want < can ? want : can;
+  const int64_t even = (tiles + 8 * kWarps - 1) / (8 * kWarps);
+  int64_t s = even < kMaxCluster ? even : kMaxCluster;
+  if (s * units > 8 * wave) s = 1;
+  if (s < want) s = want;
+  if (s > can) s = can;
   p.splits = static_cast<int>(s < 1 ? 1 : s > 256 ? 256 : s);
   return p;
 }
@@ -719,8 +770,7 @@ int launch_rows(Kv4AttnArgs a, const RowsPlan& p, bool pdl, cudaStream_t stream)
   if (!workspace) a.parts = nullptr, a.stats = nullptr;
   const int r = launch(kv4_rows_kernel<T, D, NT>,
                        dim3(p.splits, static_cast<unsigned>(p.row_blocks * a.cache.kv_heads), a.batch), 32 * kWarps,
-                       kSmem, workspace ? 1 : p.splits, pdl, stream, a, static_cast<int>(p.row_blocks),
-                       current_wait_limit_ns());
+                       kSmem, workspace ? 1 : p.splits, pdl, stream, a, static_cast<int>(p.row_blocks));
   if (r != QTTS_OK || !workspace) return r;
   const int64_t rows = static_cast<int64_t>(a.total_q) * a.q_heads;
   return launch(kv4_join_kernel<T, D>, dim3(static_cast<unsigned>((rows + 3) / 4)), 128, 0, 1, true, stream, a,
@@ -816,7 +866,6 @@ extern "C" int qtts_kv4_attention(const void* q, int64_t q_token_stride, int64_t
   a.causal = causal;
   a.out = out;
   a.out_token_stride = out_token_stride;
-  a.run = page_size % kTile == 0 ? kTile : 16;
   if (need > 0) {
     a.parts = static_cast<float*>(workspace);
     a.stats = reinterpret_cast<float2*>(a.parts + need / ((head_dim + 2) * 4) * head_dim);
