@@ -731,11 +731,6 @@ RowsPlan plan_rows(int64_t max_q, int share, int kv_heads, int batch, int64_t mo
 
 template <typename KernT, typename... Args>
 int launch(KernT kern, dim3 grid, int threads, size_t smem, int cluster, bool pdl, cudaStream_t stream, Args... args) {
-  if (smem > 48 * 1024 &&
-      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) != cudaSuccess) {
-    (void)cudaGetLastError();
-    return QTTS_ERR_LAUNCH;
-  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(threads);
@@ -766,6 +761,11 @@ int launch_rows(Kv4AttnArgs a, const RowsPlan& p, bool pdl, cudaStream_t stream)
   constexpr size_t kRing = static_cast<size_t>(kWarps) * S::kWarpRing;
   constexpr size_t kPart = static_cast<size_t>(kWarps) * 8 * NT * S::kPitch * 4;
   constexpr size_t kSmem = kRing > kPart ? kRing : kPart;
+  if (kSmem > 48 * 1024 && cudaFuncSetAttribute(kv4_rows_kernel<T, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                static_cast<int>(kSmem)) != cudaSuccess) {
+    (void)cudaGetLastError();
+    return QTTS_ERR_LAUNCH;
+  }
   const bool workspace = p.splits > kMaxCluster;
   if (!workspace) a.parts = nullptr, a.stats = nullptr;
   const int r = launch(kv4_rows_kernel<T, D, NT>,

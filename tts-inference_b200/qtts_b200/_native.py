@@ -213,6 +213,26 @@ def stream_ptr(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+# The current raw stream and device without building their Python objects (some
+# microseconds a call); the public calls where this torch has no such shortcut.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+_raw_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
+def launch(name: str, index: int, *args) -> None:
+    """Call entry point ``name`` with ``args`` and, after them, the current stream of device
+    ``index``, with that device current."""
+    fn = getattr(_lib or _load(), name)
+    if _raw_device() == index:
+        code = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            code = fn(*args, _raw_stream(index))
+    if code != OK:
+        check(code, name)
+
+
 def device_status(reset: bool = False) -> int:
     return _load().qtts_device_status(1 if reset else 0)
 

@@ -28,6 +28,11 @@ from .quant.kernels import _flags, _require_cuda
 
 GROUP = 32  # channels that share a scale and a minimum
 HEAD_DIMS = (64, 128)
+_HALVES = (32, 64)
+_DTYPES = {torch.bfloat16: nat.BF16, torch.float16: nat.FP16}
+_SCALES = {d: 1.0 / math.sqrt(d) for d in HEAD_DIMS}
+_SPLIT_FROM = 1024  # tokens
+_SECTIONS: dict[tuple[int, ...], ctypes.Array] = {}  # host arrays of the axis shares, by their values
 
 
 class Kv4Cache:
@@ -39,28 +44,35 @@ class Kv4Cache:
     multiple of 16. A slot cache is one page a request.
     """
 
-    __slots__ = ("k_codes", "k_params", "v_codes", "v_params", "pages", "kv_heads", "page_size", "head_dim", "_ptrs")
+    __slots__ = ("k_codes", "k_params", "v_codes", "v_params", "pages", "kv_heads", "page_size", "head_dim", "_ptrs",
+                 "_index")
 
     def __init__(self, k_codes: torch.Tensor, k_params: torch.Tensor, v_codes: torch.Tensor,
                  v_params: torch.Tensor) -> None:
         shape = k_codes.shape
-        if len(shape) != 4 or v_codes.shape != shape or k_codes.dtype != torch.uint8 or v_codes.dtype != torch.uint8:
+        if len(shape) != 4 or v_codes.shape != shape or k_codes.dtype is not torch.uint8 or \
+                v_codes.dtype is not torch.uint8:
             raise ValueError("codes must be uint8 [pages, kv_heads, page_size, head_dim / 2], keys and values alike")
-        self.pages, self.kv_heads, self.page_size, half = shape
-        self.head_dim = 2 * half
-        if self.head_dim not in HEAD_DIMS:
-            raise ValueError(f"head_dim {self.head_dim}: the 4-bit cache takes {HEAD_DIMS}")
-        if self.page_size < 16 or self.page_size % 16:
-            raise ValueError(f"page_size {self.page_size} is not a multiple of 16")
-        want = (*shape[:3], self.head_dim // GROUP, 2)
-        for p in (k_params, v_params):
-            if p.shape != want or p.dtype != torch.bfloat16:
-                raise ValueError(f"params must be bf16 {want}, got {p.dtype} {tuple(p.shape)}")
-        for t in (k_codes, k_params, v_codes, v_params):
-            if not t.is_contiguous():
-                raise ValueError("the cache's tensors must be contiguous")
+        pages, kv_heads, page_size, half = shape
+        if half not in _HALVES:
+            raise ValueError(f"head_dim {2 * half}: the 4-bit cache takes {HEAD_DIMS}")
+        if page_size < 16 or page_size % 16:
+            raise ValueError(f"page_size {page_size} is not a multiple of 16")
+        want = (pages, kv_heads, page_size, half * 2 // GROUP, 2)
+        if k_params.shape != want or v_params.shape != want or k_params.dtype is not torch.bfloat16 or \
+                v_params.dtype is not torch.bfloat16:
+            raise ValueError(f"params must be bf16 {want}, keys and values alike")
+        if not (k_codes.is_contiguous() and k_params.is_contiguous() and v_codes.is_contiguous()
+                and v_params.is_contiguous()):
+            raise ValueError("the cache's tensors must be contiguous")
+        index = k_codes.get_device()
+        if not index == k_params.get_device() == v_codes.get_device() == v_params.get_device():
+            raise ValueError("the cache's tensors must be on one device")
+        self.pages, self.kv_heads, self.page_size, self.head_dim = pages, kv_heads, page_size, 2 * half
         self.k_codes, self.k_params, self.v_codes, self.v_params = k_codes, k_params, v_codes, v_params
-        self._ptrs = (k_codes.data_ptr(), k_params.data_ptr(), v_codes.data_ptr(), v_params.data_ptr())
+        self._index = index
+        self._ptrs = (k_codes.data_ptr(), k_params.data_ptr(), v_codes.data_ptr(), v_params.data_ptr(), pages,
+                      page_size)
 
     @classmethod
     def empty(cls, pages: int, kv_heads: int, page_size: int, head_dim: int, device="cuda") -> Kv4Cache:
@@ -120,59 +132,73 @@ def rope_kv4_append(
     width = (q_heads + 2 * kv_heads) * d
     if qkv.dim() != 2 or qkv.shape[1] != width:
         raise ValueError(f"qkv is {tuple(qkv.shape)}, expected [tokens, {width}]")
-    if qkv.dtype not in (torch.bfloat16, torch.float16):
+    dtype = _DTYPES.get(qkv.dtype)
+    if dtype is None:
         raise TypeError(f"qkv must be bf16 or fp16, got {qkv.dtype}")
     tokens = qkv.shape[0]
-    if slots.dtype != torch.int64 or slots.shape != (tokens,) or (tokens > 1 and slots.stride(0) != 1):
+    if slots.dtype is not torch.int64 or slots.shape != (tokens,) or not slots.is_contiguous():
         raise ValueError(f"slots must be a contiguous int64 [{tokens}]")
     if (cos is None) != (sin is None):
         raise ValueError("cos and sin are given together")
-    device = _require_cuda(qkv, cache.k_codes, slots, cos, sin, positions, q_norm, k_norm)
+    index = qkv.get_device()
+    if index < 0 or cache._index != index or slots.get_device() != index:
+        _require_cuda(qkv, cache.k_codes, slots)
     if qkv.stride(1) != 1 or qkv.stride(0) % 8 or qkv.data_ptr() % 16:
         qkv = qkv.clone(memory_format=torch.contiguous_format)
-    axes, table_len, ldpos, section_array, table = 0, 0, 0, None, (None, None, None)
+    axes = table_len = ldpos = 0
+    cos_ptr = sin_ptr = pos_ptr = section_array = None
     if cos is not None:
         if positions is None:
             raise ValueError("positions are needed with cos and sin")
-        if positions.dim() == 1:
-            positions = positions[None]
-        axes = positions.shape[0]
-        if sections is None:
-            sections = (d // 2,)
-        if len(sections) != axes or not 1 <= axes <= 4 or sum(sections) != d // 2 or min(sections) < 0:
-            raise ValueError(f"sections {tuple(sections)} do not share {d // 2} pairs among {axes} axes")
-        if positions.dtype != torch.int64 or positions.shape[1] != tokens or (tokens > 1 and positions.stride(1) != 1):
+        if positions.dtype is not torch.int64 or positions.dim() not in (1, 2) or positions.shape[-1] != tokens or \
+                (tokens > 1 and positions.stride(-1) != 1):
             raise ValueError(f"positions must be int64 [axes, {tokens}] with unit stride along the tokens")
-        for t in (cos, sin):
-            if t.dtype != torch.float32 or t.dim() != 2 or t.shape != cos.shape or t.shape[1] != d // 2 or \
-                    not t.is_contiguous():
-                raise ValueError(f"cos and sin must be contiguous fp32 [length, {d // 2}]")
-        table_len = cos.shape[0]
-        ldpos = max(positions.stride(0), tokens) if axes > 1 else tokens
-        section_array = (ctypes.c_int * axes)(*sections)
-        table = (cos.data_ptr(), sin.data_ptr(), positions.data_ptr())
-    norms = []
-    for w in (q_norm, k_norm):
-        if w is not None:
-            if w.shape != (d,) or w.dtype != qkv.dtype:
-                raise ValueError(f"a norm weight must be {qkv.dtype} [{d}]")
-            if w.stride(0) != 1 or w.data_ptr() % 16:
-                w = w.clone(memory_format=torch.contiguous_format)
-        norms.append(w)
-    q = torch.empty((tokens, q_heads, d), device=device, dtype=qkv.dtype)
-    k_values = v_values = None
+        axes = positions.shape[0] if positions.dim() == 2 else 1
+        sections = (d // 2,) if sections is None else tuple(sections)
+        section_array = _SECTIONS.get(sections)
+        if section_array is None:
+            section_array = _SECTIONS[sections] = (ctypes.c_int * len(sections))(*sections)
+        if len(sections) != axes or not 1 <= axes <= 4 or sum(sections) != d // 2 or min(sections) < 0:
+            raise ValueError(f"sections {sections} do not share {d // 2} pairs among {axes} axes")
+        table_shape = cos.shape
+        if len(table_shape) != 2 or table_shape[1] != d // 2 or sin.shape != table_shape or \
+                cos.dtype is not torch.float32 or sin.dtype is not torch.float32 or not cos.is_contiguous() or \
+                not sin.is_contiguous():
+            raise ValueError(f"cos and sin must be contiguous fp32 [length, {d // 2}]")
+        if cos.get_device() != index or sin.get_device() != index or positions.get_device() != index:
+            _require_cuda(qkv, cos, sin, positions)
+        table_len = table_shape[0]
+        ldpos = tokens if axes == 1 else positions.stride(0)
+        if ldpos < tokens:  # an axis that is broadcast
+            positions = positions.contiguous()
+            ldpos = tokens
+        cos_ptr, sin_ptr, pos_ptr = cos.data_ptr(), sin.data_ptr(), positions.data_ptr()
+    if q_norm is not None:
+        q_norm = _norm_weight(q_norm, d, qkv)
+    if k_norm is not None:
+        k_norm = _norm_weight(k_norm, d, qkv)
+    q = qkv.new_empty((tokens, q_heads, d))
+    k_ptr = v_ptr = None
     if values:
-        k_values = torch.empty((tokens, kv_heads, d), device=device, dtype=qkv.dtype)
-        v_values = torch.empty((tokens, kv_heads, d), device=device, dtype=qkv.dtype)
-    code = nat.lib().qtts_rope_kv4_append(
-        qkv.data_ptr(), qkv.stride(0) if tokens > 1 else width, nat.dtype_code(qkv.dtype), tokens, q_heads, kv_heads, d,
-        norms[0].data_ptr() if norms[0] is not None else None, norms[1].data_ptr() if norms[1] is not None else None,
-        eps, table[0], table[1], table_len, table[2], ldpos, axes, section_array, int(interleaved), slots.data_ptr(),
-        q.data_ptr(), q_heads * d, *cache._ptrs, cache.pages, cache.page_size,
-        k_values.data_ptr() if values else None, v_values.data_ptr() if values else None, _flags(),
-        nat.stream_ptr(device))
-    nat.check(code, "qtts_rope_kv4_append")
+        k_values = qkv.new_empty((tokens, kv_heads, d))
+        v_values = torch.empty_like(k_values)
+        k_ptr, v_ptr = k_values.data_ptr(), v_values.data_ptr()
+    nat.launch(
+        "qtts_rope_kv4_append", index, qkv.data_ptr(), qkv.stride(0) if tokens > 1 else width, dtype, tokens, q_heads,
+        kv_heads, d, None if q_norm is None else q_norm.data_ptr(), None if k_norm is None else k_norm.data_ptr(), eps,
+        cos_ptr, sin_ptr, table_len, pos_ptr, ldpos, axes, section_array, interleaved, slots.data_ptr(), q.data_ptr(),
+        q_heads * d, *cache._ptrs, k_ptr, v_ptr, _flags())
     return (q, k_values, v_values) if values else q
+
+
+def _norm_weight(w: torch.Tensor, d: int, qkv: torch.Tensor) -> torch.Tensor:
+    if w.shape != (d,) or w.dtype is not qkv.dtype:
+        raise ValueError(f"a norm weight must be {qkv.dtype} [{d}]")
+    if w.get_device() != qkv.get_device():
+        _require_cuda(qkv, w)
+    if w.stride(0) != 1 or w.data_ptr() % 16:
+        w = w.clone(memory_format=torch.contiguous_format)
+    return w
 
 
 def kv4_attention(
@@ -200,48 +226,67 @@ def kv4_attention(
     cache's heads. A row that sees nothing gives zeros. ``scale`` defaults to
     ``1 / sqrt(head_dim)``. Returns ``[total, q_heads, head_dim]``.
     """
-    if q.dim() != 3 or q.shape[2] != cache.head_dim or q.shape[1] % cache.kv_heads:
-        raise ValueError(f"q is {tuple(q.shape)}, expected [tokens, a multiple of {cache.kv_heads}, {cache.head_dim}]")
-    if q.dtype not in (torch.bfloat16, torch.float16):
+    shape = q.shape
+    kv_heads, d = cache.kv_heads, cache.head_dim
+    if len(shape) != 3 or shape[2] != d or shape[1] % kv_heads or not shape[1]:
+        raise ValueError(f"q is {tuple(shape)}, expected [tokens, a multiple of {kv_heads}, {d}]")
+    dtype = _DTYPES.get(q.dtype)
+    if dtype is None:
         raise TypeError(f"q must be bf16 or fp16, got {q.dtype}")
-    total, heads, d = q.shape
-    batch = lengths.shape[0]
-    if lengths.dtype != torch.int32 or lengths.dim() != 1 or (batch > 1 and lengths.stride(0) != 1):
+    total, heads = shape[0], shape[1]
+    if lengths.dtype is not torch.int32 or lengths.dim() != 1 or not lengths.is_contiguous():
         raise ValueError("lengths must be a contiguous int32 [batch]")
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != batch or \
-            (block_table.shape[1] > 1 and block_table.stride(1) != 1):
+    batch = lengths.shape[0]
+    if block_table.dtype is not torch.int32 or block_table.dim() != 2 or block_table.shape[0] != batch or \
+            (block_table.stride(1) != 1 and block_table.shape[1] > 1):
         raise ValueError(f"block_table must be int32 [{batch}, columns] with unit stride along the columns")
+    columns = block_table.shape[1]
+    starts_ptr = None
+    index = q.get_device()
     if q_starts is None:
-        if batch == 0 or total % batch:
-            if total:
-                raise ValueError(f"{total} tokens do not share evenly among {batch} requests: give q_starts")
         max_q = total // batch if batch else 0
+        if max_q * batch != total:
+            raise ValueError(f"{total} tokens do not share evenly among {batch} requests: give q_starts")
     else:
-        if q_starts.dtype != torch.int32 or q_starts.shape != (batch + 1,) or (batch > 0 and q_starts.stride(0) != 1):
+        if q_starts.dtype is not torch.int32 or q_starts.shape != (batch + 1,) or not q_starts.is_contiguous():
             raise ValueError(f"q_starts must be a contiguous int32 [{batch + 1}]")
         if max_q is None:
             raise ValueError("max_q is needed with q_starts")
-        max_q = min(max_q, total)
+        if max_q > total:
+            max_q = total
+        if q_starts.get_device() != index:
+            _require_cuda(q, q_starts)
+        starts_ptr = q_starts.data_ptr()
     if scale is None:
-        scale = 1.0 / math.sqrt(d)
+        scale = _SCALES[d]
     elif not 0.0 < scale < math.inf:
         raise ValueError(f"scale {scale} is not positive and finite")
-    device = _require_cuda(q, cache.k_codes, block_table, lengths, q_starts, out)
-    if q.stride(2) != 1 or q.stride(0) % 8 or q.stride(1) % 8 or q.stride(1) < d or q.data_ptr() % 16:
+    if index < 0 or cache._index != index or block_table.get_device() != index or lengths.get_device() != index:
+        _require_cuda(q, cache.k_codes, block_table, lengths)
+    if q.is_contiguous():
+        token_stride, head_stride = heads * d, d
+    else:
+        token_stride, head_stride = q.stride(0), q.stride(1)
+        if q.stride(2) != 1 or token_stride % 8 or head_stride % 8 or head_stride < d:
+            q = q.contiguous()
+            token_stride, head_stride = heads * d, d
+    q_ptr = q.data_ptr()
+    if q_ptr % 16:
         q = q.clone(memory_format=torch.contiguous_format)
+        q_ptr, token_stride, head_stride = q.data_ptr(), heads * d, d
     if out is None:
-        out = torch.empty((total, heads, d), device=device, dtype=q.dtype)
-    elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
-        raise ValueError(f"out must be a contiguous {q.dtype} {tuple(q.shape)}")
-    columns = block_table.shape[1]
-    need = nat.lib().qtts_kv4_attention_workspace(total, max_q, batch, heads, cache.kv_heads, d,
-                                                  columns * cache.page_size)
-    workspace = torch.empty(need, device=device, dtype=torch.uint8) if need else None
-    code = nat.lib().qtts_kv4_attention(
-        q.data_ptr(), q.stride(0), q.stride(1), nat.dtype_code(q.dtype), *cache._ptrs, cache.pages, cache.page_size,
-        block_table.data_ptr(), block_table.stride(0) if batch > 1 else columns, columns, lengths.data_ptr(),
-        q_starts.data_ptr() if q_starts is not None else None, total, max_q, batch, heads, cache.kv_heads, d,
-        scale, int(causal), out.data_ptr(), heads * d,
-        workspace.data_ptr() if need else None, _flags(), nat.stream_ptr(device))
-    nat.check(code, "qtts_kv4_attention")
+        out = q.new_empty(shape)
+    elif out.shape != shape or out.dtype is not q.dtype or not out.is_contiguous() or out.get_device() != index:
+        raise ValueError(f"out must be a contiguous {q.dtype} {tuple(shape)} on q's device")
+    work_ptr = None
+    tokens = columns * cache.page_size
+    if tokens >= _SPLIT_FROM:  # fewer tokens are never split across a workspace
+        need = nat.lib().qtts_kv4_attention_workspace(total, max_q, batch, heads, kv_heads, d, tokens)
+        if need:
+            workspace = q.new_empty(need, dtype=torch.uint8)
+            work_ptr = workspace.data_ptr()
+    nat.launch(
+        "qtts_kv4_attention", index, q_ptr, token_stride, head_stride, dtype, *cache._ptrs, block_table.data_ptr(),
+        block_table.stride(0) if batch > 1 else columns, columns, lengths.data_ptr(), starts_ptr, total, max_q, batch,
+        heads, kv_heads, d, scale, causal, out.data_ptr(), heads * d, work_ptr, _flags())
     return out

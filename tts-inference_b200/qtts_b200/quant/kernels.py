@@ -183,41 +183,53 @@ def add_rms_norm_quant(
     receives h and may be ``residual`` itself; with ``residual`` None there is no addition
     and h is None. fp32 throughout: the norm reads the unrounded sum and the quantizer the
     unrounded norm."""
-    width = x.shape[-1]
-    if weight.dim() != 1 or weight.shape[0] != width:
+    shape = x.shape
+    width = shape[-1]
+    xtype = x.dtype
+    if weight.shape != (width,):
         raise ValueError(f"weight is {tuple(weight.shape)}, expected [{width}]")
-    if dtype not in (torch.float8_e4m3fn, torch.int8):
+    if dtype is not torch.float8_e4m3fn and dtype is not torch.int8:
         raise TypeError(f"codes are float8_e4m3fn or int8, not {dtype}")
-    device = _require_cuda(x, weight, residual, residual_out)
-    a = _rows_view(x, width)
+    index = x.get_device()
+    if index < 0 or weight.get_device() != index or (residual is not None and residual.get_device() != index):
+        _require_cuda(x, weight, residual)
+    if weight.dtype is not xtype or not weight.is_contiguous():
+        weight = weight.to(xtype).contiguous()
+    flat = len(shape) == 2 and x.is_contiguous()
+    a = x if flat else _rows_view(x, width)
     rows = a.shape[0]
-    if weight.dtype != x.dtype or weight.stride(0) != 1:
-        weight = weight.to(x.dtype).contiguous()
     r_ptr = ro_ptr = None
-    ldr = ldro = width
+    lda = ldr = ldro = width
+    if not flat and rows > 1:
+        lda = a.stride(0)
     if residual is not None:
-        if residual.shape != x.shape or residual.dtype != x.dtype:
-            raise ValueError(f"residual must be {x.dtype} {tuple(x.shape)}")
-        r = _rows_view(residual, width)
+        if residual.shape != shape or residual.dtype is not xtype:
+            raise ValueError(f"residual must be {xtype} {tuple(shape)}")
+        if residual.is_contiguous():
+            r_ptr = residual.data_ptr()
+        else:
+            r = _rows_view(residual, width)
+            ldr = r.stride(0) if rows > 1 else width
+            r_ptr = r.data_ptr()
         if residual_out is None:
-            residual_out = torch.empty(x.shape, device=device, dtype=x.dtype)
-            ro = residual_out.view(rows, width)
+            residual_out = x.new_empty(shape)
+        elif residual_out.get_device() != index:
+            _require_cuda(x, residual_out)
+        if residual_out.is_contiguous() and residual_out.shape == shape and residual_out.dtype is xtype:
+            ro_ptr = residual_out.data_ptr()
         else:
             ro = _rows_view(residual_out, width)
-            if residual_out.shape != x.shape or ro.dtype != x.dtype or ro.data_ptr() != residual_out.data_ptr():
-                raise ValueError(f"residual_out must be {x.dtype} {tuple(x.shape)} with unit column stride")
-        if rows > 1:
-            ldr, ldro = r.stride(0), ro.stride(0)
-        r_ptr, ro_ptr = r.data_ptr(), ro.data_ptr()
+            if residual_out.shape != shape or ro.dtype != xtype or ro.data_ptr() != residual_out.data_ptr():
+                raise ValueError(f"residual_out must be {xtype} {tuple(shape)} with unit column stride")
+            ldro = ro.stride(0) if rows > 1 else width
+            ro_ptr = ro.data_ptr()
     elif residual_out is not None:
         raise ValueError("residual_out needs a residual")
-    q = torch.empty((rows, width), device=device, dtype=dtype)
-    scale = torch.empty((rows, 1), device=device, dtype=torch.float32)
-    code = nat.lib().qtts_add_rms_norm_quant(
-        a.data_ptr(), a.stride(0) if rows > 1 else width, r_ptr, ldr, weight.data_ptr(), eps, ro_ptr, ldro,
-        nat.dtype_code(x.dtype), q.data_ptr(), width, nat.dtype_code(dtype), scale.data_ptr(), rows, width, _flags(),
-        nat.stream_ptr(device))
-    nat.check(code, "qtts_add_rms_norm_quant")
+    q = x.new_empty((rows, width), dtype=dtype)
+    scale = x.new_empty((rows, 1), dtype=torch.float32)
+    nat.launch("qtts_add_rms_norm_quant", index, a.data_ptr(), lda, r_ptr, ldr, weight.data_ptr(), eps, ro_ptr, ldro,
+               nat.dtype_code(xtype), q.data_ptr(), width, nat.dtype_code(dtype), scale.data_ptr(), rows, width,
+               _flags())
     return q, scale, residual_out
 
 
