@@ -356,7 +356,7 @@ QTTS_API int qtts_w8a16_head_argmax(const void* x, int64_t ldx, int x_dtype, con
  *   residual_out = cast(h)
  *   y        = weight * (h * (1 / sqrt(mean(h^2) + eps)))
  *   scale[m] = max(max_k |y[m,k]|, 1e-6) * fl32(1 / 448)   (e4m3; 1 / 127 for int8)
- *   q[m,k]   = e4m3_rne(y / scale), or clamp(rne(y / scale), -127, 127)
+ *   q[m,k]   = e4m3_rne(y * (1 / scale)), or rne(y * (1 / scale)) in -127..127
  * in fp32 from the inputs to the codes (neither h nor y is rounded to x's type
  * on the way, unlike the separate kernels). x, residual, residual_out, weight:
  * BF16, FP16 or FP32 (dtype); residual_out may be residual or x (in place; same

@@ -179,7 +179,8 @@ struct AddNormQuantArgs {
   int64_t ldq;
   float* scale;  // [rows]
   int rows, width;
-  bool vec;  // rows, weight and outputs allow 16-byte loads and 8-byte code stores; width % 8 == 0
+  bool vec;    // bases aligned (16 bytes; codes 8) and rows of all arrays displaced alike
+  bool whole;  // no row is displaced and the width is a multiple of eight
 };
 int launch_add_norm_quant(const AddNormQuantArgs& a, int dtype, int q_dtype, bool pdl, cudaStream_t stream);
 

@@ -14,6 +14,12 @@
 // load, a pair's partner D / 16 lanes away, a group of 32 channels on four
 // neighbouring lanes, and a lane's eight codes are exactly one 32-bit word of a
 // key row or two 16-bit words of a value row.
+//
+// Bound by memory: the projection's row read once, q, codes and (where asked for)
+// the stored values written once. A lane's channels are the same in every head,
+// so a warp takes several heads of one token and gathers its cosines and sines
+// once; how many is chosen so that a short call still has a warp for every head
+// pair and a long one few gathers. Four rows are loaded ahead.
 #include "kernels.h"
 #include "kv4.cuh"
 #include "prologue.cuh"
@@ -21,7 +27,15 @@
 namespace qtts {
 namespace {
 
-constexpr int kRkThreads = 256;
+constexpr int kRkThreads = 128;
+constexpr int kAhead = 4;  // head rows (a lane's parts of them) in flight
+
+// a / s for the s whose correctly rounded reciprocal is r: Markstein's correction of the
+// product a * r by its remainder, which gives the correctly rounded quotient.
+__device__ __forceinline__ float divide(float a, float s, float r) {
+  const float q = a * r;
+  return fmaf(fmaf(-q, s, a), r, q);
+}
 
 // The eight codes of a lane's channels; returns them one a nibble and gives the
 // values that they stand for. lo/hi: minimum and maximum of the group.
@@ -31,15 +45,22 @@ __device__ __forceinline__ uint32_t quantize_group(const float (&y)[8], float lo
   const __nv_bfloat16 zb = __float2bfloat16_rn(lo);
   params = static_cast<uint32_t>(__bfloat16_as_ushort(sb)) | (static_cast<uint32_t>(__bfloat16_as_ushort(zb)) << 16);
   const float s = __bfloat162float(sb), z = __bfloat162float(zb);
-  uint32_t word = 0;
+  // Scales below 2^-120 (and zero) leave the reciprocal's range: plain division there.
+  const bool small = s < 0x1p-120f;
+  const float r = __fdiv_rn(1.0f, s);
+  float c[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    float c = s > 0.f ? rintf(__fdiv_rn(y[i] - z, s)) : 0.f;
-    c = fminf(fmaxf(c, 0.f), 15.f);
-    word |= static_cast<uint32_t>(c) << (4 * i);
-    held[i] = __fadd_rn(__fmul_rn(c, s), z);
+    float q = divide(y[i] - z, s, r);
+    if (small) q = s > 0.f ? __fdiv_rn(y[i] - z, s) : 0.f;
+    q = fminf(fmaxf(q, 0.f), 15.f);
+    c[i] = (q + 12582912.f) - 12582912.f;  // 1.5 * 2^23: to the nearest whole number, ties to even
+    held[i] = fmaf(c[i], s, z);            // c * s is exact
   }
-  return word;
+  // Four codes at a time as one whole number below 2^16 in a float's low bits.
+  const float a = fmaf(c[3], 4096.f, fmaf(c[2], 256.f, fmaf(c[1], 16.f, c[0])));
+  const float b = fmaf(c[7], 4096.f, fmaf(c[6], 256.f, fmaf(c[5], 16.f, c[4])));
+  return __byte_perm(__float_as_uint(a + 8388608.f), __float_as_uint(b + 8388608.f), 0x5410);
 }
 
 template <typename T>
@@ -52,42 +73,24 @@ __device__ __forceinline__ uint4 pack8(const float (&y)[8]) {
 }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kRkThreads) rope_kv4_kernel(const RopeKv4Args a) {
-  constexpr int kLanes = D / 8;      // lanes a head row
+__global__ void __launch_bounds__(kRkThreads) rope_kv4_kernel(const RopeKv4Args a, int passes, int warps_a_token) {
+  constexpr int kLanes = D / 8;          // lanes a head row
+  constexpr int kHeads = 32 / kLanes;    // head rows a pass of a warp
   constexpr int kGroups = D / kKv4Group;
   pdl_launch_dependents();
+  const int64_t warp = static_cast<int64_t>(blockIdx.x) * (kRkThreads / 32) + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  const int64_t t = warp / warps_a_token;
+  if (t >= a.tokens) return;
   pdl_wait();
+  const int l = lane % kLanes;
   const int heads = a.q_heads + 2 * a.cache.kv_heads;
-  const int64_t item = (static_cast<int64_t>(blockIdx.x) * kRkThreads + threadIdx.x) / kLanes;
-  const int l = threadIdx.x % kLanes;
-  const bool live = item < static_cast<int64_t>(a.tokens) * heads;
-  const int64_t t = live ? item / heads : 0;
-  const int head = live ? static_cast<int>(item - t * heads) : 0;
-  const int kv = head - a.q_heads;  // key head, or kv_heads + value head
-  const bool is_q = kv < 0;
-  const bool is_v = kv >= a.cache.kv_heads;
+  const int first = static_cast<int>(warp - t * warps_a_token) * passes * kHeads + lane / kLanes;
+  const T* src = static_cast<const T*>(a.qkv) + t * a.ldqkv + 8 * l;
 
-  const uint4 raw = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.qkv) + t * a.ldqkv + head * D + 8 * l);
-  const T* e = reinterpret_cast<const T*>(&raw);
-  float y[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) y[i] = to_float(e[i]);
-
-  const T* w = static_cast<const T*>(is_q ? a.q_norm : a.k_norm);
-  if (w != nullptr) {
-    float ss = leaf_sumsq(y);
-#pragma unroll
-    for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    if (!is_v) {
-      const float inv = rms_inv(ss, D, a.eps);
-      const uint4 wr = __ldg(reinterpret_cast<const uint4*>(w + 8 * l));
-      const T* we = reinterpret_cast<const T*>(&wr);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] = rms_apply(y[i], inv, to_float(we[i]));
-    }
-  }
   // A token with a position outside the tables gives zeros and is not stored.
   bool ok = true;
+  float cs[8], sn[8];
   if (a.cos != nullptr) {
     int64_t pos[kMaxRopeAxes];
 #pragma unroll
@@ -98,72 +101,120 @@ __global__ void __launch_bounds__(kRkThreads) rope_kv4_kernel(const RopeKv4Args 
         ok = false;
       }
     }
-    if (!ok) record_status(QTTS_ERR_SHAPE);
+    if (!ok && lane == 0) record_status(QTTS_ERR_SHAPE);
     const int j0 = 8 * (l % (kLanes / 2));  // first of this lane's pairs
-    const float sign = l < kLanes / 2 ? -1.f : 1.f;
-    float other[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) other[i] = __shfl_xor_sync(0xffffffffu, y[i], kLanes / 2);
-    if (!is_v) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int j = j0 + i;
-        const int axis = static_cast<int>(a.axis_of[j >> 5] >> (2 * (j & 31))) & 3;
-        const int64_t at = (axis == 0 ? pos[0] : axis == 1 ? pos[1] : axis == 2 ? pos[2] : pos[3]) * (D / 2) + j;
-        y[i] = __fadd_rn(__fmul_rn(y[i], a.cos[at]), sign * __fmul_rn(other[i], a.sin[at]));
-      }
+    for (int i = 0; i < 8; ++i) {
+      const int j = j0 + i;
+      const int axis = static_cast<int>(a.axis_of[j >> 5] >> (2 * (j & 31))) & 3;
+      const int64_t at = (axis == 0 ? pos[0] : axis == 1 ? pos[1] : axis == 2 ? pos[2] : pos[3]) * (D / 2) + j;
+      cs[i] = __ldg(a.cos + at);
+      const float s = __ldg(a.sin + at);
+      sn[i] = l < kLanes / 2 ? -s : s;
     }
   }
-  if (!ok) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = 0.f;
-  }
-  float lo = y[0], hi = y[0];
-#pragma unroll
-  for (int i = 1; i < 8; ++i) lo = nan_min(lo, y[i]), hi = nan_max(hi, y[i]);
-#pragma unroll
-  for (int o = 2; o > 0; o >>= 1) {
-    lo = nan_min(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-    hi = nan_max(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-  }
-  if (!live) return;
-  if (is_q) {
-    *reinterpret_cast<uint4*>(static_cast<T*>(a.q_out) + t * a.ldq + head * D + 8 * l) = pack8<T>(y);
-    return;
-  }
-  uint32_t params;
-  float held[8];
-  const uint32_t word = quantize_group(y, lo, hi, params, held);
-  const int h = is_v ? kv - a.cache.kv_heads : kv;
-  T* values = static_cast<T*>(is_v ? a.v_values : a.k_values);
-  if (values != nullptr) {
-    *reinterpret_cast<uint4*>(values + (t * a.cache.kv_heads + h) * D + 8 * l) = pack8<T>(held);
-  }
   const int64_t slot = a.slots[t];
-  if (slot < 0 || !ok) return;
-  if (slot >= a.cache.pages * a.cache.page_size) {
-    record_status(QTTS_ERR_SHAPE);
-    return;
-  }
-  const int64_t page = slot / a.cache.page_size;
-  const int64_t row = kv4_row(a.cache, page, h, static_cast<int>(slot - page * a.cache.page_size));
-  const int j = l / 4, c = l % 4;
-  if (is_v) {
-    uint16_t* dst = reinterpret_cast<uint16_t*>(a.cache.v_codes + row * (D / 2));
-    dst[(2 * c) * kGroups + j] = static_cast<uint16_t>(word & 0xffffu);
-    dst[(2 * c + 1) * kGroups + j] = static_cast<uint16_t>(word >> 16);
-    if (c == 0) a.cache.v_params[row * kGroups + j] = params;
-  } else {
-    reinterpret_cast<uint32_t*>(a.cache.k_codes + row * (D / 2))[c * kGroups + j] = word;
-    if (c == 0) a.cache.k_params[row * kGroups + j] = params;
+  const bool inside = slot < a.cache.pages * a.cache.page_size;
+  if (!inside && lane == 0) record_status(QTTS_ERR_SHAPE);
+  const bool stored = ok && inside && slot >= 0;
+  const int64_t page = stored ? slot / a.cache.page_size : 0;
+  const int in_page = stored ? static_cast<int>(slot - page * a.cache.page_size) : 0;
+
+  for (int p0 = 0; p0 < passes; p0 += kAhead) {
+    uint4 raw[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int head = first + (p0 + u) * kHeads;
+      raw[u] = make_uint4(0u, 0u, 0u, 0u);
+      if (p0 + u < passes && head < heads) raw[u] = __ldcs(reinterpret_cast<const uint4*>(src + head * D));
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int head = first + (p0 + u) * kHeads;
+      const bool live = p0 + u < passes && head < heads;
+      if (!__any_sync(0xffffffffu, live)) break;
+      const int kv = head - a.q_heads;  // key head, or kv_heads + value head
+      const bool is_q = kv < 0;
+      const bool is_v = kv >= a.cache.kv_heads;
+      const T* e = reinterpret_cast<const T*>(&raw[u]);
+      float y[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = to_float(e[i]);
+      if (__any_sync(0xffffffffu, live && !is_v)) {
+        const T* w = static_cast<const T*>(is_q ? a.q_norm : a.k_norm);
+        float ss = leaf_sumsq(y);
+#pragma unroll
+        for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        if (w != nullptr && !is_v) {
+          const float inv = rms_inv(ss, D, a.eps);
+          const uint4 wr = __ldg(reinterpret_cast<const uint4*>(w + 8 * l));
+          const T* we = reinterpret_cast<const T*>(&wr);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) y[i] = rms_apply(y[i], inv, to_float(we[i]));
+        }
+        if (a.cos != nullptr) {
+          float other[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) other[i] = __shfl_xor_sync(0xffffffffu, y[i], kLanes / 2);
+          if (!is_v) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) y[i] = __fadd_rn(__fmul_rn(y[i], cs[i]), __fmul_rn(other[i], sn[i]));
+          }
+        }
+      }
+      if (!ok) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = 0.f;
+      }
+      if (live && is_q) {
+        *reinterpret_cast<uint4*>(static_cast<T*>(a.q_out) + t * a.ldq + head * D + 8 * l) = pack8<T>(y);
+      }
+      if (!__any_sync(0xffffffffu, live && !is_q)) continue;
+      float lo = y[0], hi = y[0];
+#pragma unroll
+      for (int i = 1; i < 8; ++i) lo = nan_min(lo, y[i]), hi = nan_max(hi, y[i]);
+#pragma unroll
+      for (int o = 2; o > 0; o >>= 1) {
+        lo = nan_min(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+        hi = nan_max(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+      }
+      if (!live || is_q) continue;
+      uint32_t params;
+      float held[8];
+      const uint32_t word = quantize_group(y, lo, hi, params, held);
+      const int h = is_v ? kv - a.cache.kv_heads : kv;
+      T* values = static_cast<T*>(is_v ? a.v_values : a.k_values);
+      if (values != nullptr) {
+        *reinterpret_cast<uint4*>(values + (t * a.cache.kv_heads + h) * D + 8 * l) = pack8<T>(held);
+      }
+      if (!stored) continue;
+      const int64_t row = kv4_row(a.cache, page, h, in_page);
+      const int j = l / 4, c = l % 4;
+      if (is_v) {
+        uint16_t* dst = reinterpret_cast<uint16_t*>(a.cache.v_codes + row * (D / 2));
+        dst[(2 * c) * kGroups + j] = static_cast<uint16_t>(word & 0xffffu);
+        dst[(2 * c + 1) * kGroups + j] = static_cast<uint16_t>(word >> 16);
+        if (c == 0) a.cache.v_params[row * kGroups + j] = params;
+      } else {
+        reinterpret_cast<uint32_t*>(a.cache.k_codes + row * (D / 2))[c * kGroups + j] = word;
+        if (c == 0) a.cache.k_params[row * kGroups + j] = params;
+      }
+    }
   }
 }
 
 template <typename T, int D>
 int launch_rk(const RopeKv4Args& a, bool pdl, cudaStream_t stream) {
-  const int64_t lanes = static_cast<int64_t>(a.tokens) * (a.q_heads + 2 * a.cache.kv_heads) * (D / 8);
+  constexpr int kHeads = 32 / (D / 8);
+  const int total = (a.q_heads + 2 * a.cache.kv_heads + kHeads - 1) / kHeads;  // passes a token needs
+  // A warp for every pass while that is less than some eight warps an SM; then longer warps, up to
+  // 16 passes, which read their angles once.
+  int passes = 1;
+  while (passes < 16 && passes < total && static_cast<int64_t>(a.tokens) * total >= 16ll * kNumSMs * passes) passes *= 2;
+  const int warps_a_token = (total + passes - 1) / passes;
+  const int64_t warps = static_cast<int64_t>(a.tokens) * warps_a_token;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>((lanes + kRkThreads - 1) / kRkThreads));
+  cfg.gridDim = dim3(static_cast<unsigned>((warps + kRkThreads / 32 - 1) / (kRkThreads / 32)));
   cfg.blockDim = dim3(kRkThreads);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
@@ -173,7 +224,8 @@ int launch_rk(const RopeKv4Args& a, bool pdl, cudaStream_t stream) {
     cfg.attrs = attr;
     cfg.numAttrs = 1;
   }
-  return cudaLaunchKernelEx(&cfg, rope_kv4_kernel<T, D>, a) == cudaSuccess ? QTTS_OK : QTTS_ERR_LAUNCH;
+  return cudaLaunchKernelEx(&cfg, rope_kv4_kernel<T, D>, a, passes, warps_a_token) == cudaSuccess ? QTTS_OK
+                                                                                                 : QTTS_ERR_LAUNCH;
 }
 
 }  // namespace
@@ -211,7 +263,6 @@ extern "C" int qtts_rope_kv4_append(const void* qkv, int64_t ldqkv, int dtype, i
   if ((k_values == nullptr) != (v_values == nullptr)) return QTTS_ERR_NULL;
   const int64_t width = static_cast<int64_t>(q_heads + 2 * kv_heads) * head_dim;
   if (ldqkv < width || ldq < static_cast<int64_t>(q_heads) * head_dim) return QTTS_ERR_SHAPE;
-  if (static_cast<int64_t>(tokens) * width / 8 > (static_cast<int64_t>(1) << 38)) return QTTS_ERR_SHAPE;
   const auto al = [](const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; };
   if (!al(qkv, 16) || !al(q_out, 16) || !al(q_norm, 16) || !al(k_norm, 16) || !al(k_values, 16) ||
       !al(v_values, 16) || !al(k_codes, 16) || !al(v_codes, 16) || !al(k_params, 16) || !al(v_params, 16) ||
