@@ -20,6 +20,8 @@
 // so a warp takes several heads of one token and gathers its cosines and sines
 // once; how many is chosen so that a short call still has a warp for every head
 // pair and a long one few gathers. Four rows are loaded ahead.
+#include <type_traits>
+
 #include "kernels.h"
 #include "kv4.cuh"
 #include "prologue.cuh"
@@ -27,7 +29,6 @@
 namespace qtts {
 namespace {
 
-constexpr int kRkThreads = 128;
 constexpr int kAhead = 4;  // head rows (a lane's parts of them) in flight
 
 // a / s for the s whose correctly rounded reciprocal is r: Markstein's correction of the
@@ -41,19 +42,19 @@ __device__ __forceinline__ float divide(float a, float s, float r) {
 // values that they stand for. lo/hi: minimum and maximum of the group.
 __device__ __forceinline__ uint32_t quantize_group(const float (&y)[8], float lo, float hi, uint32_t& params,
                                                    float (&held)[8]) {
-  const __nv_bfloat16 sb = __float2bfloat16_rn(__fdiv_rn(hi - lo, 15.0f));
+  const __nv_bfloat16 sb = __float2bfloat16_rn(divide(hi - lo, 15.0f, 1.0f / 15.0f));
   const __nv_bfloat16 zb = __float2bfloat16_rn(lo);
   params = static_cast<uint32_t>(__bfloat16_as_ushort(sb)) | (static_cast<uint32_t>(__bfloat16_as_ushort(zb)) << 16);
   const float s = __bfloat162float(sb), z = __bfloat162float(zb);
-  // Scales below 2^-120 (and zero) leave the reciprocal's range: plain division there.
-  const bool small = s < 0x1p-120f;
-  const float r = __fdiv_rn(1.0f, s);
+  // A scale below 2^-60 is divided by 2^64 times larger, as is what it divides, so that
+  // reciprocal and remainder stay in range.
+  const float up = s < 0x1p-60f ? 0x1p64f : 1.f;
+  const float su = s * up;
+  const float r = s > 0.f ? __frcp_rn(su) : 0.f;
   float c[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    float q = divide(y[i] - z, s, r);
-    if (small) q = s > 0.f ? __fdiv_rn(y[i] - z, s) : 0.f;
-    q = fminf(fmaxf(q, 0.f), 15.f);
+    const float q = fminf(fmaxf(divide((y[i] - z) * up, su, r), 0.f), 15.f);
     c[i] = (q + 12582912.f) - 12582912.f;  // 1.5 * 2^23: to the nearest whole number, ties to even
     held[i] = fmaf(c[i], s, z);            // c * s is exact
   }
@@ -73,19 +74,22 @@ __device__ __forceinline__ uint4 pack8(const float (&y)[8]) {
 }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kRkThreads) rope_kv4_kernel(const RopeKv4Args a, int passes, int warps_a_token) {
+__global__ void __launch_bounds__(32, 20) rope_kv4_kernel(const RopeKv4Args a, int passes, int warps_a_token) {
   constexpr int kLanes = D / 8;          // lanes a head row
   constexpr int kHeads = 32 / kLanes;    // head rows a pass of a warp
   constexpr int kGroups = D / kKv4Group;
   pdl_launch_dependents();
-  const int64_t warp = static_cast<int64_t>(blockIdx.x) * (kRkThreads / 32) + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  const int64_t t = warp / warps_a_token;
-  if (t >= a.tokens) return;
   pdl_wait();
+  // One warp a CTA: token, passes and kinds are the CTA's, so every branch is uniform.
+  const int lane = threadIdx.x;
+  const int64_t t = blockIdx.x / warps_a_token;
   const int l = lane % kLanes;
-  const int heads = a.q_heads + 2 * a.cache.kv_heads;
-  const int first = static_cast<int>(warp - t * warps_a_token) * passes * kHeads + lane / kLanes;
+  const int sub = lane / kLanes;  // which of the pass's heads
+  const int kvh = a.cache.kv_heads;
+  // A pass takes kHeads heads of one kind: the q passes first, then k, then v.
+  const int nq = (a.q_heads + kHeads - 1) / kHeads, nk = (kvh + kHeads - 1) / kHeads;
+  const int p_first = static_cast<int>(blockIdx.x % warps_a_token) * passes;
+  const int p_end = min(p_first + passes, nq + 2 * nk);
   const T* src = static_cast<const T*>(a.qkv) + t * a.ldqkv + 8 * l;
 
   // A token with a position outside the tables gives zeros and is not stored.
@@ -120,84 +124,92 @@ __global__ void __launch_bounds__(kRkThreads) rope_kv4_kernel(const RopeKv4Args 
   const int64_t page = stored ? slot / a.cache.page_size : 0;
   const int in_page = stored ? static_cast<int>(slot - page * a.cache.page_size) : 0;
 
-  for (int p0 = 0; p0 < passes; p0 += kAhead) {
-    uint4 raw[kAhead];
+  // Head (within its kind) of this lane in pass p, and the pass's kind: 0 q, 1 k, 2 v.
+  const auto kind_of = [&](int p) { return p < nq ? 0 : p < nq + nk ? 1 : 2; };
+  const auto head_of = [&](int p, int kind) { return (p - (kind == 0 ? 0 : kind == 1 ? nq : nq + nk)) * kHeads + sub; };
+
+  const auto norm = [&](float(&y)[8], const void* weight) {
+    float ss = leaf_sumsq(y);
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      const int head = first + (p0 + u) * kHeads;
-      raw[u] = make_uint4(0u, 0u, 0u, 0u);
-      if (p0 + u < passes && head < heads) raw[u] = __ldcs(reinterpret_cast<const uint4*>(src + head * D));
+    for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    const float inv = rsqrtf(ss * (1.0f / D) + a.eps);
+    const uint4 wr = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(weight) + 8 * l));
+    const T* we = reinterpret_cast<const T*>(&wr);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = rms_apply(y[i], inv, to_float(we[i]));
+  };
+  const auto turn = [&](float(&y)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float other = __shfl_xor_sync(0xffffffffu, y[i], kLanes / 2);
+      y[i] = __fadd_rn(__fmul_rn(y[i], cs[i]), __fmul_rn(other, sn[i]));
     }
+  };
+  const auto quantize = [&](const float(&y)[8], bool live, int h, uint8_t* codes, uint32_t* all_params, void* values,
+                            auto is_value) {
+    float lo = y[0], hi = y[0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) lo = nan_min(lo, y[i]), hi = nan_max(hi, y[i]);
+#pragma unroll
+    for (int o = 2; o > 0; o >>= 1) {
+      lo = nan_min(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+      hi = nan_max(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+    }
+    uint32_t params;
+    float held[8];
+    const uint32_t word = quantize_group(y, lo, hi, params, held);
+    if (values != nullptr && live) {
+      __stcs(reinterpret_cast<uint4*>(static_cast<T*>(values) + (t * kvh + h) * D + 8 * l), pack8<T>(held));
+    }
+    if (stored && live) {
+      const int64_t row = kv4_row(a.cache, page, h, in_page);
+      const int j = l / 4, c = l % 4;
+      if constexpr (decltype(is_value)::value) {
+        uint16_t* dst = reinterpret_cast<uint16_t*>(codes + row * (D / 2));
+        dst[(2 * c) * kGroups + j] = static_cast<uint16_t>(word & 0xffffu);
+        dst[(2 * c + 1) * kGroups + j] = static_cast<uint16_t>(word >> 16);
+      } else {
+        reinterpret_cast<uint32_t*>(codes + row * (D / 2))[c * kGroups + j] = word;
+      }
+      if (c == 0) all_params[row * kGroups + j] = params;
+    }
+  };
+
+  const auto fetch = [&](int p) {
+    uint4 raw = make_uint4(0u, 0u, 0u, 0u);
+    const int kind = kind_of(p), h = head_of(p, kind);
+    if (p < p_end && ok && h < (kind == 0 ? a.q_heads : kvh)) {
+      raw = __ldcs(reinterpret_cast<const uint4*>(
+          src + (h + (kind == 0 ? 0 : kind == 1 ? a.q_heads : a.q_heads + kvh)) * D));
+    }
+    return raw;
+  };
+  uint4 raw[kAhead];
+#pragma unroll
+  for (int u = 0; u < kAhead; ++u) raw[u] = fetch(p_first + u);
+  for (int p0 = p_first; p0 < p_end; p0 += kAhead) {
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
-      const int head = first + (p0 + u) * kHeads;
-      const bool live = p0 + u < passes && head < heads;
-      if (!__any_sync(0xffffffffu, live)) break;
-      const int kv = head - a.q_heads;  // key head, or kv_heads + value head
-      const bool is_q = kv < 0;
-      const bool is_v = kv >= a.cache.kv_heads;
+      const int p = p0 + u;
+      if (p >= p_end) break;
+      const int kind = kind_of(p), h = head_of(p, kind);
+      const bool live = h < (kind == 0 ? a.q_heads : kvh);
       const T* e = reinterpret_cast<const T*>(&raw[u]);
       float y[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) y[i] = to_float(e[i]);
-      if (__any_sync(0xffffffffu, live && !is_v)) {
-        const T* w = static_cast<const T*>(is_q ? a.q_norm : a.k_norm);
-        float ss = leaf_sumsq(y);
-#pragma unroll
-        for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        if (w != nullptr && !is_v) {
-          const float inv = rms_inv(ss, D, a.eps);
-          const uint4 wr = __ldg(reinterpret_cast<const uint4*>(w + 8 * l));
-          const T* we = reinterpret_cast<const T*>(&wr);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) y[i] = rms_apply(y[i], inv, to_float(we[i]));
-        }
-        if (a.cos != nullptr) {
-          float other[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) other[i] = __shfl_xor_sync(0xffffffffu, y[i], kLanes / 2);
-          if (!is_v) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) y[i] = __fadd_rn(__fmul_rn(y[i], cs[i]), __fmul_rn(other[i], sn[i]));
-          }
-        }
+      raw[u] = fetch(p + kAhead);
+      if (kind == 2) {
+        quantize(y, live, h, a.cache.v_codes, a.cache.v_params, a.v_values, std::true_type{});
+        continue;
       }
-      if (!ok) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = 0.f;
-      }
-      if (live && is_q) {
-        *reinterpret_cast<uint4*>(static_cast<T*>(a.q_out) + t * a.ldq + head * D + 8 * l) = pack8<T>(y);
-      }
-      if (!__any_sync(0xffffffffu, live && !is_q)) continue;
-      float lo = y[0], hi = y[0];
-#pragma unroll
-      for (int i = 1; i < 8; ++i) lo = nan_min(lo, y[i]), hi = nan_max(hi, y[i]);
-#pragma unroll
-      for (int o = 2; o > 0; o >>= 1) {
-        lo = nan_min(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-        hi = nan_max(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-      }
-      if (!live || is_q) continue;
-      uint32_t params;
-      float held[8];
-      const uint32_t word = quantize_group(y, lo, hi, params, held);
-      const int h = is_v ? kv - a.cache.kv_heads : kv;
-      T* values = static_cast<T*>(is_v ? a.v_values : a.k_values);
-      if (values != nullptr) {
-        *reinterpret_cast<uint4*>(values + (t * a.cache.kv_heads + h) * D + 8 * l) = pack8<T>(held);
-      }
-      if (!stored) continue;
-      const int64_t row = kv4_row(a.cache, page, h, in_page);
-      const int j = l / 4, c = l % 4;
-      if (is_v) {
-        uint16_t* dst = reinterpret_cast<uint16_t*>(a.cache.v_codes + row * (D / 2));
-        dst[(2 * c) * kGroups + j] = static_cast<uint16_t>(word & 0xffffu);
-        dst[(2 * c + 1) * kGroups + j] = static_cast<uint16_t>(word >> 16);
-        if (c == 0) a.cache.v_params[row * kGroups + j] = params;
-      } else {
-        reinterpret_cast<uint32_t*>(a.cache.k_codes + row * (D / 2))[c * kGroups + j] = word;
-        if (c == 0) a.cache.k_params[row * kGroups + j] = params;
+      const void* weight = kind == 0 ? a.q_norm : a.k_norm;
+      if (weight != nullptr) norm(y, weight);
+      if (a.cos != nullptr) turn(y);
+      if (kind == 1) {
+        quantize(y, live, h, a.cache.k_codes, a.cache.k_params, a.k_values, std::false_type{});
+      } else if (live) {
+        *reinterpret_cast<uint4*>(static_cast<T*>(a.q_out) + t * a.ldq + h * D + 8 * l) = pack8<T>(y);
       }
     }
   }
@@ -206,7 +218,8 @@ __global__ void __launch_bounds__(kRkThreads) rope_kv4_kernel(const RopeKv4Args 
 template <typename T, int D>
 int launch_rk(const RopeKv4Args& a, bool pdl, cudaStream_t stream) {
   constexpr int kHeads = 32 / (D / 8);
-  const int total = (a.q_heads + 2 * a.cache.kv_heads + kHeads - 1) / kHeads;  // passes a token needs
+  // Passes a token needs.
+  const int total = (a.q_heads + kHeads - 1) / kHeads + 2 * ((a.cache.kv_heads + kHeads - 1) / kHeads);
   // A warp for every pass while that is less than some eight warps an SM; then longer warps, up to
   // 16 passes, which read their angles once.
   int passes = 1;
@@ -214,8 +227,9 @@ int launch_rk(const RopeKv4Args& a, bool pdl, cudaStream_t stream) {
   const int warps_a_token = (total + passes - 1) / passes;
   const int64_t warps = static_cast<int64_t>(a.tokens) * warps_a_token;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>((warps + kRkThreads / 32 - 1) / (kRkThreads / 32)));
-  cfg.blockDim = dim3(kRkThreads);
+  if (warps > 0x7fffffff) return QTTS_ERR_SHAPE;
+  cfg.gridDim = dim3(static_cast<unsigned>(warps));
+  cfg.blockDim = dim3(32);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   if (pdl) {
