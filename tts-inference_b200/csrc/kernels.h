@@ -238,6 +238,8 @@ struct Kv4AttnArgs {
   float* parts;   // workspace [total_q, q_heads, splits, head_dim] and its statistics
   float2* stats;  // [total_q, q_heads, splits]: running maximum (log2) and sum
 };
+// Many rows a request (csrc/kv4_prompt.cu).
+int launch_kv4_prompt(const Kv4AttnArgs& a, int dtype, int head_dim, bool pdl, cudaStream_t stream);
 int launch_kv4_attention(const Kv4AttnArgs& a, int dtype, int head_dim, bool pdl, cudaStream_t stream);
 
 #ifdef QTTS_TRACE

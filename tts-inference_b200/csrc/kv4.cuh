@@ -35,4 +35,16 @@ __device__ __forceinline__ int64_t kv4_row(const Kv4Cache& c, int64_t page, int 
 __device__ __forceinline__ float kv4_scale(uint32_t p) { return __uint_as_float(p << 16); }
 __device__ __forceinline__ float kv4_min(uint32_t p) { return __uint_as_float(p & 0xffff0000u); }
 
+// First row and number of new tokens of request b, checked against the arguments.
+__device__ __forceinline__ bool request_rows(const Kv4AttnArgs& a, int b, int& start, int& n) {
+  if (a.q_starts == nullptr) {
+    start = b * a.max_q;
+    n = a.max_q;
+    return true;
+  }
+  start = a.q_starts[b];
+  n = a.q_starts[b + 1] - start;
+  return start >= 0 && n >= 0 && n <= a.max_q && start <= a.total_q - n;
+}
+
 }  // namespace qtts

@@ -98,18 +98,6 @@ __device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
   return v;
 }
 
-// First row and number of new tokens of request b, checked against the arguments.
-__device__ __forceinline__ bool request_rows(const Kv4AttnArgs& a, int b, int& start, int& n) {
-  if (a.q_starts == nullptr) {
-    start = b * a.max_q;
-    n = a.max_q;
-    return true;
-  }
-  start = a.q_starts[b];
-  n = a.q_starts[b + 1] - start;
-  return start >= 0 && n >= 0 && n <= a.max_q && start <= a.total_q - n;
-}
-
 template <int D>
 struct RowsSmem {
   static constexpr int kCodes = kTile * D / 2;              // bytes of a tile's key (or value) codes
@@ -698,6 +686,10 @@ __global__ void __launch_bounds__(128) kv4_join_kernel(const Kv4AttnArgs a, int 
   for (int i = 0; i < D / 32; ++i) dst[i] = from_float<T>(out[i] * inv);
 }
 
+// Rows a request from which whole 128-row tiles are the faster.
+constexpr int64_t kPromptRows = 64;
+bool kv4_takes_prompt(int64_t max_q, int share) { return max_q * share >= kPromptRows; }
+
 // How a call is laid out: rows a CTA, and CTAs that share the tokens of one (request, key
 // head, row block).
 struct RowsPlan {
@@ -788,6 +780,9 @@ int launch_ka(const Kv4AttnArgs& a, bool pdl, cudaStream_t stream) {
 }  // namespace
 
 int launch_kv4_attention(const Kv4AttnArgs& a, int dtype, int head_dim, bool pdl, cudaStream_t stream) {
+  if (kv4_takes_prompt(a.max_q, a.q_heads / a.cache.kv_heads)) {
+    return launch_kv4_prompt(a, dtype, head_dim, pdl, stream);
+  }
   if (dtype == QTTS_BF16) {
     return head_dim == 128 ? launch_ka<__nv_bfloat16, 128>(a, pdl, stream)
                            : launch_ka<__nv_bfloat16, 64>(a, pdl, stream);
@@ -801,6 +796,7 @@ extern "C" int64_t qtts_kv4_attention_workspace(int total_q, int max_q, int batc
                                                 int head_dim, int64_t max_tokens) {
   using namespace qtts;
   if (total_q < 1 || max_q < 1 || batch < 1 || kv_heads < 1 || q_heads < 1 || q_heads % kv_heads != 0) return 0;
+  if (kv4_takes_prompt(max_q, q_heads / kv_heads)) return 0;
   const RowsPlan p = plan_rows(max_q, q_heads / kv_heads, kv_heads, batch, max_tokens);
   if (p.splits <= kMaxCluster) return 0;
   return static_cast<int64_t>(total_q) * q_heads * p.splits * (head_dim + 2) * 4;

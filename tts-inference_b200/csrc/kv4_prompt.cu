@@ -1,0 +1,500 @@
+// Attention over the 4-bit cache for many rows a request (prompts, chunks): the
+// 5th-generation tensor cores, 128 rows a tile, a row being a (new token, query
+// head) pair that shares the key head; see kv4_attention.cu for the definition.
+//
+// A CTA takes one or two tiles of rows of one (request, key head) and walks over
+// the tokens, 128 at a time:
+//   * warps 8-11 turn the tile's codes into bf16 in shared memory, one token a
+//     thread: (128 + code) by a mask, minus 128 (exact), times scale plus minimum in
+//     one fused multiply-add, so a key or value is rounded once. Keys and values
+//     have the same layout there, 128-byte rows of 64 channels a token,
+//     swizzled: the keys are the K-major B operand of S = Q K^T, the values the
+//     transposed (N-contiguous) B operand of O += P V. The order of channels
+//     within a row is the order in which masks give pairs; q is stored to match, and
+//     the outputs are put back in order at the end;
+//   * warp 12 issues the products: S of one tile while the other tile's
+//     probabilities are made, P from tensor memory, where it replaces S. The
+//     products of one tile run in the order issued, so S(j + 1) may overwrite P(j)
+//     and whoever has seen S(j) knows that O has taken P(j - 1);
+//   * warps 0-3 and 4-7 (a thread a row, no exchange between threads) take the
+//     running maximum and sum in fp32 and write P as bf16. The reference maximum
+//     follows only when the maximum has grown by more than 2^8, so O is rescaled
+//     rarely; the row's sum divides at the end.
+// Bound by the two products (2 x 512 cycles a tile of 128 x 128 x 128) and, as
+// much, by 16384 exponentials a tile at 16 a cycle.
+#include <type_traits>
+
+#include "kernels.h"
+#include "kv4.cuh"
+#include "tmem.cuh"
+
+namespace qtts {
+namespace {
+
+constexpr int kPmTile = 128;  // rows of a tile, and tokens at a time
+constexpr int kPmStages = 2;
+constexpr int kPmDqWarp = 8;   // first of four warps that make the operands
+constexpr int kPmMmaWarp = 12;
+constexpr int kPmThreads = 13 * 32;
+
+template <int D>
+struct PromptSmem {
+  static constexpr int kTileBytes = kPmTile * D * 2;  // a tile of q, keys or values in bf16
+  static constexpr int kQ = 0;
+  static constexpr int kK = 2 * kTileBytes;
+  static constexpr int kV = kK + kPmStages * kTileBytes;
+  static constexpr int kBars = kV + kPmStages * kTileBytes;
+  static constexpr int kBytes = kBars + 256 + 1024;  // barriers; slack to align the base to 1024
+};
+
+__device__ __forceinline__ float ex2f(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+// (code * s + z) of nibbles n and n + 4 of a word, as a bf16 pair.
+__device__ __forceinline__ uint32_t nibbles_to_bf16(uint32_t w, int n, uint32_t s, uint32_t z) {
+  uint32_t x = ((w >> (4 * n)) & 0x000F000Fu) | 0x43004300u;  // 128 + code
+  asm("sub.rn.bf16x2 %0, %0, %1;" : "+r"(x) : "r"(0x43004300u));
+  asm("fma.rn.bf16x2 %0, %0, %1, %2;" : "+r"(x) : "r"(s), "r"(z));
+  return x;
+}
+__device__ __forceinline__ void sts128(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+// Byte offset of 16-byte chunk `chunk` (eight channels) of row `row` of a tile.
+__device__ __forceinline__ uint32_t tile_offset(int row, int chunk) {
+  return static_cast<uint32_t>((chunk >> 3) * (kPmTile * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4));
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kPmThreads, 1)
+    kv4_prompt_kernel(const Kv4AttnArgs a, int tiles_a_cta, uint64_t wait_ns) {
+  using S = PromptSmem<D>;
+  constexpr int NG = D / kKv4Group;
+  constexpr int kWords = D / 8;  // 32-bit words of codes a row; chunks of eight channels
+  constexpr uint32_t kIdescS = umma_idesc(1u, 1u, kPmTile, kPmTile);
+  constexpr uint32_t kIdescO = umma_idesc(1u, 1u, kPmTile, D) | kUmmaBTransposed;
+  constexpr uint32_t kColS = 0, kColO = 2 * kPmTile;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* kfull = reinterpret_cast<uint64_t*>(smem + S::kBars);
+  uint64_t* kempty = kfull + kPmStages;
+  uint64_t* vfull = kempty + kPmStages;
+  uint64_t* vempty = vfull + kPmStages;
+  uint64_t* sfull = vempty + kPmStages;  // [tile]: S is there (and O has taken the P before)
+  uint64_t* pfull = sfull + 2;           // [tile]: P is there
+  uint64_t* odone = pfull + 2;           // [tile]: all of O is there
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(odone + 2);
+
+  const int tid = threadIdx.x;
+  const int warp = tid >> 5;
+  const int lane = tid & 31;
+  if (tid == 0) {
+    for (int s = 0; s < kPmStages; ++s) {
+      mbar_init(&kfull[s], kPmTile);
+      mbar_init(&kempty[s], 1);
+      mbar_init(&vfull[s], kPmTile);
+      mbar_init(&vempty[s], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sfull[i], 1);
+      mbar_init(&pfull[i], kPmTile);
+      mbar_init(&odone[i], 1);
+    }
+    fence_mbarrier_init();
+  }
+  if (warp == kPmMmaWarp) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
+  pdl_launch_dependents();
+  pdl_wait();
+
+  // The longest blocks first: with `causal` the last rows see most.
+  const int rb = static_cast<int>(gridDim.x - 1 - blockIdx.x);
+  const int kvh = blockIdx.y;
+  const int b = blockIdx.z;
+  int start = 0, n = 0;
+  bool fine = request_rows(a, b, start, n);
+  int len = a.lengths[b];
+  fine = fine && len >= 0 && len <= static_cast<int64_t>(a.table_cols) * a.cache.page_size &&
+         (len == 0 || a.cache.pages > 0);
+  if (!fine) {
+    if (tid == 0) record_status(QTTS_ERR_SHAPE);
+    len = 0;
+    if (!request_rows(a, b, start, n)) n = 0;  // rows that cannot be told are not written
+  }
+  const int share = a.q_heads / a.cache.kv_heads;
+  const int rows = n * share;
+  const int r0 = rb * tiles_a_cta * kPmTile;
+  // Tiles of rows that exist, and the 128-token steps that each of them needs.
+  int steps[2];
+  int kmax = 0;  // tokens that any row sees
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int first = r0 + i * kPmTile;
+    steps[i] = 0;
+    if (i < tiles_a_cta && first < rows) {
+      const int last = (min(rows, first + kPmTile) - 1) / share;
+      const int sees = max(0, a.causal ? len - n + last + 1 : len);
+      steps[i] = (sees + kPmTile - 1) / kPmTile;
+      kmax = max(kmax, sees);
+    }
+  }
+  const int most = max(steps[0], steps[1]);
+
+  // q in bf16, channels of a chunk in the order 0 4 1 5 2 6 3 7.
+  if (most > 0) {
+    for (int i = tid; i < tiles_a_cta * kPmTile * kWords; i += kPmThreads) {
+      const int r = i / kWords, ch = i % kWords;
+      uint4 u = make_uint4(0u, 0u, 0u, 0u);
+      if (r0 + r < rows) {
+        const int rr = r0 + r;
+        u = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) +
+                                            static_cast<int64_t>(start + rr / share) * a.q_token_stride +
+                                            (kvh * share + rr % share) * a.q_head_stride + 8 * ch);
+      }
+      if constexpr (!std::is_same<T, __nv_bfloat16>::value) {
+        const __half* e = reinterpret_cast<const __half*>(&u);
+        u = make_uint4(pack_bf16x2(__half2float(e[0]), __half2float(e[1])),
+                       pack_bf16x2(__half2float(e[2]), __half2float(e[3])),
+                       pack_bf16x2(__half2float(e[4]), __half2float(e[5])),
+                       pack_bf16x2(__half2float(e[6]), __half2float(e[7])));
+      }
+      sts128(smem_u32(smem + S::kQ) + (r >> 7) * S::kTileBytes + tile_offset(r & 127, ch),
+             __byte_perm(u.x, u.z, 0x5410), __byte_perm(u.x, u.z, 0x7632), __byte_perm(u.y, u.w, 0x5410),
+             __byte_perm(u.y, u.w, 0x7632));
+    }
+    fence_proxy_async_smem();
+  }
+  __syncthreads();
+
+  if (warp >= kPmDqWarp && warp < kPmMmaWarp) {
+    // ---------------- operands: one token a thread ----------------
+    const int t = tid - kPmDqWarp * 32;
+    const int per_page = a.cache.page_size / 16;
+    const int32_t* table = a.table + b * a.ld_table;
+    int col = (t / 16) / per_page, off = (t / 16) - col * per_page;
+    const int dcol = (kPmTile / 16) / per_page, doff = (kPmTile / 16) - dcol * per_page;
+    // What every row of the block sees from here on: below it no row is masked.
+    const int first_lim = a.causal ? len - n + r0 / share + 1 : len;
+    uint4 kc[NG], vc[NG];
+    uint32_t kp[NG], vp[NG];
+    auto fetch = [&](int j) {  // codes and params of this thread's token of step j
+      const int tok = j * kPmTile + t;
+#pragma unroll
+      for (int i = 0; i < NG; ++i) kc[i] = vc[i] = make_uint4(0u, 0u, 0u, 0u), kp[i] = vp[i] = 0u;
+      if (tok < kmax) {
+        int64_t page = table[col];
+        if (page < 0 || page >= a.cache.pages) {
+          record_status(QTTS_ERR_SHAPE);
+          page = 0;
+        }
+        const int64_t row = kv4_row(a.cache, page, kvh, 16 * off + (t & 15));
+        const uint4* k4 = reinterpret_cast<const uint4*>(a.cache.k_codes + row * (D / 2));
+        const uint4* v4 = reinterpret_cast<const uint4*>(a.cache.v_codes + row * (D / 2));
+#pragma unroll
+        for (int i = 0; i < NG; ++i) kc[i] = __ldg(k4 + i), vc[i] = __ldg(v4 + i);
+        const uint2* p2 = reinterpret_cast<const uint2*>(a.cache.k_params + row * NG);
+        const uint2* q2 = reinterpret_cast<const uint2*>(a.cache.v_params + row * NG);
+#pragma unroll
+        for (int i = 0; i < NG / 2; ++i) {
+          const uint2 x = __ldg(p2 + i), y = __ldg(q2 + i);
+          kp[2 * i] = x.x, kp[2 * i + 1] = x.y, vp[2 * i] = y.x, vp[2 * i + 1] = y.y;
+        }
+      }
+      col += dcol, off += doff;
+      if (off >= per_page) off -= per_page, ++col;
+    };
+    if (most > 0) fetch(0);
+    bool ok = true;
+    for (int j = 0; ok && j < most; ++j) {
+      const int s = j % kPmStages;
+      if (j * kPmTile + kPmTile > first_lim) {
+        // Rows that do not see a token must not meet its NaN or infinity (0 * NaN): a token with
+        // one among its values becomes zeros there, and NaN in its key for the rows that see it.
+        bool bad = false;
+#pragma unroll
+        for (int i = 0; i < NG; ++i) {
+          bad = bad || (vp[i] & 0x7F80u) == 0x7F80u || (vp[i] & 0x7F800000u) == 0x7F800000u;
+        }
+        if (bad) {
+#pragma unroll
+          for (int i = 0; i < NG; ++i) vp[i] = 0u, kp[i] = 0x7FC07FC0u;
+        }
+      }
+      if (j >= kPmStages) ok = mbar_wait_bounded(&kempty[s], ((j / kPmStages) - 1) & 1, wait_ns);
+      const uint32_t kt = smem_u32(smem + S::kK) + s * S::kTileBytes;
+      const uint32_t vt = smem_u32(smem + S::kV) + s * S::kTileBytes;
+      // Keys: word c * NG + g holds channels 32 g + 8 c .. + 7, one group; chunk 4 g + c.
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        const uint32_t sc = __byte_perm(kp[g], 0u, 0x1010), z = __byte_perm(kp[g], 0u, 0x3232);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const int wi = c * NG + g;
+          const uint32_t w = reinterpret_cast<const uint32_t*>(kc)[wi];
+          sts128(kt + tile_offset(t, 4 * g + c), nibbles_to_bf16(w, 0, sc, z), nibbles_to_bf16(w, 1, sc, z),
+                 nibbles_to_bf16(w, 2, sc, z), nibbles_to_bf16(w, 3, sc, z));
+        }
+      }
+      fence_proxy_async_smem();
+      mbar_arrive(&kfull[s]);
+      if (ok && j >= kPmStages) ok = mbar_wait_bounded(&vempty[s], ((j / kPmStages) - 1) & 1, wait_ns);
+      // Values: word wi holds four channels each of two neighbouring groups in its halves.
+#pragma unroll
+      for (int h = 0; h < NG / 2; ++h) {
+        const uint32_t sc = __byte_perm(vp[2 * h], vp[2 * h + 1], 0x5410);
+        const uint32_t z = __byte_perm(vp[2 * h], vp[2 * h + 1], 0x7632);
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          const int wi = c * (NG / 2) + h;
+          const uint32_t w = reinterpret_cast<const uint32_t*>(vc)[wi];
+          sts128(vt + tile_offset(t, wi), nibbles_to_bf16(w, 0, sc, z), nibbles_to_bf16(w, 1, sc, z),
+                 nibbles_to_bf16(w, 2, sc, z), nibbles_to_bf16(w, 3, sc, z));
+        }
+      }
+      fence_proxy_async_smem();
+      mbar_arrive(&vfull[s]);
+      if (j + 1 < most) fetch(j + 1);
+    }
+    if (!ok) record_status(QTTS_ERR_TIMEOUT);
+  } else if (warp == kPmMmaWarp) {
+    // ---------------- the products ----------------
+    if (lane == 0 && most > 0) {
+      const uint32_t qa = smem_u32(smem + S::kQ), ka = smem_u32(smem + S::kK), va = smem_u32(smem + S::kV);
+      auto scores = [&](int i, int s) {
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) {
+          const uint32_t o = (ks / 4) * (kPmTile * 128) + (ks % 4) * 32;
+          umma_f16_ss(tmem + kColS + i * kPmTile, smem_desc_k_sw128(qa + i * S::kTileBytes + o),
+                      smem_desc_k_sw128(ka + s * S::kTileBytes + o), kIdescS, ks != 0 ? 1u : 0u);
+        }
+        tc_commit(&sfull[i]);
+      };
+      bool ok = mbar_wait_bounded(&kfull[0], 0, wait_ns);
+      tc_fence_after();
+      for (int i = 0; ok && i < 2; ++i) {
+        if (steps[i] > 0) scores(i, 0);
+      }
+      tc_commit(&kempty[0]);
+      for (int j = 0; ok && j < most; ++j) {
+        const int s = j % kPmStages;
+        for (int i = 0; ok && i < 2; ++i) {
+          if (j >= steps[i]) continue;
+          ok = mbar_wait_bounded(&pfull[i], j & 1, wait_ns) &&
+               mbar_wait_bounded(&vfull[s], (j / kPmStages) & 1, wait_ns);
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll
+          for (int ks = 0; ks < kPmTile / 16; ++ks) {
+            umma_f16_ts(tmem + kColO + i * D, tmem + kColS + i * kPmTile + 8 * ks,
+                        smem_desc_mn_sw128(va + s * S::kTileBytes + ks * 2048, kPmTile * 128, 1024), kIdescO,
+                        (j | ks) != 0 ? 1u : 0u);
+          }
+          if (j + 1 == steps[i]) tc_commit(&odone[i]);
+          if (j + 1 < steps[i]) {
+            const int s1 = (j + 1) % kPmStages;
+            ok = mbar_wait_bounded(&kfull[s1], ((j + 1) / kPmStages) & 1, wait_ns);
+            if (!ok) break;
+            tc_fence_after();
+            scores(i, s1);
+          }
+        }
+        tc_commit(&vempty[s]);
+        if (j + 1 < most) tc_commit(&kempty[(j + 1) % kPmStages]);
+      }
+      // Nothing issued here may outlive the CTA: its last commit has to arrive.
+      if (!ok) {
+        record_status(QTTS_ERR_TIMEOUT);
+        tc_commit(&odone[0]);
+        tc_commit(&odone[1]);
+        (void)mbar_wait_bounded(&odone[1], 0, wait_ns);
+      } else if (!mbar_wait_bounded(&vempty[(most - 1) % kPmStages], ((most - 1) / kPmStages) & 1, wait_ns)) {
+        record_status(QTTS_ERR_TIMEOUT);
+      }
+    }
+    __syncwarp();
+  } else {
+    // ---------------- softmax: one row a thread ----------------
+    const int i = warp >> 2;
+    const int r = r0 + i * kPmTile + (tid & 127);
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t ts = tmem + lanes + kColS + i * kPmTile;
+    const uint32_t to = tmem + lanes + kColO + i * D;
+    const int tok = r / share;
+    const int lim = r < rows ? (a.causal ? len - n + tok + 1 : len) : 0;
+    // Tokens that all rows of this tile see (they are in order).
+    const int first_lim = a.causal ? len - n + (r0 + i * kPmTile) / share + 1 : len;
+    const bool whole = r0 + i * kPmTile + kPmTile <= rows;
+    const float to_log2 = a.scale * 1.4426950408889634f;
+    float m = -INFINITY, l = 0.f;
+    bool ok = true;
+    auto step = [&](int j, auto masked) {
+      constexpr bool kMasked = decltype(masked)::value;
+      const int left = lim - j * kPmTile;  // columns that this row sees
+      float mx = -INFINITY;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        uint32_t s[32];
+        tmem_ld<32>(ts + 32 * c, s);
+        tc_wait_ld();
+#pragma unroll
+        for (int k = 0; k < 32; ++k) {
+          const float x = __uint_as_float(s[k]);
+          mx = fmaxf(mx, kMasked && 32 * c + k >= left ? -INFINITY : x);
+        }
+      }
+      mx *= to_log2;  // scale > 0
+      if (__any_sync(0xffffffffu, mx > m + 8.f)) {
+        const float up = fmaxf(m, mx);
+        const float f = up > m ? ex2f(m - up) : 1.f;
+        m = up;
+        l *= f;
+        if (j > 0) {  // O is idle: its last product came before S
+#pragma unroll
+          for (int c = 0; c < D / 32; ++c) {
+            uint32_t o[32];
+            tmem_ld<32>(to + 32 * c, o);
+            tc_wait_ld();
+#pragma unroll
+            for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+            tmem_st_x32(to + 32 * c, o);
+          }
+        }
+      }
+      const float off = m == -INFINITY ? 0.f : -m;
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        uint32_t s[32], p[16];
+        tmem_ld<32>(ts + 32 * c, s);
+        tc_wait_ld();
+#pragma unroll
+        for (int k = 0; k < 32; k += 2) {
+          float x = ex2f(fmaf(__uint_as_float(s[k]), to_log2, off));
+          float y = ex2f(fmaf(__uint_as_float(s[k + 1]), to_log2, off));
+          if constexpr (kMasked) {
+            if (32 * c + k >= left) x = 0.f;
+            if (32 * c + k + 1 >= left) y = 0.f;
+          }
+          sum[k / 2 % 4] += x;
+          sum[k / 2 % 4] += y;
+          p[k / 2] = pack_bf16x2(x, y);
+        }
+        tmem_st_x16(ts + 16 * c, p);
+      }
+      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      tc_wait_st();
+      tc_fence_before();
+      mbar_arrive(&pfull[i]);
+    };
+    for (int j = 0; ok && j < steps[i]; ++j) {
+      ok = __all_sync(0xffffffffu, mbar_wait_bounded(&sfull[i], j & 1, wait_ns));
+      if (!ok) break;
+      tc_fence_after();
+      if (whole && (j + 1) * kPmTile <= first_lim) {
+        step(j, std::false_type{});
+      } else {
+        step(j, std::true_type{});
+      }
+    }
+    if (ok && steps[i] > 0) {
+      ok = __all_sync(0xffffffffu, mbar_wait_bounded(&odone[i], 0, wait_ns));
+      tc_fence_after();
+    }
+    if (!ok && lane == 0) record_status(QTTS_ERR_TIMEOUT);
+    if (i < tiles_a_cta) {
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      T* dst = static_cast<T*>(a.out) + static_cast<int64_t>(start + tok) * a.out_token_stride +
+               static_cast<int64_t>(kvh * share + r % share) * D;
+      // Column 8 wi + 2 x + e of O is channel 32 (2 (wi % (NG/2)) + e) + 4 (wi / (NG/2)) + x: the
+      // columns of NG words together are eight channels of every group.
+#pragma unroll
+      for (int c = 0; c < D / (8 * NG); ++c) {
+        uint32_t o[8 * NG];
+        if (steps[i] > 0) {
+          if constexpr (NG == 4) {
+            tmem_ld<32>(to + 32 * c, o);
+          } else {
+            tmem_ld<16>(to + 16 * c, o);
+          }
+          tc_wait_ld();
+        } else {
+#pragma unroll
+          for (int k = 0; k < 8 * NG; ++k) o[k] = 0u;
+        }
+        if (r < rows) {
+#pragma unroll
+          for (int g = 0; g < NG; ++g) {
+            T v[8];
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+              const int wi = (q / 4) * (NG / 2) + g / 2;
+              v[q] = from_float<T>(__uint_as_float(o[8 * wi + 2 * (q % 4) + (g & 1)]) * inv);
+            }
+            *reinterpret_cast<uint4*>(dst + 32 * g + 8 * c) = *reinterpret_cast<uint4*>(v);
+          }
+        }
+      }
+    }
+    tc_fence_before();
+  }
+  __syncthreads();
+  tc_fence_after();
+  if (warp == kPmMmaWarp) tmem_dealloc(tmem, 512);
+}
+
+template <typename T, int D>
+int launch_pm(const Kv4AttnArgs& a, int tiles, bool pdl, cudaStream_t stream) {
+  constexpr int kSmem = PromptSmem<D>::kBytes;
+  if (cudaFuncSetAttribute(kv4_prompt_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) !=
+      cudaSuccess) {
+    (void)cudaGetLastError();
+    return QTTS_ERR_LAUNCH;
+  }
+  const int64_t rows = static_cast<int64_t>(a.max_q) * (a.q_heads / a.cache.kv_heads);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>((rows + tiles * kPmTile - 1) / (tiles * kPmTile)), a.cache.kv_heads, a.batch);
+  cfg.blockDim = dim3(kPmThreads);
+  cfg.dynamicSmemBytes = kSmem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  if (pdl) {
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+  }
+  return cudaLaunchKernelEx(&cfg, kv4_prompt_kernel<T, D>, a, tiles, current_wait_limit_ns()) == cudaSuccess
+             ? QTTS_OK
+             : QTTS_ERR_LAUNCH;
+}
+
+}  // namespace
+
+int launch_kv4_prompt(const Kv4AttnArgs& a, int dtype, int head_dim, bool pdl, cudaStream_t stream) {
+  const int64_t rows = static_cast<int64_t>(a.max_q) * (a.q_heads / a.cache.kv_heads);
+  // Two tiles a CTA share the operands and hide each other's softmax; one where two would leave
+  // SMs without a CTA.
+  const int64_t pairs = (rows + 2 * kPmTile - 1) / (2 * kPmTile) * a.cache.kv_heads * a.batch;
+  const int tiles = rows > kPmTile && pairs >= kNumSMs ? 2 : 1;
+  if (dtype == QTTS_BF16) {
+    return head_dim == 128 ? launch_pm<__nv_bfloat16, 128>(a, tiles, pdl, stream)
+                           : launch_pm<__nv_bfloat16, 64>(a, tiles, pdl, stream);
+  }
+  return head_dim == 128 ? launch_pm<__half, 128>(a, tiles, pdl, stream)
+                         : launch_pm<__half, 64>(a, tiles, pdl, stream);
+}
+
+}  // namespace qtts
