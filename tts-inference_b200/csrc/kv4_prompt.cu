@@ -271,57 +271,67 @@ __global__ void __launch_bounds__(kPmThreads, 1)
     if (!ok) record_status(QTTS_ERR_TIMEOUT);
   } else if (warp == kPmMmaWarp) {
     // ---------------- the products ----------------
-    if (lane == 0 && most > 0) {
+    // The whole warp runs along, so that operands and branches are uniform; one elected lane issues.
+    if (most > 0) {
       const uint32_t qa = smem_u32(smem + S::kQ), ka = smem_u32(smem + S::kK), va = smem_u32(smem + S::kV);
-      auto scores = [&](int i, int s) {
-#pragma unroll
-        for (int ks = 0; ks < D / 16; ++ks) {
-          const uint32_t o = (ks / 4) * (kPmTile * 128) + (ks % 4) * 32;
-          umma_f16_ss(tmem + kColS + i * kPmTile, smem_desc_k_sw128(qa + i * S::kTileBytes + o),
-                      smem_desc_k_sw128(ka + s * S::kTileBytes + o), kIdescS, ks != 0 ? 1u : 0u);
-        }
-        tc_commit(&sfull[i]);
+      const auto wait = [&](uint64_t* bar, int phase) {
+        const bool got = __all_sync(0xffffffffu, mbar_wait_bounded(bar, phase & 1, wait_ns));
+        tc_fence_after();
+        return got;
       };
-      bool ok = mbar_wait_bounded(&kfull[0], 0, wait_ns);
-      tc_fence_after();
+      const auto commit = [&](uint64_t* bar) {
+        if (elect_one()) tc_commit(bar);
+      };
+      const auto scores = [&](int i, int s) {
+        const uint64_t ad = smem_desc_k_sw128(qa + i * S::kTileBytes);
+        const uint64_t bd = smem_desc_k_sw128(ka + s * S::kTileBytes);
+        if (elect_one()) {
+#pragma unroll
+          for (int ks = 0; ks < D / 16; ++ks) {
+            const uint32_t o = ((ks / 4) * (kPmTile * 128) + (ks % 4) * 32) >> 4;
+            umma_f16_ss(tmem + kColS + i * kPmTile, ad + o, bd + o, kIdescS, ks != 0 ? 1u : 0u);
+          }
+          tc_commit(&sfull[i]);
+        }
+      };
+      bool ok = wait(&kfull[0], 0);
       for (int i = 0; ok && i < 2; ++i) {
         if (steps[i] > 0) scores(i, 0);
       }
-      tc_commit(&kempty[0]);
+      commit(&kempty[0]);
       for (int j = 0; ok && j < most; ++j) {
         const int s = j % kPmStages;
-        for (int i = 0; ok && i < 2; ++i) {
+        for (int i = 0; i < 2; ++i) {
           if (j >= steps[i]) continue;
-          ok = mbar_wait_bounded(&pfull[i], j & 1, wait_ns) &&
-               mbar_wait_bounded(&vfull[s], (j / kPmStages) & 1, wait_ns);
+          ok = wait(&pfull[i], j) && wait(&vfull[s], j / kPmStages);
           if (!ok) break;
-          tc_fence_after();
+          const uint64_t vd = smem_desc_mn_sw128(va + s * S::kTileBytes, kPmTile * 128, 1024);
+          if (elect_one()) {
 #pragma unroll
-          for (int ks = 0; ks < kPmTile / 16; ++ks) {
-            umma_f16_ts(tmem + kColO + i * D, tmem + kColS + i * kPmTile + 8 * ks,
-                        smem_desc_mn_sw128(va + s * S::kTileBytes + ks * 2048, kPmTile * 128, 1024), kIdescO,
-                        (j | ks) != 0 ? 1u : 0u);
+            for (int ks = 0; ks < kPmTile / 16; ++ks) {
+              umma_f16_ts(tmem + kColO + i * D, tmem + kColS + i * kPmTile + 8 * ks, vd + ks * (2048 >> 4), kIdescO,
+                          (j | ks) != 0 ? 1u : 0u);
+            }
+            if (j + 1 == steps[i]) tc_commit(&odone[i]);
           }
-          if (j + 1 == steps[i]) tc_commit(&odone[i]);
           if (j + 1 < steps[i]) {
             const int s1 = (j + 1) % kPmStages;
-            ok = mbar_wait_bounded(&kfull[s1], ((j + 1) / kPmStages) & 1, wait_ns);
+            ok = wait(&kfull[s1], (j + 1) / kPmStages);
             if (!ok) break;
-            tc_fence_after();
             scores(i, s1);
           }
         }
-        tc_commit(&vempty[s]);
-        if (j + 1 < most) tc_commit(&kempty[(j + 1) % kPmStages]);
+        commit(&vempty[s]);
+        if (j + 1 < most) commit(&kempty[(j + 1) % kPmStages]);
       }
       // Nothing issued here may outlive the CTA: its last commit has to arrive.
       if (!ok) {
-        record_status(QTTS_ERR_TIMEOUT);
-        tc_commit(&odone[0]);
-        tc_commit(&odone[1]);
-        (void)mbar_wait_bounded(&odone[1], 0, wait_ns);
-      } else if (!mbar_wait_bounded(&vempty[(most - 1) % kPmStages], ((most - 1) / kPmStages) & 1, wait_ns)) {
-        record_status(QTTS_ERR_TIMEOUT);
+        if (lane == 0) record_status(QTTS_ERR_TIMEOUT);
+        commit(&odone[0]);
+        commit(&odone[1]);
+        (void)wait(&odone[1], 0);
+      } else if (!wait(&vempty[(most - 1) % kPmStages], (most - 1) / kPmStages)) {
+        if (lane == 0) record_status(QTTS_ERR_TIMEOUT);
       }
     }
     __syncwarp();
