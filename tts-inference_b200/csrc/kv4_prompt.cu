@@ -12,14 +12,14 @@
 //     transposed (N-contiguous) B operand of O += P V. The order of channels
 //     within a row is the order in which masks give pairs; q is stored to match, and
 //     the outputs are put back in order at the end;
-//   * warp 12 issues the products: S of one tile while the other tile's
-//     probabilities are made, P from tensor memory, where it replaces S. The
-//     products of one tile run in the order issued, so S(j + 1) may overwrite P(j)
-//     and whoever has seen S(j) knows that O has taken P(j - 1);
+//   * warp 12 issues the products, 64 tokens of S at a time into one of two buffers
+//     a tile, so that S(u + 1) is made while the probabilities of S(u) are. P
+//     replaces S in tensor memory. The products of one tile run in the order
+//     issued, so S(u + 2) may overwrite P(u);
 //   * warps 0-3 and 4-7 (a thread a row, no exchange between threads) take the
 //     running maximum and sum in fp32 and write P as bf16. The reference maximum
 //     follows only when the maximum has grown by more than 2^8, so O is rescaled
-//     rarely; the row's sum divides at the end.
+//     rarely (and then waits for the product before); the row's sum divides at the end.
 // Bound by the two products (2 x 512 cycles a tile of 128 x 128 x 128) and, as
 // much, by 16384 exponentials a tile at 16 a cycle.
 #include <type_traits>
@@ -32,6 +32,7 @@ namespace qtts {
 namespace {
 
 constexpr int kPmTile = 128;  // rows of a tile, and tokens at a time
+constexpr int kPmSub = 64;     // tokens of S at a time
 constexpr int kPmStages = 2;
 constexpr int kPmDqWarp = 8;   // first of four warps that make the operands
 constexpr int kPmMmaWarp = 12;
@@ -78,7 +79,7 @@ __global__ void __launch_bounds__(kPmThreads, 1)
   using S = PromptSmem<D>;
   constexpr int NG = D / kKv4Group;
   constexpr int kWords = D / 8;  // 32-bit words of codes a row; chunks of eight channels
-  constexpr uint32_t kIdescS = umma_idesc(1u, 1u, kPmTile, kPmTile);
+  constexpr uint32_t kIdescS = umma_idesc(1u, 1u, kPmTile, kPmSub);
   constexpr uint32_t kIdescO = umma_idesc(1u, 1u, kPmTile, D) | kUmmaBTransposed;
   constexpr uint32_t kColS = 0, kColO = 2 * kPmTile;
   extern __shared__ uint8_t smem_raw[];
@@ -87,10 +88,11 @@ __global__ void __launch_bounds__(kPmThreads, 1)
   uint64_t* kempty = kfull + kPmStages;
   uint64_t* vfull = kempty + kPmStages;
   uint64_t* vempty = vfull + kPmStages;
-  uint64_t* sfull = vempty + kPmStages;  // [tile]: S is there (and O has taken the P before)
-  uint64_t* pfull = sfull + 2;           // [tile]: P is there
-  uint64_t* odone = pfull + 2;           // [tile]: all of O is there
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(odone + 2);
+  uint64_t* sfull = vempty + kPmStages;  // [tile][buffer]: S is there
+  uint64_t* pfull = sfull + 4;           // [tile][buffer]: P is there
+  uint64_t* odone = pfull + 4;           // [tile]: O has taken one more P
+  uint64_t* ofull = odone + 2;           // [tile]: all of O is there
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(ofull + 2);
 
   const int tid = threadIdx.x;
   const int warp = tid >> 5;
@@ -102,11 +104,11 @@ __global__ void __launch_bounds__(kPmThreads, 1)
       mbar_init(&vfull[s], kPmTile);
       mbar_init(&vempty[s], 1);
     }
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < 4; ++i) {
       mbar_init(&sfull[i], 1);
       mbar_init(&pfull[i], kPmTile);
-      mbar_init(&odone[i], 1);
     }
+    for (int i = 0; i < 4; ++i) mbar_init(&odone[i], 1);  // and ofull
     fence_mbarrier_init();
   }
   if (warp == kPmMmaWarp) {
@@ -190,33 +192,40 @@ __global__ void __launch_bounds__(kPmThreads, 1)
     const int first_lim = a.causal ? len - n + r0 / share + 1 : len;
     uint4 kc[NG], vc[NG];
     uint32_t kp[NG], vp[NG];
-    auto fetch = [&](int j) {  // codes and params of this thread's token of step j
-      const int tok = j * kPmTile + t;
-#pragma unroll
-      for (int i = 0; i < NG; ++i) kc[i] = vc[i] = make_uint4(0u, 0u, 0u, 0u), kp[i] = vp[i] = 0u;
-      if (tok < kmax) {
+    int64_t row = 0;  // of this thread's token of the step being fetched; -1 beyond the tokens
+    auto find = [&](int j) {
+      row = -1;
+      if (j * kPmTile + t < kmax) {
         int64_t page = table[col];
         if (page < 0 || page >= a.cache.pages) {
           record_status(QTTS_ERR_SHAPE);
           page = 0;
         }
-        const int64_t row = kv4_row(a.cache, page, kvh, 16 * off + (t & 15));
-        const uint4* k4 = reinterpret_cast<const uint4*>(a.cache.k_codes + row * (D / 2));
-        const uint4* v4 = reinterpret_cast<const uint4*>(a.cache.v_codes + row * (D / 2));
-#pragma unroll
-        for (int i = 0; i < NG; ++i) kc[i] = __ldg(k4 + i), vc[i] = __ldg(v4 + i);
-        const uint2* p2 = reinterpret_cast<const uint2*>(a.cache.k_params + row * NG);
-        const uint2* q2 = reinterpret_cast<const uint2*>(a.cache.v_params + row * NG);
-#pragma unroll
-        for (int i = 0; i < NG / 2; ++i) {
-          const uint2 x = __ldg(p2 + i), y = __ldg(q2 + i);
-          kp[2 * i] = x.x, kp[2 * i + 1] = x.y, vp[2 * i] = y.x, vp[2 * i + 1] = y.y;
-        }
+        row = kv4_row(a.cache, page, kvh, 16 * off + (t & 15));
       }
       col += dcol, off += doff;
       if (off >= per_page) off -= per_page, ++col;
     };
-    if (most > 0) fetch(0);
+    auto fetch = [&](const uint8_t* codes, const uint32_t* params, uint4(&c)[NG], uint32_t(&p)[NG]) {
+#pragma unroll
+      for (int i = 0; i < NG; ++i) c[i] = make_uint4(0u, 0u, 0u, 0u), p[i] = 0u;
+      if (row >= 0) {
+        const uint4* c4 = reinterpret_cast<const uint4*>(codes + row * (D / 2));
+        const uint2* p2 = reinterpret_cast<const uint2*>(params + row * NG);
+#pragma unroll
+        for (int i = 0; i < NG / 2; ++i) {
+          const uint2 x = __ldg(p2 + i);
+          p[2 * i] = x.x, p[2 * i + 1] = x.y;
+        }
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) c[i] = __ldg(c4 + i);
+      }
+    };
+    if (most > 0) {
+      find(0);
+      fetch(a.cache.v_codes, a.cache.v_params, vc, vp);
+      fetch(a.cache.k_codes, a.cache.k_params, kc, kp);
+    }
     bool ok = true;
     for (int j = 0; ok && j < most; ++j) {
       const int s = j % kPmStages;
@@ -250,6 +259,10 @@ __global__ void __launch_bounds__(kPmThreads, 1)
       }
       fence_proxy_async_smem();
       mbar_arrive(&kfull[s]);
+      if (j + 1 < most) {  // the next keys are on their way while the values are made
+        find(j + 1);
+        fetch(a.cache.k_codes, a.cache.k_params, kc, kp);
+      }
       if (ok && j >= kPmStages) ok = mbar_wait_bounded(&vempty[s], ((j / kPmStages) - 1) & 1, wait_ns);
       // Values: word wi holds four channels each of two neighbouring groups in its halves.
 #pragma unroll
@@ -266,7 +279,7 @@ __global__ void __launch_bounds__(kPmThreads, 1)
       }
       fence_proxy_async_smem();
       mbar_arrive(&vfull[s]);
-      if (j + 1 < most) fetch(j + 1);
+      if (j + 1 < most) fetch(a.cache.v_codes, a.cache.v_params, vc, vp);
     }
     if (!ok) record_status(QTTS_ERR_TIMEOUT);
   } else if (warp == kPmMmaWarp) {
@@ -282,54 +295,59 @@ __global__ void __launch_bounds__(kPmThreads, 1)
       const auto commit = [&](uint64_t* bar) {
         if (elect_one()) tc_commit(bar);
       };
-      const auto scores = [&](int i, int s) {
+      // Sub-step u of a tile: tokens 64 u .. + 63, half u % 2 of stage (u / 2) % kPmStages.
+      const auto scores = [&](int i, int u) {
         const uint64_t ad = smem_desc_k_sw128(qa + i * S::kTileBytes);
-        const uint64_t bd = smem_desc_k_sw128(ka + s * S::kTileBytes);
+        const uint64_t bd = smem_desc_k_sw128(ka + (u / 2 % kPmStages) * S::kTileBytes + (u & 1) * (kPmSub * 128));
         if (elect_one()) {
 #pragma unroll
           for (int ks = 0; ks < D / 16; ++ks) {
             const uint32_t o = ((ks / 4) * (kPmTile * 128) + (ks % 4) * 32) >> 4;
-            umma_f16_ss(tmem + kColS + i * kPmTile, ad + o, bd + o, kIdescS, ks != 0 ? 1u : 0u);
+            umma_f16_ss(tmem + kColS + i * kPmTile + (u & 1) * kPmSub, ad + o, bd + o, kIdescS, ks != 0 ? 1u : 0u);
           }
-          tc_commit(&sfull[i]);
+          tc_commit(&sfull[2 * i + (u & 1)]);
         }
       };
       bool ok = wait(&kfull[0], 0);
-      for (int i = 0; ok && i < 2; ++i) {
-        if (steps[i] > 0) scores(i, 0);
+      for (int u = 0; ok && u < 2; ++u) {
+        for (int i = 0; i < 2; ++i) {
+          if (steps[i] > 0) scores(i, u);
+        }
       }
       commit(&kempty[0]);
-      for (int j = 0; ok && j < most; ++j) {
-        const int s = j % kPmStages;
+      for (int u = 0; ok && u < 2 * most; ++u) {
+        const int j = u / 2, h = u & 1, s = j % kPmStages;
         for (int i = 0; i < 2; ++i) {
           if (j >= steps[i]) continue;
-          ok = wait(&pfull[i], j) && wait(&vfull[s], j / kPmStages);
+          ok = wait(&pfull[2 * i + h], j) && wait(&vfull[s], j / kPmStages);
           if (!ok) break;
-          const uint64_t vd = smem_desc_mn_sw128(va + s * S::kTileBytes, kPmTile * 128, 1024);
+          const uint64_t vd = smem_desc_mn_sw128(va + s * S::kTileBytes + h * (kPmSub * 128), kPmTile * 128, 1024);
           if (elect_one()) {
 #pragma unroll
-            for (int ks = 0; ks < kPmTile / 16; ++ks) {
-              umma_f16_ts(tmem + kColO + i * D, tmem + kColS + i * kPmTile + 8 * ks, vd + ks * (2048 >> 4), kIdescO,
-                          (j | ks) != 0 ? 1u : 0u);
+            for (int ks = 0; ks < kPmSub / 16; ++ks) {
+              umma_f16_ts(tmem + kColO + i * D, tmem + kColS + i * kPmTile + h * kPmSub + 8 * ks,
+                          vd + ks * (2048 >> 4), kIdescO, (u | ks) != 0 ? 1u : 0u);
             }
-            if (j + 1 == steps[i]) tc_commit(&odone[i]);
+            tc_commit(&odone[i]);
+            if (u + 1 == 2 * steps[i]) tc_commit(&ofull[i]);
           }
           if (j + 1 < steps[i]) {
-            const int s1 = (j + 1) % kPmStages;
-            ok = wait(&kfull[s1], (j + 1) / kPmStages);
+            ok = wait(&kfull[(j + 1) % kPmStages], (j + 1) / kPmStages);
             if (!ok) break;
-            scores(i, s1);
+            scores(i, u + 2);
           }
         }
-        commit(&vempty[s]);
-        if (j + 1 < most) commit(&kempty[(j + 1) % kPmStages]);
+        if (h == 1) {
+          commit(&vempty[s]);
+          if (j + 1 < most) commit(&kempty[(j + 1) % kPmStages]);
+        }
       }
       // Nothing issued here may outlive the CTA: its last commit has to arrive.
       if (!ok) {
         if (lane == 0) record_status(QTTS_ERR_TIMEOUT);
-        commit(&odone[0]);
-        commit(&odone[1]);
-        (void)wait(&odone[1], 0);
+        commit(&vempty[0]);  // whichever phase this completes, all products came before
+        (void)wait(&vempty[0], 0);
+        (void)wait(&vempty[0], 1);
       } else if (!wait(&vempty[(most - 1) % kPmStages], (most - 1) / kPmStages)) {
         if (lane == 0) record_status(QTTS_ERR_TIMEOUT);
       }
@@ -350,20 +368,19 @@ __global__ void __launch_bounds__(kPmThreads, 1)
     const float to_log2 = a.scale * 1.4426950408889634f;
     float m = -INFINITY, l = 0.f;
     bool ok = true;
-    auto step = [&](int j, auto masked) {
+    auto step = [&](int u, auto masked) {
       constexpr bool kMasked = decltype(masked)::value;
-      const int left = lim - j * kPmTile;  // columns that this row sees
+      const int left = lim - u * kPmSub;  // columns that this row sees
+      const uint32_t tb = ts + (u & 1) * kPmSub;
+      uint32_t s[2][32];
+      tmem_ld<32>(tb, s[0]);
+      tmem_ld<32>(tb + 32, s[1]);
+      tc_wait_ld();
       float mx = -INFINITY;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint32_t s[32];
-        tmem_ld<32>(ts + 32 * c, s);
-        tc_wait_ld();
-#pragma unroll
-        for (int k = 0; k < 32; ++k) {
-          const float x = __uint_as_float(s[k]);
-          mx = fmaxf(mx, kMasked && 32 * c + k >= left ? -INFINITY : x);
-        }
+      for (int k = 0; k < kPmSub; ++k) {
+        if (kMasked && k >= left) s[k / 32][k % 32] = 0xFF800000u;  // -inf
+        mx = fmaxf(mx, __uint_as_float(s[k / 32][k % 32]));
       }
       mx *= to_log2;  // scale > 0
       if (__any_sync(0xffffffffu, mx > m + 8.f)) {
@@ -371,56 +388,53 @@ __global__ void __launch_bounds__(kPmThreads, 1)
         const float f = up > m ? ex2f(m - up) : 1.f;
         m = up;
         l *= f;
-        if (j > 0) {  // O is idle: its last product came before S
+        if (u > 0) {
+          // S(u) came after O took P(u - 2); it may be taking P(u - 1).
+          ok = ok && __all_sync(0xffffffffu, mbar_wait_bounded(&odone[i], (u - 1) & 1, wait_ns));
+          tc_fence_after();
 #pragma unroll
-          for (int c = 0; c < D / 32; ++c) {
-            uint32_t o[32];
-            tmem_ld<32>(to + 32 * c, o);
+          for (int c = 0; c < D / 16; ++c) {
+            uint32_t o[16];
+            tmem_ld<16>(to + 16 * c, o);
             tc_wait_ld();
 #pragma unroll
-            for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
-            tmem_st_x32(to + 32 * c, o);
+            for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+            tmem_st_x16(to + 16 * c, o);
           }
         }
       }
       const float off = m == -INFINITY ? 0.f : -m;
       float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint32_t s[32], p[16];
-        tmem_ld<32>(ts + 32 * c, s);
-        tc_wait_ld();
+      for (int c = 0; c < 2; ++c) {
+        uint32_t p[16];
 #pragma unroll
         for (int k = 0; k < 32; k += 2) {
-          float x = ex2f(fmaf(__uint_as_float(s[k]), to_log2, off));
-          float y = ex2f(fmaf(__uint_as_float(s[k + 1]), to_log2, off));
-          if constexpr (kMasked) {
-            if (32 * c + k >= left) x = 0.f;
-            if (32 * c + k + 1 >= left) y = 0.f;
-          }
-          sum[k / 2 % 4] += x;
-          sum[k / 2 % 4] += y;
+          const float x = ex2f(fmaf(__uint_as_float(s[c][k]), to_log2, off));
+          const float y = ex2f(fmaf(__uint_as_float(s[c][k + 1]), to_log2, off));
+          sum[k / 2 % 2] += x;
+          sum[2 + k / 2 % 2] += y;
           p[k / 2] = pack_bf16x2(x, y);
         }
-        tmem_st_x16(ts + 16 * c, p);
+        tmem_st_x16(tb + 16 * c, p);
       }
       l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
       tc_wait_st();
       tc_fence_before();
-      mbar_arrive(&pfull[i]);
+      mbar_arrive(&pfull[2 * i + (u & 1)]);
     };
-    for (int j = 0; ok && j < steps[i]; ++j) {
-      ok = __all_sync(0xffffffffu, mbar_wait_bounded(&sfull[i], j & 1, wait_ns));
+    for (int u = 0; ok && u < 2 * steps[i]; ++u) {
+      ok = __all_sync(0xffffffffu, mbar_wait_bounded(&sfull[2 * i + (u & 1)], (u / 2) & 1, wait_ns));
       if (!ok) break;
       tc_fence_after();
-      if (whole && (j + 1) * kPmTile <= first_lim) {
-        step(j, std::false_type{});
+      if (whole && (u + 1) * kPmSub <= first_lim) {
+        step(u, std::false_type{});
       } else {
-        step(j, std::true_type{});
+        step(u, std::true_type{});
       }
     }
     if (ok && steps[i] > 0) {
-      ok = __all_sync(0xffffffffu, mbar_wait_bounded(&odone[i], 0, wait_ns));
+      ok = __all_sync(0xffffffffu, mbar_wait_bounded(&ofull[i], 0, wait_ns));
       tc_fence_after();
     }
     if (!ok && lane == 0) record_status(QTTS_ERR_TIMEOUT);
