@@ -122,10 +122,10 @@ __global__ void __launch_bounds__(kPmThreads, 1)
   pdl_launch_dependents();
   pdl_wait();
 
-  // The longest blocks first: with `causal` the last rows see most.
-  const int rb = static_cast<int>(gridDim.x - 1 - blockIdx.x);
-  const int kvh = blockIdx.y;
-  const int b = blockIdx.z;
+  // The longest blocks first, of all requests and heads: with `causal` the last rows see most.
+  const int rb = static_cast<int>(gridDim.z - 1 - blockIdx.z);
+  const int kvh = blockIdx.x;
+  const int b = blockIdx.y;
   int start = 0, n = 0;
   bool fine = request_rows(a, b, start, n);
   int len = a.lengths[b];
@@ -317,9 +317,13 @@ __global__ void __launch_bounds__(kPmThreads, 1)
       commit(&kempty[0]);
       for (int u = 0; ok && u < 2 * most; ++u) {
         const int j = u / 2, h = u & 1, s = j % kPmStages;
-        for (int i = 0; i < 2; ++i) {
+        if (h == 0) {
+          ok = wait(&vfull[s], j / kPmStages) &&
+               (j + 1 >= most || wait(&kfull[(j + 1) % kPmStages], (j + 1) / kPmStages));
+        }
+        for (int i = 0; ok && i < 2; ++i) {
           if (j >= steps[i]) continue;
-          ok = wait(&pfull[2 * i + h], j) && wait(&vfull[s], j / kPmStages);
+          ok = wait(&pfull[2 * i + h], j);
           if (!ok) break;
           const uint64_t vd = smem_desc_mn_sw128(va + s * S::kTileBytes + h * (kPmSub * 128), kPmTile * 128, 1024);
           if (elect_one()) {
@@ -331,11 +335,7 @@ __global__ void __launch_bounds__(kPmThreads, 1)
             tc_commit(&odone[i]);
             if (u + 1 == 2 * steps[i]) tc_commit(&ofull[i]);
           }
-          if (j + 1 < steps[i]) {
-            ok = wait(&kfull[(j + 1) % kPmStages], (j + 1) / kPmStages);
-            if (!ok) break;
-            scores(i, u + 2);
-          }
+          if (j + 1 < steps[i]) scores(i, u + 2);
         }
         if (h == 1) {
           commit(&vempty[s]);
@@ -489,7 +489,9 @@ int launch_pm(const Kv4AttnArgs& a, int tiles, bool pdl, cudaStream_t stream) {
   }
   const int64_t rows = static_cast<int64_t>(a.max_q) * (a.q_heads / a.cache.kv_heads);
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>((rows + tiles * kPmTile - 1) / (tiles * kPmTile)), a.cache.kv_heads, a.batch);
+  const int64_t blocks = (rows + tiles * kPmTile - 1) / (tiles * kPmTile);
+  if (blocks > 65535) return QTTS_ERR_SHAPE;
+  cfg.gridDim = dim3(a.cache.kv_heads, a.batch, static_cast<unsigned>(blocks));
   cfg.blockDim = dim3(kPmThreads);
   cfg.dynamicSmemBytes = kSmem;
   cfg.stream = stream;
