@@ -92,7 +92,8 @@ __global__ void __launch_bounds__(kPmThreads, 1)
   uint64_t* pfull = sfull + 4;           // [tile][buffer]: P is there
   uint64_t* odone = pfull + 4;           // [tile]: O has taken one more P
   uint64_t* ofull = odone + 2;           // [tile]: all of O is there
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(ofull + 2);
+  uint64_t* qfull = ofull + 2;           // q is there
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(qfull + 1);
 
   const int tid = threadIdx.x;
   const int warp = tid >> 5;
@@ -109,6 +110,7 @@ __global__ void __launch_bounds__(kPmThreads, 1)
       mbar_init(&pfull[i], kPmTile);
     }
     for (int i = 0; i < 4; ++i) mbar_init(&odone[i], 1);  // and ofull
+    mbar_init(qfull, 2 * kPmTile);
     fence_mbarrier_init();
   }
   if (warp == kPmMmaWarp) {
@@ -154,32 +156,6 @@ __global__ void __launch_bounds__(kPmThreads, 1)
     }
   }
   const int most = max(steps[0], steps[1]);
-
-  // q in bf16, channels of a chunk in the order 0 4 1 5 2 6 3 7.
-  if (most > 0) {
-    for (int i = tid; i < tiles_a_cta * kPmTile * kWords; i += kPmThreads) {
-      const int r = i / kWords, ch = i % kWords;
-      uint4 u = make_uint4(0u, 0u, 0u, 0u);
-      if (r0 + r < rows) {
-        const int rr = r0 + r;
-        u = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) +
-                                            static_cast<int64_t>(start + rr / share) * a.q_token_stride +
-                                            (kvh * share + rr % share) * a.q_head_stride + 8 * ch);
-      }
-      if constexpr (!std::is_same<T, __nv_bfloat16>::value) {
-        const __half* e = reinterpret_cast<const __half*>(&u);
-        u = make_uint4(pack_bf16x2(__half2float(e[0]), __half2float(e[1])),
-                       pack_bf16x2(__half2float(e[2]), __half2float(e[3])),
-                       pack_bf16x2(__half2float(e[4]), __half2float(e[5])),
-                       pack_bf16x2(__half2float(e[6]), __half2float(e[7])));
-      }
-      sts128(smem_u32(smem + S::kQ) + (r >> 7) * S::kTileBytes + tile_offset(r & 127, ch),
-             __byte_perm(u.x, u.z, 0x5410), __byte_perm(u.x, u.z, 0x7632), __byte_perm(u.y, u.w, 0x5410),
-             __byte_perm(u.y, u.w, 0x7632));
-    }
-    fence_proxy_async_smem();
-  }
-  __syncthreads();
 
   if (warp >= kPmDqWarp && warp < kPmMmaWarp) {
     // ---------------- operands: one token a thread ----------------
@@ -308,7 +284,7 @@ __global__ void __launch_bounds__(kPmThreads, 1)
           tc_commit(&sfull[2 * i + (u & 1)]);
         }
       };
-      bool ok = wait(&kfull[0], 0);
+      bool ok = wait(qfull, 0) && wait(&kfull[0], 0);
       for (int u = 0; ok && u < 2; ++u) {
         for (int i = 0; i < 2; ++i) {
           if (steps[i] > 0) scores(i, u);
@@ -360,14 +336,51 @@ __global__ void __launch_bounds__(kPmThreads, 1)
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t ts = tmem + lanes + kColS + i * kPmTile;
     const uint32_t to = tmem + lanes + kColO + i * D;
-    const int tok = r / share;
-    const int lim = r < rows ? (a.causal ? len - n + tok + 1 : len) : 0;
+    const int lim = r < rows ? (a.causal ? len - n + r / share + 1 : len) : 0;
     // Tokens that all rows of this tile see (they are in order).
     const int first_lim = a.causal ? len - n + (r0 + i * kPmTile) / share + 1 : len;
     const bool whole = r0 + i * kPmTile + kPmTile <= rows;
     const float to_log2 = a.scale * 1.4426950408889634f;
     float m = -INFINITY, l = 0.f;
     bool ok = true;
+
+    // q in bf16, channels of a chunk in the order 0 4 1 5 2 6 3 7: kWords lanes a row, eight rows
+    // of loads at a time.
+    if (most > 0) {
+      constexpr int kRowsAPass = 2 * kPmTile / kWords;
+      const int ch = tid % kWords;
+      for (int q0 = tid / kWords; q0 < tiles_a_cta * kPmTile; q0 += 8 * kRowsAPass) {
+        uint4 u[8];
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+          const int rr = r0 + q0 + x * kRowsAPass;
+          u[x] = make_uint4(0u, 0u, 0u, 0u);
+          if (q0 + x * kRowsAPass < tiles_a_cta * kPmTile && rr < rows) {
+            u[x] = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) +
+                                                   static_cast<int64_t>(start + rr / share) * a.q_token_stride +
+                                                   (kvh * share + rr % share) * a.q_head_stride + 8 * ch);
+          }
+        }
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+          const int row = q0 + x * kRowsAPass;
+          if (row >= tiles_a_cta * kPmTile) break;
+          uint4 v = u[x];
+          if constexpr (!std::is_same<T, __nv_bfloat16>::value) {
+            const __half* e = reinterpret_cast<const __half*>(&v);
+            v = make_uint4(pack_bf16x2(__half2float(e[0]), __half2float(e[1])),
+                           pack_bf16x2(__half2float(e[2]), __half2float(e[3])),
+                           pack_bf16x2(__half2float(e[4]), __half2float(e[5])),
+                           pack_bf16x2(__half2float(e[6]), __half2float(e[7])));
+          }
+          sts128(smem_u32(smem + S::kQ) + (row >> 7) * S::kTileBytes + tile_offset(row & 127, ch),
+                 __byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632), __byte_perm(v.y, v.w, 0x5410),
+                 __byte_perm(v.y, v.w, 0x7632));
+        }
+      }
+      fence_proxy_async_smem();
+      mbar_arrive(qfull);
+    }
     auto step = [&](int u, auto masked) {
       constexpr bool kMasked = decltype(masked)::value;
       const int left = lim - u * kPmSub;  // columns that this row sees
@@ -438,12 +451,14 @@ __global__ void __launch_bounds__(kPmThreads, 1)
       tc_fence_after();
     }
     if (!ok && lane == 0) record_status(QTTS_ERR_TIMEOUT);
-    if (i < tiles_a_cta) {
+    if (i < tiles_a_cta && r0 + i * kPmTile < rows) {
       const float inv = l == 0.f ? 0.f : 1.f / l;
-      T* dst = static_cast<T*>(a.out) + static_cast<int64_t>(start + tok) * a.out_token_stride +
-               static_cast<int64_t>(kvh * share + r % share) * D;
       // Column 8 wi + 2 x + e of O is channel 32 (2 (wi % (NG/2)) + e) + 4 (wi / (NG/2)) + x: the
-      // columns of NG words together are eight channels of every group.
+      // columns of NG words together are eight channels of every group. A warp's 32 rows go through
+      // shared memory (its part of q's tile, which no product reads any more), so that whole
+      // rows are stored; lane and chunk are swizzled as in the operand tiles.
+      const uint32_t qt = smem_u32(smem + S::kQ) + i * S::kTileBytes;
+      const int row = tid & 127;
 #pragma unroll
       for (int c = 0; c < D / (8 * NG); ++c) {
         uint32_t o[8 * NG];
@@ -458,17 +473,29 @@ __global__ void __launch_bounds__(kPmThreads, 1)
 #pragma unroll
           for (int k = 0; k < 8 * NG; ++k) o[k] = 0u;
         }
-        if (r < rows) {
 #pragma unroll
-          for (int g = 0; g < NG; ++g) {
-            T v[8];
+        for (int g = 0; g < NG; ++g) {
+          T v[8];
 #pragma unroll
-            for (int q = 0; q < 8; ++q) {
-              const int wi = (q / 4) * (NG / 2) + g / 2;
-              v[q] = from_float<T>(__uint_as_float(o[8 * wi + 2 * (q % 4) + (g & 1)]) * inv);
-            }
-            *reinterpret_cast<uint4*>(dst + 32 * g + 8 * c) = *reinterpret_cast<uint4*>(v);
+          for (int q = 0; q < 8; ++q) {
+            const int wi = (q / 4) * (NG / 2) + g / 2;
+            v[q] = from_float<T>(__uint_as_float(o[8 * wi + 2 * (q % 4) + (g & 1)]) * inv);
           }
+          const uint4 u = *reinterpret_cast<uint4*>(v);
+          sts128(qt + tile_offset(row, 4 * g + c), u.x, u.y, u.z, u.w);
+        }
+      }
+      __syncwarp();
+      constexpr int kRowsAStore = 32 / kWords;
+#pragma unroll 4
+      for (int x = 0; x < 32; x += kRowsAStore) {
+        const int wrow = (warp & 3) * 32 + x + lane / kWords;
+        const int rr = r0 + i * kPmTile + wrow;
+        if (rr < rows) {
+          *reinterpret_cast<uint4*>(static_cast<T*>(a.out) +
+                                    static_cast<int64_t>(start + rr / share) * a.out_token_stride +
+                                    static_cast<int64_t>(kvh * share + rr % share) * D + 8 * (lane % kWords)) =
+              lds128(qt + tile_offset(wrow, lane % kWords));
         }
       }
     }
