@@ -12,7 +12,7 @@
 //     transposed (N-contiguous) B operand of O += P V. The order of channels
 //     within a row is the order in which masks give pairs; q is stored to match, and
 //     the outputs are put back in order at the end;
-//   * warp 12 issues the products, 64 tokens of S at a time into one of two buffers
+//   * warps 12 and 13 issue the products of a tile each, 64 tokens of S at a time into one of two buffers
 //     a tile, so that S(u + 1) is made while the probabilities of S(u) are. P
 //     replaces S in tensor memory. The products of one tile run in the order
 //     issued, so S(u + 2) may overwrite P(u);
@@ -35,8 +35,8 @@ constexpr int kPmTile = 128;  // rows of a tile, and tokens at a time
 constexpr int kPmSub = 64;     // tokens of S at a time
 constexpr int kPmStages = 2;
 constexpr int kPmDqWarp = 8;   // first of four warps that make the operands
-constexpr int kPmMmaWarp = 12;
-constexpr int kPmThreads = 13 * 32;
+constexpr int kPmMmaWarp = 12;  // one issuing warp a tile
+constexpr int kPmThreads = 14 * 32;
 
 template <int D>
 struct PromptSmem {
@@ -92,7 +92,8 @@ __global__ void __launch_bounds__(kPmThreads, 1)
   uint64_t* pfull = sfull + 4;           // [tile][buffer]: P is there
   uint64_t* odone = pfull + 4;           // [tile]: O has taken one more P
   uint64_t* ofull = odone + 2;           // [tile]: all of O is there
-  uint64_t* qfull = ofull + 2;           // q is there
+  uint64_t* mdone = ofull + 2;           // [tile]: everything issued is done
+  uint64_t* qfull = mdone + 2;           // q is there
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(qfull + 1);
 
   const int tid = threadIdx.x;
@@ -101,15 +102,15 @@ __global__ void __launch_bounds__(kPmThreads, 1)
   if (tid == 0) {
     for (int s = 0; s < kPmStages; ++s) {
       mbar_init(&kfull[s], kPmTile);
-      mbar_init(&kempty[s], 1);
+      mbar_init(&kempty[s], tiles_a_cta);
       mbar_init(&vfull[s], kPmTile);
-      mbar_init(&vempty[s], 1);
+      mbar_init(&vempty[s], tiles_a_cta);
     }
     for (int i = 0; i < 4; ++i) {
       mbar_init(&sfull[i], 1);
       mbar_init(&pfull[i], kPmTile);
     }
-    for (int i = 0; i < 4; ++i) mbar_init(&odone[i], 1);  // and ofull
+    for (int i = 0; i < 6; ++i) mbar_init(&odone[i], 1);  // and ofull, mdone
     mbar_init(qfull, 2 * kPmTile);
     fence_mbarrier_init();
   }
@@ -258,77 +259,70 @@ __global__ void __launch_bounds__(kPmThreads, 1)
       if (j + 1 < most) fetch(a.cache.v_codes, a.cache.v_params, vc, vp);
     }
     if (!ok) record_status(QTTS_ERR_TIMEOUT);
-  } else if (warp == kPmMmaWarp) {
-    // ---------------- the products ----------------
+  } else if (warp >= kPmMmaWarp) {
+    // ---------------- the products of tile i ----------------
     // The whole warp runs along, so that operands and branches are uniform; one elected lane issues.
-    if (most > 0) {
-      const uint32_t qa = smem_u32(smem + S::kQ), ka = smem_u32(smem + S::kK), va = smem_u32(smem + S::kV);
+    const int i = warp - kPmMmaWarp;
+    if (most > 0 && i < tiles_a_cta) {
+      const uint32_t qa = smem_u32(smem + S::kQ) + i * S::kTileBytes;
+      const uint32_t ka = smem_u32(smem + S::kK), va = smem_u32(smem + S::kV);
+      const uint32_t ts = tmem + kColS + i * kPmTile, to = tmem + kColO + i * D;
       const auto wait = [&](uint64_t* bar, int phase) {
         const bool got = __all_sync(0xffffffffu, mbar_wait_bounded(bar, phase & 1, wait_ns));
         tc_fence_after();
         return got;
       };
-      const auto commit = [&](uint64_t* bar) {
-        if (elect_one()) tc_commit(bar);
-      };
-      // Sub-step u of a tile: tokens 64 u .. + 63, half u % 2 of stage (u / 2) % kPmStages.
-      const auto scores = [&](int i, int u) {
-        const uint64_t ad = smem_desc_k_sw128(qa + i * S::kTileBytes);
+      // Sub-step u: tokens 64 u .. + 63, half u % 2 of stage (u / 2) % kPmStages. By the elected lane.
+      const auto scores = [&](int u) {
+        const uint64_t ad = smem_desc_k_sw128(qa);
         const uint64_t bd = smem_desc_k_sw128(ka + (u / 2 % kPmStages) * S::kTileBytes + (u & 1) * (kPmSub * 128));
-        if (elect_one()) {
 #pragma unroll
-          for (int ks = 0; ks < D / 16; ++ks) {
-            const uint32_t o = ((ks / 4) * (kPmTile * 128) + (ks % 4) * 32) >> 4;
-            umma_f16_ss(tmem + kColS + i * kPmTile + (u & 1) * kPmSub, ad + o, bd + o, kIdescS, ks != 0 ? 1u : 0u);
-          }
-          tc_commit(&sfull[2 * i + (u & 1)]);
+        for (int ks = 0; ks < D / 16; ++ks) {
+          const uint32_t o = ((ks / 4) * (kPmTile * 128) + (ks % 4) * 32) >> 4;
+          umma_f16_ss(ts + (u & 1) * kPmSub, ad + o, bd + o, kIdescS, ks != 0 ? 1u : 0u);
         }
+        tc_commit(&sfull[2 * i + (u & 1)]);
       };
+      const int mine = steps[i];
       bool ok = wait(qfull, 0) && wait(&kfull[0], 0);
-      for (int u = 0; ok && u < 2; ++u) {
-        for (int i = 0; i < 2; ++i) {
-          if (steps[i] > 0) scores(i, u);
+      if (ok && elect_one()) {
+        if (mine > 0) {
+          scores(0);
+          scores(1);
         }
+        tc_commit(&kempty[0]);
       }
-      commit(&kempty[0]);
-      for (int u = 0; ok && u < 2 * most; ++u) {
-        const int j = u / 2, h = u & 1, s = j % kPmStages;
-        if (h == 0) {
-          ok = wait(&vfull[s], j / kPmStages) &&
-               (j + 1 >= most || wait(&kfull[(j + 1) % kPmStages], (j + 1) / kPmStages));
-        }
-        for (int i = 0; ok && i < 2; ++i) {
-          if (j >= steps[i]) continue;
+      // A tile that needs fewer steps than the other goes on handing the stages back, each only
+      // once it has seen it filled.
+      for (int j = 0; ok && j < most; ++j) {
+        const int s = j % kPmStages, s1 = (j + 1) % kPmStages;
+        ok = wait(&vfull[s], j / kPmStages) && (j + 1 >= most || wait(&kfull[s1], (j + 1) / kPmStages));
+        for (int h = 0; ok && h < 2 && j < mine; ++h) {
+          const int u = 2 * j + h;
           ok = wait(&pfull[2 * i + h], j);
-          if (!ok) break;
-          const uint64_t vd = smem_desc_mn_sw128(va + s * S::kTileBytes + h * (kPmSub * 128), kPmTile * 128, 1024);
-          if (elect_one()) {
+          if (ok && elect_one()) {
+            const uint64_t vd = smem_desc_mn_sw128(va + s * S::kTileBytes + h * (kPmSub * 128), kPmTile * 128, 1024);
 #pragma unroll
             for (int ks = 0; ks < kPmSub / 16; ++ks) {
-              umma_f16_ts(tmem + kColO + i * D, tmem + kColS + i * kPmTile + h * kPmSub + 8 * ks,
-                          vd + ks * (2048 >> 4), kIdescO, (u | ks) != 0 ? 1u : 0u);
+              umma_f16_ts(to, ts + h * kPmSub + 8 * ks, vd + ks * (2048 >> 4), kIdescO, (u | ks) != 0 ? 1u : 0u);
             }
             tc_commit(&odone[i]);
-            if (u + 1 == 2 * steps[i]) tc_commit(&ofull[i]);
+            if (u + 1 == 2 * mine) tc_commit(&ofull[i]);
+            if (j + 1 < mine) scores(u + 2);
           }
-          if (j + 1 < steps[i]) scores(i, u + 2);
+          __syncwarp();
         }
-        if (h == 1) {
-          commit(&vempty[s]);
-          if (j + 1 < most) commit(&kempty[(j + 1) % kPmStages]);
+        if (ok && elect_one()) {
+          tc_commit(&vempty[s]);
+          if (j + 1 < most) tc_commit(&kempty[s1]);
         }
+        __syncwarp();
       }
       // Nothing issued here may outlive the CTA: its last commit has to arrive.
-      if (!ok) {
-        if (lane == 0) record_status(QTTS_ERR_TIMEOUT);
-        commit(&vempty[0]);  // whichever phase this completes, all products came before
-        (void)wait(&vempty[0], 0);
-        (void)wait(&vempty[0], 1);
-      } else if (!wait(&vempty[(most - 1) % kPmStages], (most - 1) / kPmStages)) {
-        if (lane == 0) record_status(QTTS_ERR_TIMEOUT);
-      }
+      if (elect_one()) tc_commit(&mdone[i]);
+      if (!wait(&mdone[i], 0)) ok = false;
+      if (!ok && lane == 0) record_status(QTTS_ERR_TIMEOUT);
     }
-    __syncwarp();
   } else {
     // ---------------- softmax: one row a thread ----------------
     const int i = warp >> 2;
