@@ -238,8 +238,16 @@ struct Kv4AttnArgs {
   float* parts;   // workspace [total_q, q_heads, splits, head_dim] and its statistics
   float2* stats;  // [total_q, q_heads, splits]: running maximum (log2) and sum
 };
-// Many rows a request (csrc/kv4_prompt.cu).
-int launch_kv4_prompt(const Kv4AttnArgs& a, int dtype, int head_dim, bool pdl, cudaStream_t stream);
+// Many rows a request (csrc/kv4_prompt.cu): tiles of 128 rows a CTA, CTAs a (request, key head)
+// and CTAs that share the tokens of one of them (their parts meet in the workspace).
+struct PromptPlan {
+  int tiles;
+  int64_t blocks;
+  int splits;
+};
+PromptPlan plan_prompt(int64_t max_q, int share, int kv_heads, int batch, int64_t most_tokens);
+int launch_kv4_prompt(const Kv4AttnArgs& a, const PromptPlan& p, int dtype, int head_dim, bool pdl,
+                      cudaStream_t stream);
 int launch_kv4_attention(const Kv4AttnArgs& a, int dtype, int head_dim, bool pdl, cudaStream_t stream);
 
 #ifdef QTTS_TRACE

@@ -760,34 +760,49 @@ int launch_rows(Kv4AttnArgs a, const RowsPlan& p, bool pdl, cudaStream_t stream)
   }
   const bool workspace = p.splits > kMaxCluster;
   if (!workspace) a.parts = nullptr, a.stats = nullptr;
-  const int r = launch(kv4_rows_kernel<T, D, NT>,
-                       dim3(p.splits, static_cast<unsigned>(p.row_blocks * a.cache.kv_heads), a.batch), 32 * kWarps,
-                       kSmem, workspace ? 1 : p.splits, pdl, stream, a, static_cast<int>(p.row_blocks));
-  if (r != QTTS_OK || !workspace) return r;
-  const int64_t rows = static_cast<int64_t>(a.total_q) * a.q_heads;
-  return launch(kv4_join_kernel<T, D>, dim3(static_cast<unsigned>((rows + 3) / 4)), 128, 0, 1, true, stream, a,
-                p.splits);
+  return launch(kv4_rows_kernel<T, D, NT>,
+                dim3(p.splits, static_cast<unsigned>(p.row_blocks * a.cache.kv_heads), a.batch), 32 * kWarps, kSmem,
+                workspace ? 1 : p.splits, pdl, stream, a, static_cast<int>(p.row_blocks));
 }
 
 template <typename T, int D>
-int launch_ka(const Kv4AttnArgs& a, bool pdl, cudaStream_t stream) {
-  const RowsPlan p = plan_rows(a.max_q, a.q_heads / a.cache.kv_heads, a.cache.kv_heads, a.batch,
-                               static_cast<int64_t>(a.table_cols) * a.cache.page_size);
+int launch_join(const Kv4AttnArgs& a, int splits, cudaStream_t stream) {
+  const int64_t rows = static_cast<int64_t>(a.total_q) * a.q_heads;
+  return launch(kv4_join_kernel<T, D>, dim3(static_cast<unsigned>((rows + 3) / 4)), 128, 0, 1, true, stream, a,
+                splits);
+}
+
+template <typename T, int D>
+int launch_ka(const Kv4AttnArgs& a, int dtype, bool pdl, cudaStream_t stream) {
+  const int share = a.q_heads / a.cache.kv_heads;
+  const int64_t tokens = static_cast<int64_t>(a.table_cols) * a.cache.page_size;
+  if (kv4_takes_prompt(a.max_q, share)) {
+    const PromptPlan p = plan_prompt(a.max_q, share, a.cache.kv_heads, a.batch, tokens);
+    const int r = launch_kv4_prompt(a, p, dtype, D, pdl, stream);
+    return r != QTTS_OK || p.splits == 1 ? r : launch_join<T, D>(a, p.splits, stream);
+  }
+  const RowsPlan p = plan_rows(a.max_q, share, a.cache.kv_heads, a.batch, tokens);
   if (p.row_blocks * a.cache.kv_heads > 65535) return QTTS_ERR_SHAPE;
-  return p.nt == 1 ? launch_rows<T, D, 1>(a, p, pdl, stream) : launch_rows<T, D, 2>(a, p, pdl, stream);
+  const int r = p.nt == 1 ? launch_rows<T, D, 1>(a, p, pdl, stream) : launch_rows<T, D, 2>(a, p, pdl, stream);
+  return r != QTTS_OK || p.splits <= kMaxCluster ? r : launch_join<T, D>(a, p.splits, stream);
+}
+
+// CTAs whose parts meet in the workspace; 1 where none do.
+int workspace_splits(int64_t max_q, int share, int kv_heads, int batch, int64_t tokens) {
+  if (kv4_takes_prompt(max_q, share)) return plan_prompt(max_q, share, kv_heads, batch, tokens).splits;
+  const int s = plan_rows(max_q, share, kv_heads, batch, tokens).splits;
+  return s > kMaxCluster ? s : 1;
 }
 
 }  // namespace
 
 int launch_kv4_attention(const Kv4AttnArgs& a, int dtype, int head_dim, bool pdl, cudaStream_t stream) {
-  if (kv4_takes_prompt(a.max_q, a.q_heads / a.cache.kv_heads)) {
-    return launch_kv4_prompt(a, dtype, head_dim, pdl, stream);
-  }
   if (dtype == QTTS_BF16) {
-    return head_dim == 128 ? launch_ka<__nv_bfloat16, 128>(a, pdl, stream)
-                           : launch_ka<__nv_bfloat16, 64>(a, pdl, stream);
+    return head_dim == 128 ? launch_ka<__nv_bfloat16, 128>(a, dtype, pdl, stream)
+                           : launch_ka<__nv_bfloat16, 64>(a, dtype, pdl, stream);
   }
-  return head_dim == 128 ? launch_ka<__half, 128>(a, pdl, stream) : launch_ka<__half, 64>(a, pdl, stream);
+  return head_dim == 128 ? launch_ka<__half, 128>(a, dtype, pdl, stream)
+                         : launch_ka<__half, 64>(a, dtype, pdl, stream);
 }
 
 }  // namespace qtts
@@ -796,10 +811,8 @@ extern "C" int64_t qtts_kv4_attention_workspace(int total_q, int max_q, int batc
                                                 int head_dim, int64_t max_tokens) {
   using namespace qtts;
   if (total_q < 1 || max_q < 1 || batch < 1 || kv_heads < 1 || q_heads < 1 || q_heads % kv_heads != 0) return 0;
-  if (kv4_takes_prompt(max_q, q_heads / kv_heads)) return 0;
-  const RowsPlan p = plan_rows(max_q, q_heads / kv_heads, kv_heads, batch, max_tokens);
-  if (p.splits <= kMaxCluster) return 0;
-  return static_cast<int64_t>(total_q) * q_heads * p.splits * (head_dim + 2) * 4;
+  const int splits = workspace_splits(max_q, q_heads / kv_heads, kv_heads, batch, max_tokens);
+  return splits == 1 ? 0 : static_cast<int64_t>(total_q) * q_heads * splits * (head_dim + 2) * 4;
 }
 
 extern "C" int qtts_kv4_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, int dtype,

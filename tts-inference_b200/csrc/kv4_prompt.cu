@@ -75,7 +75,7 @@ __device__ __forceinline__ uint32_t tile_offset(int row, int chunk) {
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kPmThreads, 1)
-    kv4_prompt_kernel(const Kv4AttnArgs a, int tiles_a_cta, uint64_t wait_ns) {
+    kv4_prompt_kernel(const Kv4AttnArgs a, int tiles_a_cta, int splits, uint64_t wait_ns) {
   using S = PromptSmem<D>;
   constexpr int NG = D / kKv4Group;
   constexpr int kWords = D / 8;  // 32-bit words of codes a row; chunks of eight channels
@@ -127,7 +127,8 @@ __global__ void __launch_bounds__(kPmThreads, 1)
 
   // The longest blocks first, of all requests and heads: with `causal` the last rows see most.
   const int rb = static_cast<int>(gridDim.z - 1 - blockIdx.z);
-  const int kvh = blockIdx.x;
+  const int split = blockIdx.x % splits;
+  const int kvh = blockIdx.x / splits;
   const int b = blockIdx.y;
   int start = 0, n = 0;
   bool fine = request_rows(a, b, start, n);
@@ -156,14 +157,20 @@ __global__ void __launch_bounds__(kPmThreads, 1)
       kmax = max(kmax, sees);
     }
   }
-  const int most = max(steps[0], steps[1]);
+  // This CTA's share of the steps: `most` from step j0 on, and what each tile needs of them.
+  const int all = max(steps[0], steps[1]);
+  const int j0 = static_cast<int>(static_cast<int64_t>(all) * split / splits);
+  const int most = static_cast<int>(static_cast<int64_t>(all) * (split + 1) / splits) - j0;
+  steps[0] = max(0, min(steps[0] - j0, most));
+  steps[1] = max(0, min(steps[1] - j0, most));
 
   if (warp >= kPmDqWarp && warp < kPmMmaWarp) {
     // ---------------- operands: one token a thread ----------------
     const int t = tid - kPmDqWarp * 32;
     const int per_page = a.cache.page_size / 16;
     const int32_t* table = a.table + b * a.ld_table;
-    int col = (t / 16) / per_page, off = (t / 16) - col * per_page;
+    const int run0 = (j0 * kPmTile + t) / 16;
+    int col = run0 / per_page, off = run0 - col * per_page;
     const int dcol = (kPmTile / 16) / per_page, doff = (kPmTile / 16) - dcol * per_page;
     // What every row of the block sees from here on: below it no row is masked.
     const int first_lim = a.causal ? len - n + r0 / share + 1 : len;
@@ -172,7 +179,7 @@ __global__ void __launch_bounds__(kPmThreads, 1)
     int64_t row = 0;  // of this thread's token of the step being fetched; -1 beyond the tokens
     auto find = [&](int j) {
       row = -1;
-      if (j * kPmTile + t < kmax) {
+      if ((j0 + j) * kPmTile + t < kmax) {
         int64_t page = table[col];
         if (page < 0 || page >= a.cache.pages) {
           record_status(QTTS_ERR_SHAPE);
@@ -206,7 +213,7 @@ __global__ void __launch_bounds__(kPmThreads, 1)
     bool ok = true;
     for (int j = 0; ok && j < most; ++j) {
       const int s = j % kPmStages;
-      if (j * kPmTile + kPmTile > first_lim) {
+      if ((j0 + j + 1) * kPmTile > first_lim) {
         // Rows that do not see a token must not meet its NaN or infinity (0 * NaN): a token with
         // one among its values becomes zeros there, and NaN in its key for the rows that see it.
         bool bad = false;
@@ -330,9 +337,10 @@ __global__ void __launch_bounds__(kPmThreads, 1)
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t ts = tmem + lanes + kColS + i * kPmTile;
     const uint32_t to = tmem + lanes + kColO + i * D;
-    const int lim = r < rows ? (a.causal ? len - n + r / share + 1 : len) : 0;
+    // What the row sees, from this CTA's first token on.
+    const int lim = r < rows ? (a.causal ? len - n + r / share + 1 : len) - j0 * kPmTile : 0;
     // Tokens that all rows of this tile see (they are in order).
-    const int first_lim = a.causal ? len - n + (r0 + i * kPmTile) / share + 1 : len;
+    const int first_lim = (a.causal ? len - n + (r0 + i * kPmTile) / share + 1 : len) - j0 * kPmTile;
     const bool whole = r0 + i * kPmTile + kPmTile <= rows;
     const float to_log2 = a.scale * 1.4426950408889634f;
     float m = -INFINITY, l = 0.f;
@@ -453,6 +461,11 @@ __global__ void __launch_bounds__(kPmThreads, 1)
       // rows are stored; lane and chunk are swizzled as in the operand tiles.
       const uint32_t qt = smem_u32(smem + S::kQ) + i * S::kTileBytes;
       const int row = tid & 127;
+      const bool part = splits > 1;
+      const int64_t at = part && r < rows ? ((static_cast<int64_t>(start) + r / share) * a.q_heads + kvh * share +
+                                             r % share) * splits + split
+                                          : 0;
+      if (part && r < rows) a.stats[at] = make_float2(m, l);
 #pragma unroll
       for (int c = 0; c < D / (8 * NG); ++c) {
         uint32_t o[8 * NG];
@@ -466,6 +479,20 @@ __global__ void __launch_bounds__(kPmThreads, 1)
         } else {
 #pragma unroll
           for (int k = 0; k < 8 * NG; ++k) o[k] = 0u;
+        }
+        if (part) {  // unnormalized, to be joined; a row that saw nothing leaves its statistics only
+          if (r < rows && m != -INFINITY) {
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+#pragma unroll
+              for (int q = 0; q < 2; ++q) {
+                const int k = 8 * (q * (NG / 2) + g / 2) + (g & 1);
+                *reinterpret_cast<uint4*>(a.parts + at * D + 32 * g + 8 * c + 4 * q) =
+                    make_uint4(o[k], o[k + 2], o[k + 4], o[k + 6]);
+              }
+            }
+          }
+          continue;
         }
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
@@ -482,7 +509,7 @@ __global__ void __launch_bounds__(kPmThreads, 1)
       __syncwarp();
       constexpr int kRowsAStore = 32 / kWords;
 #pragma unroll 4
-      for (int x = 0; x < 32; x += kRowsAStore) {
+      for (int x = 0; !part && x < 32; x += kRowsAStore) {
         const int wrow = (warp & 3) * 32 + x + lane / kWords;
         const int rr = r0 + i * kPmTile + wrow;
         if (rr < rows) {
@@ -501,18 +528,16 @@ __global__ void __launch_bounds__(kPmThreads, 1)
 }
 
 template <typename T, int D>
-int launch_pm(const Kv4AttnArgs& a, int tiles, bool pdl, cudaStream_t stream) {
+int launch_pm(const Kv4AttnArgs& a, const PromptPlan& p, bool pdl, cudaStream_t stream) {
   constexpr int kSmem = PromptSmem<D>::kBytes;
   if (cudaFuncSetAttribute(kv4_prompt_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) !=
       cudaSuccess) {
     (void)cudaGetLastError();
     return QTTS_ERR_LAUNCH;
   }
-  const int64_t rows = static_cast<int64_t>(a.max_q) * (a.q_heads / a.cache.kv_heads);
+  if (p.blocks > 65535) return QTTS_ERR_SHAPE;
   cudaLaunchConfig_t cfg = {};
-  const int64_t blocks = (rows + tiles * kPmTile - 1) / (tiles * kPmTile);
-  if (blocks > 65535) return QTTS_ERR_SHAPE;
-  cfg.gridDim = dim3(a.cache.kv_heads, a.batch, static_cast<unsigned>(blocks));
+  cfg.gridDim = dim3(a.cache.kv_heads * p.splits, a.batch, static_cast<unsigned>(p.blocks));
   cfg.blockDim = dim3(kPmThreads);
   cfg.dynamicSmemBytes = kSmem;
   cfg.stream = stream;
@@ -523,25 +548,38 @@ int launch_pm(const Kv4AttnArgs& a, int tiles, bool pdl, cudaStream_t stream) {
     cfg.attrs = attr;
     cfg.numAttrs = 1;
   }
-  return cudaLaunchKernelEx(&cfg, kv4_prompt_kernel<T, D>, a, tiles, current_wait_limit_ns()) == cudaSuccess
+  return cudaLaunchKernelEx(&cfg, kv4_prompt_kernel<T, D>, a, p.tiles, p.splits, current_wait_limit_ns()) ==
+                 cudaSuccess
              ? QTTS_OK
              : QTTS_ERR_LAUNCH;
 }
 
 }  // namespace
 
-int launch_kv4_prompt(const Kv4AttnArgs& a, int dtype, int head_dim, bool pdl, cudaStream_t stream) {
-  const int64_t rows = static_cast<int64_t>(a.max_q) * (a.q_heads / a.cache.kv_heads);
-  // Two tiles a CTA share the operands and hide each other's softmax; one where two would leave
-  // SMs without a CTA.
-  const int64_t pairs = (rows + 2 * kPmTile - 1) / (2 * kPmTile) * a.cache.kv_heads * a.batch;
-  const int tiles = rows > kPmTile && pairs >= kNumSMs ? 2 : 1;
+PromptPlan plan_prompt(int64_t max_q, int share, int kv_heads, int batch, int64_t most_tokens) {
+  PromptPlan p;
+  const int64_t rows = max_q * share;
+  // Two tiles a CTA share the operands and hide each other's softmax.
+  p.tiles = rows > kPmTile ? 2 : 1;
+  p.blocks = (rows + p.tiles * kPmTile - 1) / (p.tiles * kPmTile);
+  const int64_t units = p.blocks * kv_heads * batch;
+  const int64_t steps = (most_tokens + kPmTile - 1) / kPmTile;
+  // Enough CTAs for three a SM, so that long ones among short ones do not hold the call up, but
+  // at least four steps each.
+  const int64_t want = units >= 2 * kNumSMs ? 1 : (3 * kNumSMs + units - 1) / (units > 0 ? units : 1);
+  const int64_t can = steps / 4;
+  const int64_t s = want < can ? want : can;
+  p.splits = static_cast<int>(s < 1 ? 1 : s > 64 ? 64 : s);
+  return p;
+}
+
+int launch_kv4_prompt(const Kv4AttnArgs& a, const PromptPlan& p, int dtype, int head_dim, bool pdl,
+                      cudaStream_t stream) {
   if (dtype == QTTS_BF16) {
-    return head_dim == 128 ? launch_pm<__nv_bfloat16, 128>(a, tiles, pdl, stream)
-                           : launch_pm<__nv_bfloat16, 64>(a, tiles, pdl, stream);
+    return head_dim == 128 ? launch_pm<__nv_bfloat16, 128>(a, p, pdl, stream)
+                           : launch_pm<__nv_bfloat16, 64>(a, p, pdl, stream);
   }
-  return head_dim == 128 ? launch_pm<__half, 128>(a, tiles, pdl, stream)
-                         : launch_pm<__half, 64>(a, tiles, pdl, stream);
+  return head_dim == 128 ? launch_pm<__half, 128>(a, p, pdl, stream) : launch_pm<__half, 64>(a, p, pdl, stream);
 }
 
 }  // namespace qtts
