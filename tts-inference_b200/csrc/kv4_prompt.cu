@@ -462,10 +462,10 @@ __global__ void __launch_bounds__(kPmThreads, 1)
       const uint32_t qt = smem_u32(smem + S::kQ) + i * S::kTileBytes;
       const int row = tid & 127;
       const bool part = splits > 1;
-      const int64_t at = part && r < rows ? ((static_cast<int64_t>(start) + r / share) * a.q_heads + kvh * share +
-                                             r % share) * splits + split
-                                          : 0;
-      if (part && r < rows) a.stats[at] = make_float2(m, l);
+      const auto part_row = [&](int rr) {
+        return ((static_cast<int64_t>(start) + rr / share) * a.q_heads + kvh * share + rr % share) * splits + split;
+      };
+      if (part && r < rows) a.stats[part_row(r)] = make_float2(m, l);
 #pragma unroll
       for (int c = 0; c < D / (8 * NG); ++c) {
         uint32_t o[8 * NG];
@@ -480,17 +480,31 @@ __global__ void __launch_bounds__(kPmThreads, 1)
 #pragma unroll
           for (int k = 0; k < 8 * NG; ++k) o[k] = 0u;
         }
-        if (part) {  // unnormalized, to be joined; a row that saw nothing leaves its statistics only
-          if (r < rows && m != -INFINITY) {
+        if (part) {
+          // Unnormalized fp32, to be joined: 16 channels of every group are a row of this layout, so
+          // the row goes in two halves.
 #pragma unroll
-            for (int g = 0; g < NG; ++g) {
+          for (int g = 0; g < NG; ++g) {
 #pragma unroll
-              for (int q = 0; q < 2; ++q) {
-                const int k = 8 * (q * (NG / 2) + g / 2) + (g & 1);
-                *reinterpret_cast<uint4*>(a.parts + at * D + 32 * g + 8 * c + 4 * q) =
-                    make_uint4(o[k], o[k + 2], o[k + 4], o[k + 6]);
+            for (int q = 0; q < 2; ++q) {
+              const int k = 8 * (q * (NG / 2) + g / 2) + (g & 1);
+              sts128(qt + tile_offset(row, 4 * g + 2 * (c & 1) + q), o[k], o[k + 2], o[k + 4], o[k + 6]);
+            }
+          }
+          if (c & 1) {
+            __syncwarp();
+            constexpr int kChunks = 4 * NG;
+            const int ch = lane % kChunks;
+#pragma unroll 4
+            for (int x = 0; x < 32; x += 32 / kChunks) {
+              const int wrow = (warp & 3) * 32 + x + lane / kChunks;
+              const int rr = r0 + i * kPmTile + wrow;
+              if (rr < rows) {
+                *reinterpret_cast<uint4*>(a.parts + part_row(rr) * D + 32 * (ch / 4) + 8 * (c - 1) + 4 * (ch % 4)) =
+                    lds128(qt + tile_offset(wrow, ch));
               }
             }
+            __syncwarp();
           }
           continue;
         }
