@@ -4,9 +4,8 @@
 //
 // A CTA takes one or two tiles of rows of one (request, key head) and walks over
 // the tokens, 128 at a time:
-//   * warps 8-11 turn the tile's codes into bf16 in shared memory, one token a
-//     thread: (128 + code) by a mask, minus 128 (exact), times scale plus minimum in
-//     one fused multiply-add, so a key or value is rounded once. Keys and values
+//   * warps 8-11 turn the tile's codes into the activations' type in shared memory,
+//     one token a thread, a key or value rounded once. Keys and values
 //     have the same layout there, 128-byte rows of 64 channels a token,
 //     swizzled: the keys are the K-major B operand of S = Q K^T, the values the
 //     transposed (N-contiguous) B operand of O += P V. The order of channels
@@ -17,7 +16,7 @@
 //     replaces S in tensor memory. The products of one tile run in the order
 //     issued, so S(u + 2) may overwrite P(u);
 //   * warps 0-3 and 4-7 (a thread a row, no exchange between threads) take the
-//     running maximum and sum in fp32 and write P as bf16. The reference maximum
+//     running maximum and sum in fp32 and write P in the operands' type. The reference maximum
 //     follows only when the maximum has grown by more than 2^8, so O is rescaled
 //     rarely (and then waits for the product before); the row's sum divides at the end.
 // Bound by the two products (2 x 512 cycles a tile of 128 x 128 x 128) and, as
@@ -40,7 +39,7 @@ constexpr int kPmThreads = 14 * 32;
 
 template <int D>
 struct PromptSmem {
-  static constexpr int kTileBytes = kPmTile * D * 2;  // a tile of q, keys or values in bf16
+  static constexpr int kTileBytes = kPmTile * D * 2;  // a tile of q, keys or values, 16 bits each
   static constexpr int kQ = 0;
   static constexpr int kK = 2 * kTileBytes;
   static constexpr int kV = kK + kPmStages * kTileBytes;
@@ -58,13 +57,53 @@ __device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
   asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
-// (code * s + z) of nibbles n and n + 4 of a word, as a bf16 pair.
-__device__ __forceinline__ uint32_t nibbles_to_bf16(uint32_t w, int n, uint32_t s, uint32_t z) {
-  uint32_t x = ((w >> (4 * n)) & 0x000F000Fu) | 0x43004300u;  // 128 + code
-  asm("sub.rn.bf16x2 %0, %0, %1;" : "+r"(x) : "r"(0x43004300u));
-  asm("fma.rn.bf16x2 %0, %0, %1, %2;" : "+r"(x) : "r"(s), "r"(z));
-  return x;
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
 }
+
+// The operands' type is the activations'. bf16: a group's scale and minimum as they are held.
+// fp16: both brought to fp16, where they fit because the keys and values were fp16 (the
+// largest finite ones rounded up to 2^16 by bf16 come back to 65504).
+template <typename T>
+struct Operand;
+template <>
+struct Operand<__nv_bfloat16> {
+  static constexpr uint32_t kFormat = 1u;
+  static constexpr float kLift = 0.f;  // exponent that probabilities are lifted by
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return pack_bf16x2(lo, hi); }
+  // Scales (z = false) or minima (z = true) of two groups as a pair.
+  static __device__ __forceinline__ uint32_t params(uint32_t a, uint32_t b, bool z) {
+    return __byte_perm(a, b, z ? 0x7632 : 0x5410);
+  }
+  // code * s + z of nibbles n and n + 4 of a word: 128 + code by a mask, less 128 (exact), and one
+  // rounding in the multiply-add.
+  static __device__ __forceinline__ uint32_t values(uint32_t w, int n, uint32_t s, uint32_t z) {
+    uint32_t x = ((w >> (4 * n)) & 0x000F000Fu) | 0x43004300u;
+    asm("sub.rn.bf16x2 %0, %0, %1;" : "+r"(x) : "r"(0x43004300u));
+    asm("fma.rn.bf16x2 %0, %0, %1, %2;" : "+r"(x) : "r"(s), "r"(z));
+    return x;
+  }
+};
+template <>
+struct Operand<__half> {
+  static constexpr uint32_t kFormat = 0u;
+  static constexpr float kLift = 7.f;  // at most 2^15 while the maximum lags by 2^8; normal down to 2^-21
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return pack_f16x2(lo, hi); }
+  static __device__ __forceinline__ float fit(float x) {
+    return fabsf(x) <= 65536.f ? fminf(fmaxf(x, -65504.f), 65504.f) : x;
+  }
+  static __device__ __forceinline__ uint32_t params(uint32_t a, uint32_t b, bool z) {
+    return z ? pack_f16x2(fit(kv4_min(a)), fit(kv4_min(b))) : pack_f16x2(kv4_scale(a), kv4_scale(b));
+  }
+  static __device__ __forceinline__ uint32_t values(uint32_t w, int n, uint32_t s, uint32_t z) {
+    uint32_t x = ((w >> (4 * n)) & 0x000F000Fu) | 0x64006400u;  // 1024 + code
+    asm("sub.rn.f16x2 %0, %0, %1;" : "+r"(x) : "r"(0x64006400u));
+    asm("fma.rn.f16x2 %0, %0, %1, %2;" : "+r"(x) : "r"(s), "r"(z));
+    return x;
+  }
+};
 __device__ __forceinline__ void sts128(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
@@ -79,8 +118,9 @@ __global__ void __launch_bounds__(kPmThreads, 1)
   using S = PromptSmem<D>;
   constexpr int NG = D / kKv4Group;
   constexpr int kWords = D / 8;  // 32-bit words of codes a row; chunks of eight channels
-  constexpr uint32_t kIdescS = umma_idesc(1u, 1u, kPmTile, kPmSub);
-  constexpr uint32_t kIdescO = umma_idesc(1u, 1u, kPmTile, D) | kUmmaBTransposed;
+  constexpr uint32_t kIdescS = umma_idesc(Operand<T>::kFormat, Operand<T>::kFormat, kPmTile, kPmSub);
+  constexpr uint32_t kIdescO = 
+      umma_idesc(Operand<T>::kFormat, Operand<T>::kFormat, kPmTile, D) | kUmmaBTransposed;
   constexpr uint32_t kColS = 0, kColO = 2 * kPmTile;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -232,13 +272,13 @@ __global__ void __launch_bounds__(kPmThreads, 1)
       // Keys: word c * NG + g holds channels 32 g + 8 c .. + 7, one group; chunk 4 g + c.
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
-        const uint32_t sc = __byte_perm(kp[g], 0u, 0x1010), z = __byte_perm(kp[g], 0u, 0x3232);
+        const uint32_t sc = Operand<T>::params(kp[g], kp[g], false), z = Operand<T>::params(kp[g], kp[g], true);
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           const int wi = c * NG + g;
           const uint32_t w = reinterpret_cast<const uint32_t*>(kc)[wi];
-          sts128(kt + tile_offset(t, 4 * g + c), nibbles_to_bf16(w, 0, sc, z), nibbles_to_bf16(w, 1, sc, z),
-                 nibbles_to_bf16(w, 2, sc, z), nibbles_to_bf16(w, 3, sc, z));
+          sts128(kt + tile_offset(t, 4 * g + c), Operand<T>::values(w, 0, sc, z), Operand<T>::values(w, 1, sc, z),
+                 Operand<T>::values(w, 2, sc, z), Operand<T>::values(w, 3, sc, z));
         }
       }
       fence_proxy_async_smem();
@@ -251,14 +291,14 @@ __global__ void __launch_bounds__(kPmThreads, 1)
       // Values: word wi holds four channels each of two neighbouring groups in its halves.
 #pragma unroll
       for (int h = 0; h < NG / 2; ++h) {
-        const uint32_t sc = __byte_perm(vp[2 * h], vp[2 * h + 1], 0x5410);
-        const uint32_t z = __byte_perm(vp[2 * h], vp[2 * h + 1], 0x7632);
+        const uint32_t sc = Operand<T>::params(vp[2 * h], vp[2 * h + 1], false);
+        const uint32_t z = Operand<T>::params(vp[2 * h], vp[2 * h + 1], true);
 #pragma unroll
         for (int c = 0; c < 8; ++c) {
           const int wi = c * (NG / 2) + h;
           const uint32_t w = reinterpret_cast<const uint32_t*>(vc)[wi];
-          sts128(vt + tile_offset(t, wi), nibbles_to_bf16(w, 0, sc, z), nibbles_to_bf16(w, 1, sc, z),
-                 nibbles_to_bf16(w, 2, sc, z), nibbles_to_bf16(w, 3, sc, z));
+          sts128(vt + tile_offset(t, wi), Operand<T>::values(w, 0, sc, z), Operand<T>::values(w, 1, sc, z),
+                 Operand<T>::values(w, 2, sc, z), Operand<T>::values(w, 3, sc, z));
         }
       }
       fence_proxy_async_smem();
@@ -346,7 +386,7 @@ __global__ void __launch_bounds__(kPmThreads, 1)
     float m = -INFINITY, l = 0.f;
     bool ok = true;
 
-    // q in bf16, channels of a chunk in the order 0 4 1 5 2 6 3 7: kWords lanes a row, eight rows
+    // q, channels of a chunk in the order 0 4 1 5 2 6 3 7: kWords lanes a row, eight rows
     // of loads at a time.
     if (most > 0) {
       constexpr int kRowsAPass = 2 * kPmTile / kWords;
@@ -367,14 +407,7 @@ __global__ void __launch_bounds__(kPmThreads, 1)
         for (int x = 0; x < 8; ++x) {
           const int row = q0 + x * kRowsAPass;
           if (row >= tiles_a_cta * kPmTile) break;
-          uint4 v = u[x];
-          if constexpr (!std::is_same<T, __nv_bfloat16>::value) {
-            const __half* e = reinterpret_cast<const __half*>(&v);
-            v = make_uint4(pack_bf16x2(__half2float(e[0]), __half2float(e[1])),
-                           pack_bf16x2(__half2float(e[2]), __half2float(e[3])),
-                           pack_bf16x2(__half2float(e[4]), __half2float(e[5])),
-                           pack_bf16x2(__half2float(e[6]), __half2float(e[7])));
-          }
+          const uint4 v = u[x];
           sts128(smem_u32(smem + S::kQ) + (row >> 7) * S::kTileBytes + tile_offset(row & 127, ch),
                  __byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632), __byte_perm(v.y, v.w, 0x5410),
                  __byte_perm(v.y, v.w, 0x7632));
@@ -418,7 +451,7 @@ __global__ void __launch_bounds__(kPmThreads, 1)
           }
         }
       }
-      const float off = m == -INFINITY ? 0.f : -m;
+      const float off = Operand<T>::kLift - (m == -INFINITY ? 0.f : m);
       float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
@@ -429,7 +462,7 @@ __global__ void __launch_bounds__(kPmThreads, 1)
           const float y = ex2f(fmaf(__uint_as_float(s[c][k + 1]), to_log2, off));
           sum[k / 2 % 2] += x;
           sum[2 + k / 2 % 2] += y;
-          p[k / 2] = pack_bf16x2(x, y);
+          p[k / 2] = Operand<T>::pack(x, y);
         }
         tmem_st_x16(tb + 16 * c, p);
       }
