@@ -20,6 +20,11 @@ One frame, for a batch of B streams:
   code and appends its embedding.
 
 All shapes are static, so a whole frame is captured in one CUDA graph.
+
+With ``kv_cache="int4"`` the talker keeps its cache in 4 bits (:class:`~qtts_b200.kv4.Kv4Cache`,
+one page of slots a stream) and each of its layers runs as the fused path: residual addition +
+norm + 8-bit activations into the projections (where their quant method is W8A8), per-head norm +
+rotary + cache write in one launch, attention over the 4-bit cache.
 """
 
 from __future__ import annotations
@@ -30,6 +35,7 @@ import torch
 import torch.nn.functional as F
 from torch import nn
 
+from .kv4 import Kv4Cache, kv4_attention, rope_kv4_append
 from .layers.linear import LinearBase
 
 
@@ -117,6 +123,21 @@ class Block(nn.Module):
         h = x + self.o_proj(att.transpose(1, 2).reshape(b, 1, -1))
         return self._mlp(h)
 
+    def decode_kv4(self, delta: torch.Tensor, residual: torch.Tensor | None, cache: Kv4Cache, slots: torch.Tensor,
+                   table: torch.Tensor, lengths: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
+                   positions: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+        """One token per stream over a 4-bit cache. ``residual + delta`` is the layer's input
+        (``residual`` None: delta alone), and what it returns the same pair for the next layer.
+        ``slots`` and ``positions`` place the new tokens, ``table`` and ``lengths`` (these included)
+        say what each stream sees; cos/sin are the whole tables."""
+        b = delta.shape[0]
+        qkv, h = self.qkv_proj.forward_add_rmsnorm(delta, residual, self.input_norm)
+        q = rope_kv4_append(qkv, cache, slots, self.d.heads, cos=cos, sin=sin, positions=positions,
+                            q_norm=self.q_norm, k_norm=self.k_norm)
+        att = kv4_attention(q, cache, table, lengths)
+        gate_up, h = self.gate_up_proj.forward_add_rmsnorm(self.o_proj(att.view(b, -1)), h, self.post_norm)
+        return self.down_proj.forward_silu_mul(gate_up), h
+
     def prefix(self, x: torch.Tensor, cos, sin) -> torch.Tensor:
         """Causal attention over the whole (short) sequence, no cache."""
         b, t, _ = x.shape
@@ -128,8 +149,10 @@ class Block(nn.Module):
 
 class Talker(nn.Module):
     def __init__(self, batch: int, dtype=torch.bfloat16, device="cuda", layers: int = TALKER.layers,
-                 seed: int = 0) -> None:
+                 seed: int = 0, kv_cache: str = "bf16") -> None:
         super().__init__()
+        if kv_cache not in ("bf16", "int4"):
+            raise ValueError(f"kv_cache {kv_cache!r} is not 'bf16' or 'int4'")
         d = Dims(layers=layers, hidden=TALKER.hidden, inter=TALKER.inter)
         self.d = d
         self.layers = nn.ModuleList([Block(d, dtype, device) for _ in range(layers)])
@@ -147,13 +170,45 @@ class Talker(nn.Module):
         self.logit_mask = mask
         self.pos = PRIOR_TOKENS
         self.cos, self.sin = rope_tables(torch.tensor([self.pos], device=device), d.head_dim)
+        self.kv4: list[Kv4Cache] | None = None
+        if kv_cache == "int4":
+            self._hold_in_4_bits(batch, slots, device)
+
+    def _hold_in_4_bits(self, batch: int, slots: int, device) -> None:
+        """Move the prior tokens to 4-bit caches, one page of ``slots`` tokens a stream."""
+        d, prior = self.d, self.pos
+        first = torch.arange(batch, device=device)[:, None] * slots
+        places = (first + torch.arange(prior, device=device)).flatten()
+        self.kv4 = []
+        for k, v in zip(self.cache_k, self.cache_v):
+            cache = Kv4Cache.empty(batch, d.kv_heads, slots, d.head_dim, device=device)
+            kv = torch.cat([t[:, :, :prior].transpose(1, 2).reshape(batch * prior, -1) for t in (k, v)], dim=-1)
+            rope_kv4_append(kv, cache, places, 0)
+            self.kv4.append(cache)
+        del self.cache_k, self.cache_v
+        self.kv4_slots = first.flatten() + prior
+        self.kv4_table = torch.arange(batch, dtype=torch.int32, device=device)[:, None]
+        self.kv4_lengths = torch.full((batch,), prior + 1, dtype=torch.int32, device=device)
+        self.kv4_positions = torch.full((batch,), prior, dtype=torch.int64, device=device)
+        self.kv4_cos, self.kv4_sin = rope_tables(torch.arange(slots, device=device), d.head_dim)
+
+    def _step_kv4(self, x: torch.Tensor) -> torch.Tensor:
+        delta, h = x, None
+        for layer, cache in zip(self.layers, self.kv4):
+            delta, h = layer.decode_kv4(delta, h, cache, self.kv4_slots, self.kv4_table, self.kv4_lengths,
+                                        self.kv4_cos, self.kv4_sin, self.kv4_positions)
+        return h + delta
 
     def step(self, x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
         """x [B, hidden] -> (last hidden [B, hidden], greedy code 0 [B])."""
-        h = x[:, None, :]
-        for i, layer in enumerate(self.layers):
-            h = layer.decode(h, self.cache_k[i], self.cache_v[i], self.pos, self.cos, self.sin)
-        h = rms_norm(h[:, 0], self.norm)
+        if self.kv4 is not None:
+            h = self._step_kv4(x)
+        else:
+            h = x[:, None, :]
+            for i, layer in enumerate(self.layers):
+                h = layer.decode(h, self.cache_k[i], self.cache_v[i], self.pos, self.cos, self.sin)
+            h = h[:, 0]
+        h = rms_norm(h, self.norm)
         logits = self.codec_head(h).float() + self.logit_mask
         return h, logits.argmax(dim=-1)
 
@@ -238,9 +293,10 @@ class Frame:
     """Talker step + code predictor for a batch of streams, capturable as one CUDA graph."""
 
     def __init__(self, batch: int = 8, *, device="cuda", talker_layers: int = TALKER.layers,
-                 predictor_layers: int = PREDICTOR.layers, codebooks: int = CODEBOOKS - 1, seed: int = 0) -> None:
+                 predictor_layers: int = PREDICTOR.layers, codebooks: int = CODEBOOKS - 1, seed: int = 0,
+                 kv_cache: str = "bf16") -> None:
         self.batch = batch
-        self.talker = Talker(batch, device=device, layers=talker_layers, seed=seed + 3)
+        self.talker = Talker(batch, device=device, layers=talker_layers, seed=seed + 3, kv_cache=kv_cache)
         self.predictor = CodePredictor(device=device, layers=predictor_layers, codebooks=codebooks, seed=seed + 4)
         random_init_(self.talker, seed)
         random_init_(self.predictor, seed + 1)

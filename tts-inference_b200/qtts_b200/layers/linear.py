@@ -63,6 +63,19 @@ class LinearBase(nn.Module):
             return fused(self, x, norm_weight, eps, self.bias)
         return self(F.rms_norm(x, (x.shape[-1],), norm_weight, eps))
 
+    def forward_add_rmsnorm(
+        self, x: torch.Tensor, residual: torch.Tensor | None, norm_weight: torch.Tensor, eps: float = 1e-6
+    ) -> tuple[torch.Tensor, torch.Tensor]:
+        """``h = x + residual; (self(rms_norm(h)), h)``: the residual stream's addition and norm
+        ahead of this projection (qtts/models/talker.py:249, 271). A quant method with
+        ``apply_add_rmsnorm`` (the W8A8 ones) runs addition, norm and the activations'
+        quantization in one launch. ``residual`` None is a stream that starts here."""
+        fused = getattr(self.quant_method, "apply_add_rmsnorm", None)
+        if fused is not None:
+            return fused(self, x, residual, norm_weight, eps, self.bias)
+        h = x if residual is None else x + residual
+        return self.forward_rmsnorm(h, norm_weight, eps), h
+
     def forward_silu_mul(self, gate_up: torch.Tensor) -> torch.Tensor:
         """``self(F.silu(gate) * up)`` of ``gate_up = [gate | up]``: the down projection of a
         gated MLP (qtts/layers/activation.py:143-147), fused where the quant method can."""

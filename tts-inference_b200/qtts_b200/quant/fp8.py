@@ -22,7 +22,14 @@ from ..layers.linear import LinearBase
 from ..utils import get_logger
 from .base import QuantMethodBase
 from .calibrate import worth_quantizing
-from .kernels import fp8_quant_rows, fp8_scaled_mm, fp8w_gemm, kernel_available, quantize_fp8_rows
+from .kernels import (
+    add_rms_norm_quant,
+    fp8_quant_rows,
+    fp8_scaled_mm,
+    fp8w_gemm,
+    kernel_available,
+    quantize_fp8_rows,
+)
 
 logger = get_logger("quant.fp8")
 
@@ -74,6 +81,23 @@ class Fp8Method(QuantMethodBase):
             x.dtype,
         )
         return out.reshape(*shape[:-1], layer.out_features)
+
+    def apply_add_rmsnorm(self, layer: LinearBase, x: torch.Tensor, residual: torch.Tensor | None,
+                          norm_weight: torch.Tensor, eps: float,
+                          bias: torch.Tensor | None) -> tuple[torch.Tensor, torch.Tensor]:
+        """``h = x + residual; (apply(layer, rms_norm(h), bias), h)`` with addition, norm and
+        per-token quantization in one launch (fp32 up to the codes: the norm is not rounded to
+        the activation type in between, as the separate ops do)."""
+        q, scale_x, h = add_rms_norm_quant(x, residual, norm_weight, eps, dtype=torch.float8_e4m3fn)
+        out = fp8_scaled_mm(
+            q,
+            scale_x,
+            layer.fp8_weight.t(),  # type: ignore[attr-defined]
+            layer.fp8_scale,  # type: ignore[attr-defined]
+            bias,
+            x.dtype,
+        )
+        return out.reshape(*x.shape[:-1], layer.out_features), x if h is None else h
 
 
 class Fp8WeightOnlyMethod(QuantMethodBase):

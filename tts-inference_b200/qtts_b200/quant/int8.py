@@ -26,6 +26,7 @@ from ..utils import get_logger
 from .base import QuantMethodBase
 from .calibrate import choose_variant, lookup_variant, worth_quantizing
 from .kernels import (
+    add_rms_norm_quant,
     i8_scaled_mm,
     int8_quant_rows,
     kernel_available,
@@ -219,3 +220,15 @@ class Int8Method(QuantMethodBase):
             q, scale_x, layer.int8_weight.t(), layer.int8_scale, bias, x.dtype  # type: ignore[attr-defined]
         )
         return out.reshape(*shape[:-1], layer.out_features)
+
+    def apply_add_rmsnorm(self, layer: LinearBase, x: torch.Tensor, residual: torch.Tensor | None,
+                          norm_weight: torch.Tensor, eps: float,
+                          bias: torch.Tensor | None) -> tuple[torch.Tensor, torch.Tensor]:
+        """``h = x + residual; (apply(layer, rms_norm(h), bias), h)`` with addition, norm and
+        per-token quantization in one launch (fp32 up to the codes, so neither the norm nor the
+        scale is rounded to the activation type as in ``apply``)."""
+        q, scale_x, h = add_rms_norm_quant(x, residual, norm_weight, eps, dtype=torch.int8)
+        out = i8_scaled_mm(
+            q, scale_x, layer.int8_weight.t(), layer.int8_scale, bias, x.dtype  # type: ignore[attr-defined]
+        )
+        return out.reshape(*x.shape[:-1], layer.out_features), x if h is None else h
