@@ -26,9 +26,10 @@
 //     may lag by 2^8, and the small ones normal down to 2^-21;
 //   * every warp streams its own tiles of 32 tokens through a ring of asynchronous copies
 //     and keeps its own running maximum and sum; the warps of a CTA meet in shared
-//     memory, and where there are few (request, head) pairs a cluster of up to 16
-//     CTAs splits one of them and meets in distributed shared memory: one launch,
-//     no workspace, sums in a fixed order.
+//     memory, and where there are few (request, head) pairs a cluster of up to 8
+//     CTAs splits one of them and meets in distributed shared memory, or, where
+//     that is not enough to fill the machine, any number of CTAs through a
+//     workspace that a second kernel joins. Sums are in a fixed order.
 #include <type_traits>
 
 #include "kernels.h"
@@ -108,7 +109,8 @@ struct RowsSmem {
 };
 
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 4 : 2) kv4_rows_kernel(const Kv4AttnArgs a, int row_blocks) {
+__global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 3 : 2) kv4_rows_kernel(const Kv4AttnArgs a, int row_blocks,
+                                                                                int warp_tiles) {
   using S = RowsSmem<D>;
   constexpr int NG = D / kKv4Group;
   constexpr int kRows = 8 * NT;
@@ -122,7 +124,6 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 4 : 2) kv4_rows_kernel(
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   const int g = lane >> 2, c = lane & 3;
-  const int splits = gridDim.x;
   const int rank = blockIdx.x;
   const int rb = blockIdx.y % row_blocks;
   const int kvh = blockIdx.y / row_blocks;
@@ -147,7 +148,14 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 4 : 2) kv4_rows_kernel(
   const int last = (min(rows, r0 + kRows) - 1) / share;  // its last new token
   const int first_lim = a.causal ? len - n + r0 / share + 1 : len;  // what its first row sees (may be negative)
   const int kmax = r0 >= rows ? 0 : max(0, a.causal ? len - n + last + 1 : len);
-  const int tiles = (kmax + kTile - 1) / kTile;
+  int tiles = (kmax + kTile - 1) / kTile;
+  // CTAs that take part in this unit: as many as have warp_tiles tiles for each warp. The others
+  // leave (one at least stays, to answer for a unit that sees nothing).
+  const int splits = max(1, min(static_cast<int>(gridDim.x), (tiles + warps * warp_tiles - 1) / (warps * warp_tiles)));
+  if (rank >= splits) {
+    if (a.parts == nullptr) return;
+    tiles = 0;  // only says that it saw nothing
+  }
 
   // This warp's tiles: every (splits * warps)-th one, 16 bytes a lane and copy into a ring. A
   // tile is two runs of 16 tokens, each within one page. Column and row within the page advance
@@ -604,7 +612,7 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 4 : 2) kv4_rows_kernel(
       *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + orow * a.out_token_stride + head * D + ch) =
           *reinterpret_cast<uint2*>(v);
     } else if (mode == 2) {
-      const int64_t at_row = (orow * a.q_heads + head) * splits + rank;
+      const int64_t at_row = (orow * a.q_heads + head) * gridDim.x + rank;
       if (top != -INFINITY) *reinterpret_cast<float4*>(a.parts + at_row * D + ch) = o;
       if (ch == 0) a.stats[at_row] = make_float2(top, lsum);
     } else {
@@ -695,7 +703,8 @@ bool kv4_takes_prompt(int64_t max_q, int share) { return max_q * share >= kPromp
 struct RowsPlan {
   int nt;
   int64_t row_blocks;
-  int splits;
+  int splits;      // CTAs at most
+  int warp_tiles;  // tiles a warp for which another CTA joins in
 };
 
 RowsPlan plan_rows(int64_t max_q, int share, int kv_heads, int batch, int64_t most_tokens) {
@@ -704,17 +713,18 @@ RowsPlan plan_rows(int64_t max_q, int share, int kv_heads, int batch, int64_t mo
   p.nt = rows <= 8 ? 1 : 2;
   p.row_blocks = (rows + 8 * p.nt - 1) / (8 * p.nt);
   const int64_t units = p.row_blocks * kv_heads * batch;
-  // One wave of CTAs (four of 128 threads an SM; two with 16 rows, for their registers), at
-  // least one tile a warp; and, as far as a cluster goes, no more than 8 tiles a warp, so that
-  // one long request among short ones does not hold the call up (many units even out by
-  // themselves).
-  const int64_t wave = static_cast<int64_t>(kNumSMs) * (p.nt == 1 ? 4 : 2);
+  // One wave of CTAs (three of 128 threads an SM; two with 16 rows, for their registers), at
+  // least one tile a warp; and, as far as a cluster goes, no more than 8 tiles a warp of the longest
+  // request, so that it does not hold the others up (CTAs that a shorter one has no use for
+  // leave at once).
+  const int64_t wave = static_cast<int64_t>(kNumSMs) * (p.nt == 1 ? 3 : 2);
   const int64_t tiles = (most_tokens + kTile - 1) / kTile;
   const int64_t want = wave / (units > 0 ? units : 1);
   const int64_t can = (tiles + kWarps - 1) / kWarps;
   const int64_t even = (tiles + 8 * kWarps - 1) / (8 * kWarps);
   int64_t s = even < kMaxCluster ? even : kMaxCluster;
-  if (s * units > 8 * wave) s = 1;
+  if (s * units > 16 * wave) s = 16 * wave / units;
+  p.warp_tiles = s > want ? 4 : 1;
   if (s < want) s = want;
   if (s > can) s = can;
   p.splits = static_cast<int>(s < 1 ? 1 : s > 256 ? 256 : s);
@@ -762,7 +772,8 @@ int launch_rows(Kv4AttnArgs a, const RowsPlan& p, bool pdl, cudaStream_t stream)
   if (!workspace) a.parts = nullptr, a.stats = nullptr;
   return launch(kv4_rows_kernel<T, D, NT>,
                 dim3(p.splits, static_cast<unsigned>(p.row_blocks * a.cache.kv_heads), a.batch), 32 * kWarps, kSmem,
-                workspace ? 1 : p.splits, pdl, stream, a, static_cast<int>(p.row_blocks));
+                workspace ? 1 : p.splits, pdl, stream, a, static_cast<int>(p.row_blocks),
+                p.warp_tiles);
 }
 
 template <typename T, int D>
