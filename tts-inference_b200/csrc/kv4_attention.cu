@@ -42,6 +42,8 @@ constexpr int kTile = 32;   // tokens a warp takes at a time
 constexpr int kStages = 2;  // tiles in flight a warp
 constexpr int kWarps = 4;   // a CTA
 constexpr int kMaxCluster = 8;
+constexpr int kMaxSplits = 512;  // parts of a row in the workspace
+constexpr int kFewSplits = 32;   // up to which one warp joins a row
 
 // Nibbles n and n + 4 (n = 0, 1) of a word as a pair of fp16 subnormals: code * 2^-24 for
 // n = 0, code * 2^-20 for n = 1; nibbles n + 2 and n + 6 from the word shifted by eight.
@@ -663,35 +665,100 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 3 : 2) kv4_rows_kernel(
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-// The parts of each (token, head) row from the workspace, one warp a row.
-template <typename T, int D>
-__global__ void __launch_bounds__(128) kv4_join_kernel(const Kv4AttnArgs a, int splits) {
+// The parts of a (token, head) row from the workspace. Bound by latency: all statistics are read
+// at once, and four parts a warp are in flight. Eight warps a row where there are many parts (one
+// long cache: 256 parts in 4 us instead of 28 with one warp), one where there are many rows.
+constexpr int kJoinWarps = 8;  // a CTA
+
+template <typename T, int D, int kRowWarps>
+__global__ void __launch_bounds__(32 * kJoinWarps) kv4_join_kernel(const Kv4AttnArgs a, int splits) {
+  constexpr int kPer = D / 32;  // channels a lane
+  constexpr int kRows = kJoinWarps / kRowWarps;
+  constexpr int kParts = kRowWarps == 1 ? kFewSplits : kMaxSplits;
+  constexpr int kSlots = (kParts + 32 * kRowWarps - 1) / (32 * kRowWarps);
+  __shared__ float weight[kRows][kParts];
+  __shared__ float red[2][kJoinWarps];
+  __shared__ float out[kJoinWarps][D];
   pdl_launch_dependents();
   pdl_wait();
-  const int lane = threadIdx.x & 31;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
-  if (row >= static_cast<int64_t>(a.total_q) * a.q_heads) return;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int sub = warp / kRowWarps, rw = warp % kRowWarps;
+  const int tid = rw * 32 + lane;  // within the row
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + sub;
+  const bool there = row < static_cast<int64_t>(a.total_q) * a.q_heads;
   const float2* st = a.stats + row * splits;
+  float2 s[kSlots];
   float top = -INFINITY;
-  for (int q = lane; q < splits; q += 32) top = fmaxf(top, st[q].x);
+#pragma unroll
+  for (int k = 0; k < kSlots; ++k) {
+    const int q = tid + k * 32 * kRowWarps;
+    s[k] = there && q < splits ? st[q] : make_float2(-INFINITY, 0.f);
+    top = fmaxf(top, s[k].x);
+  }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  const float safe = top == -INFINITY ? 0.f : top;
-  float lsum = 0.f, out[D / 32] = {};
-  const float* part = a.parts + row * splits * D + lane * (D / 32);
-#pragma unroll 4
-  for (int q = 0; q < splits; ++q) {
-    const float2 s = st[q];
-    if (s.x == -INFINITY) continue;  // saw nothing: its part was not written
-    const float f = ex2(s.x - safe);
-    lsum = fmaf(f, s.y, lsum);
+  if constexpr (kRowWarps > 1) {
+    if (lane == 0) red[0][warp] = top;
+    __syncthreads();
 #pragma unroll
-    for (int i = 0; i < D / 32; ++i) out[i] = fmaf(f, part[static_cast<int64_t>(q) * D + i], out[i]);
+    for (int w = 0; w < kRowWarps; ++w) top = fmaxf(top, red[0][sub * kRowWarps + w]);
   }
-  const float inv = lsum == 0.f ? 0.f : 1.f / lsum;
-  T* dst = static_cast<T*>(a.out) + row / a.q_heads * a.out_token_stride + row % a.q_heads * D + lane * (D / 32);
+  const float safe = top == -INFINITY ? 0.f : top;
+  float lsum = 0.f;
 #pragma unroll
-  for (int i = 0; i < D / 32; ++i) dst[i] = from_float<T>(out[i] * inv);
+  for (int k = 0; k < kSlots; ++k) {
+    const int q = tid + k * 32 * kRowWarps;
+    // A part that saw nothing was not written: its weight is exactly 0 and it is passed over.
+    const float f = s[k].x == -INFINITY ? 0.f : ex2(s[k].x - safe);
+    lsum = fmaf(f, s[k].y, lsum);
+    if (q < splits) weight[sub][q] = f;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) lsum += __shfl_xor_sync(0xffffffffu, lsum, o);
+  if constexpr (kRowWarps > 1) {
+    if (lane == 0) red[1][warp] = lsum;
+    __syncthreads();
+  } else {
+    __syncwarp();
+  }
+  float acc[kPer] = {};
+  const float* part = a.parts + row * splits * D + lane * kPer;
+#pragma unroll 4
+  for (int q = rw; q < splits; q += kRowWarps) {
+    const float f = weight[sub][q];
+    float x[kPer] = {};
+    if (there && f != 0.f) {
+      if constexpr (kPer == 4) {
+        *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(part + static_cast<int64_t>(q) * D);
+      } else {
+        *reinterpret_cast<float2*>(x) = *reinterpret_cast<const float2*>(part + static_cast<int64_t>(q) * D);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) acc[i] = fmaf(f, x[i], acc[i]);
+  }
+  T* dst = static_cast<T*>(a.out) + row / a.q_heads * a.out_token_stride + row % a.q_heads * D;
+  if constexpr (kRowWarps > 1) {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) out[warp][lane * kPer + i] = acc[i];
+    __syncthreads();
+    if (there && tid < D) {
+      float l = 0.f, o = 0.f;
+#pragma unroll
+      for (int w = 0; w < kRowWarps; ++w) l += red[1][sub * kRowWarps + w], o += out[sub * kRowWarps + w][tid];
+      dst[tid] = from_float<T>(l == 0.f ? 0.f : o / l);
+    }
+  } else if (there) {
+    const float inv = lsum == 0.f ? 0.f : 1.f / lsum;
+    T v[kPer];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) v[i] = from_float<T>(acc[i] * inv);
+    if constexpr (kPer == 4) {
+      *reinterpret_cast<uint2*>(dst + lane * kPer) = *reinterpret_cast<uint2*>(v);
+    } else {
+      *reinterpret_cast<uint32_t*>(dst + lane * kPer) = *reinterpret_cast<uint32_t*>(v);
+    }
+  }
 }
 
 // Rows a request from which whole 128-row tiles are the faster.
@@ -727,7 +794,7 @@ RowsPlan plan_rows(int64_t max_q, int share, int kv_heads, int batch, int64_t mo
   p.warp_tiles = s > want ? 4 : 1;
   if (s < want) s = want;
   if (s > can) s = can;
-  p.splits = static_cast<int>(s < 1 ? 1 : s > 256 ? 256 : s);
+  p.splits = static_cast<int>(s < 1 ? 1 : s > kMaxSplits ? kMaxSplits : s);
   return p;
 }
 
@@ -779,8 +846,12 @@ int launch_rows(Kv4AttnArgs a, const RowsPlan& p, bool pdl, cudaStream_t stream)
 template <typename T, int D>
 int launch_join(const Kv4AttnArgs& a, int splits, cudaStream_t stream) {
   const int64_t rows = static_cast<int64_t>(a.total_q) * a.q_heads;
-  return launch(kv4_join_kernel<T, D>, dim3(static_cast<unsigned>((rows + 3) / 4)), 128, 0, 1, true, stream, a,
-                splits);
+  if (splits <= kFewSplits) {
+    return launch(kv4_join_kernel<T, D, 1>, dim3(static_cast<unsigned>((rows + kJoinWarps - 1) / kJoinWarps)),
+                  32 * kJoinWarps, 0, 1, true, stream, a, splits);
+  }
+  return launch(kv4_join_kernel<T, D, kJoinWarps>, dim3(static_cast<unsigned>(rows)), 32 * kJoinWarps, 0, 1, true,
+                stream, a, splits);
 }
 
 template <typename T, int D>
