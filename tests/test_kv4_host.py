@@ -157,3 +157,42 @@ def test_wrappers_refuse():
     for args, kw, err in (((x, x, w[:32]), {}, ValueError), ((x, x, w), dict(dtype=torch.uint8), TypeError)):
         with pytest.raises(err):
             qk.add_rms_norm_quant(*args, **kw)
+
+
+def test_fast_calls_convert_as_ctypes_does(lib):
+    """The converted-argument calls against ctypes: the same answers, and errors instead of
+    wrong conversions."""
+    fast = nat._fastcall()
+    if fast is None:
+        pytest.skip("csrc/fastcall.c is not built here")
+
+    def both(name, args):
+        slow = nat._through_ctypes(name)
+        assert getattr(fast, name)(*args) == slow(*args)
+
+    norm = [16, 64, 16, 64, 16, 1e-6, 16, 64, nat.BF16, 16, 64, nat.E4M3, 16, 4, 64, 0, None]
+    write_args = [16, 32 * 128, nat.BF16, 3, 16, 8, 128, None, None, 1e-6, 16, 16, 10, 16, 3, 1, (64,), False, 16, 16,
+                  16 * 128, 16, 16, 16, 16, 2, 16, None, None, 0, None]
+    attend_args = [16, 16 * 128, 128, nat.BF16, 16, 16, 16, 16, 4, 16, 16, 2, 2, 16, None, 3, 1, 3, 16, 8, 128, 0.1, True,
+                   16, 16 * 128, None, 0, None]
+    for name, args, bad in (("qtts_add_rms_norm_quant", norm, (13, 14, 1, 8, 11)),
+                            ("qtts_rope_kv4_append", write_args, (3, 5, 1, 2, 26)),
+                            ("qtts_kv4_attention", attend_args, (17, 19, 1, 3, 9))):
+        if not torch.cuda.is_available():
+            both(name, args)
+        for at in bad:
+            both(name, args[:at] + [-1] + args[at + 1:])
+        both(name, [None] + args[1:])
+        both(name, [1 << 40 | 1] + args[1:])
+        with pytest.raises(TypeError):
+            getattr(fast, name)(*args[:-1])
+        with pytest.raises(TypeError):
+            getattr(fast, name)("x", *args[1:])
+        with pytest.raises(OverflowError):
+            getattr(fast, name)(*args[:3], *[1 << 40 if i == bad[0] else a for i, a in enumerate(args) if i >= 3])
+    for sections in ((24, 20, 20), (63,), None):
+        both("qtts_rope_kv4_append", write_args[:15] + [len(sections or (1,)), sections] + write_args[17:])
+    with pytest.raises(TypeError):
+        fast.qtts_rope_kv4_append(*write_args[:16], (1, 2, 3, 4, 5), *write_args[17:])
+    with pytest.raises(TypeError):
+        fast.bind(1, 2)

@@ -150,13 +150,17 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 3 : 2) kv4_rows_kernel(
   const int last = (min(rows, r0 + kRows) - 1) / share;  // its last new token
   const int first_lim = a.causal ? len - n + r0 / share + 1 : len;  // what its first row sees (may be negative)
   const int kmax = r0 >= rows ? 0 : max(0, a.causal ? len - n + last + 1 : len);
-  int tiles = (kmax + kTile - 1) / kTile;
+  const int tiles = (kmax + kTile - 1) / kTile;
   // CTAs that take part in this unit: as many as have warp_tiles tiles for each warp. The others
   // leave (one at least stays, to answer for a unit that sees nothing).
   const int splits = max(1, min(static_cast<int>(gridDim.x), (tiles + warps * warp_tiles - 1) / (warps * warp_tiles)));
   if (rank >= splits) {
-    if (a.parts == nullptr) return;
-    tiles = 0;  // only says that it saw nothing
+    if (a.parts != nullptr && threadIdx.x < kRows && r0 + threadIdx.x < rows) {  // says that it saw nothing
+      const int rr = r0 + threadIdx.x;
+      const int64_t orow = static_cast<int64_t>(start + rr / share) * a.q_heads + kvh * share + rr % share;
+      a.stats[orow * gridDim.x + rank] = make_float2(-INFINITY, 0.f);
+    }
+    return;
   }
 
   // This warp's tiles: every (splits * warps)-th one, 16 bytes a lane and copy into a ring. A
@@ -774,6 +778,7 @@ struct RowsPlan {
   int warp_tiles;  // tiles a warp for which another CTA joins in
 };
 
+constexpr int kEven = 16, kEvenMax = 8;
 RowsPlan plan_rows(int64_t max_q, int share, int kv_heads, int batch, int64_t most_tokens) {
   RowsPlan p;
   const int64_t rows = max_q * share;
@@ -788,8 +793,8 @@ RowsPlan plan_rows(int64_t max_q, int share, int kv_heads, int batch, int64_t mo
   const int64_t tiles = (most_tokens + kTile - 1) / kTile;
   const int64_t want = wave / (units > 0 ? units : 1);
   const int64_t can = (tiles + kWarps - 1) / kWarps;
-  const int64_t even = (tiles + 8 * kWarps - 1) / (8 * kWarps);
-  int64_t s = even < kMaxCluster ? even : kMaxCluster;
+  const int64_t even = (tiles + kEven * kWarps - 1) / (kEven * kWarps);
+  int64_t s = even < kEvenMax ? even : kEvenMax;
   if (s * units > 16 * wave) s = 16 * wave / units;
   p.warp_tiles = s > want ? 4 : 1;
   if (s < want) s = want;

@@ -9,12 +9,13 @@ point raises ``RuntimeError`` with the reason.
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import threading
 from pathlib import Path
 
 import torch
 
-from .build import LIB_PATH
+from .build import FAST_PATH, LIB_PATH
 
 # dtype codes (enum qtts_dtype)
 BF16, FP16, FP32, E4M3, INT8 = 0, 1, 2, 3, 4
@@ -220,10 +221,52 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
 _raw_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
+#: Entry points that ``launch`` calls; csrc/fastcall.c converts their arguments where it is built.
+_LAUNCHED = ("qtts_add_rms_norm_quant", "qtts_rope_kv4_append", "qtts_kv4_attention")
+_calls: dict[str, object] = {}
+
+
+def _fastcall():
+    """The module built from csrc/fastcall.c, bound to the loaded library; None where it is not built."""
+    path = Path(FAST_PATH)
+    if not path.exists():
+        return None
+    spec = importlib.util.spec_from_file_location("_qtts_fastcall", path)
+    module = importlib.util.module_from_spec(spec)
+    try:
+        spec.loader.exec_module(module)
+    except ImportError:  # built for another Python
+        return None
+    module.bind(*(ctypes.cast(getattr(lib(), name), ctypes.c_void_p).value for name in _LAUNCHED))
+    return module
+
+
+def _through_ctypes(name: str):
+    fn = getattr(lib(), name)
+    if name != "qtts_rope_kv4_append":
+        return fn
+
+    def call(*args):  # the axis shares come as a tuple
+        args = list(args)
+        if args[16] is not None:
+            args[16] = (ctypes.c_int * len(args[16]))(*args[16])
+        return fn(*args)
+
+    return call
+
+
+def _bind_calls() -> None:
+    fast = _fastcall()
+    for name in _LAUNCHED:
+        _calls[name] = getattr(fast, name) if fast is not None else _through_ctypes(name)
+
+
 def launch(name: str, index: int, *args) -> None:
     """Call entry point ``name`` with ``args`` and, after them, the current stream of device
     ``index``, with that device current."""
-    fn = getattr(_lib or _load(), name)
+    if not _calls:
+        _bind_calls()
+    fn = _calls[name]
     if _raw_device() == index:
         code = fn(*args, _raw_stream(index))
     else:

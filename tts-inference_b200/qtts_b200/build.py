@@ -14,6 +14,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG_DIR = Path(__file__).resolve().parent
@@ -22,6 +23,9 @@ REPO_DIR = PKG_DIR.parent.parent
 INCLUDE_DIR = REPO_DIR / "include"
 LIB_DIR = PKG_DIR / "lib"
 LIB_PATH = LIB_DIR / "libqtts_b200.so"
+
+#: Argument conversion of the hot entry points (csrc/fastcall.c), built where CPython's headers are.
+FAST_PATH = LIB_DIR / ("_qtts_fastcall" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = [
@@ -77,6 +81,8 @@ def build(force: bool = False, verbose: bool = False, extra_flags: list[str] | N
     nvcc per file), then one nvcc call device-links and links them into the
     shared library."""
     if not force and not _stale():
+        if not FAST_PATH.exists():
+            build_fastcall(verbose)
         return LIB_PATH
     from concurrent.futures import ThreadPoolExecutor
 
@@ -94,7 +100,22 @@ def build(force: bool = False, verbose: bool = False, extra_flags: list[str] | N
     _run([nvcc_path()] + ARCH_FLAGS + ["-shared", "-Xcompiler", "-fPIC", "-o", str(tmp)] + [str(o) for o in objs],
          verbose)
     os.replace(tmp, LIB_PATH)
+    build_fastcall(verbose)
     return LIB_PATH
+
+
+def build_fastcall(verbose: bool = False) -> Path | None:
+    """Compile the fast argument conversion; None where there is no C compiler or no Python.h
+    (the binding then goes through ctypes)."""
+    include = Path(sysconfig.get_paths()["include"])
+    cc = shutil.which("gcc") or shutil.which("cc")
+    if cc is None or not (include / "Python.h").exists():
+        return None
+    LIB_DIR.mkdir(parents=True, exist_ok=True)
+    tmp = FAST_PATH.with_suffix(".so.tmp")
+    _run([cc, "-O2", "-fPIC", "-shared", "-I", str(include), "-o", str(tmp), str(SRC_DIR / "fastcall.c")], verbose)
+    os.replace(tmp, FAST_PATH)
+    return FAST_PATH
 
 
 if __name__ == "__main__":

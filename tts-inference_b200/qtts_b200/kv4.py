@@ -18,7 +18,6 @@ lengths) are checked by the kernels: one out of range is left out and recorded
 
 from __future__ import annotations
 
-import ctypes
 import math
 
 import torch
@@ -31,8 +30,7 @@ HEAD_DIMS = (64, 128)
 _HALVES = (32, 64)
 _DTYPES = {torch.bfloat16: nat.BF16, torch.float16: nat.FP16}
 _SCALES = {d: 1.0 / math.sqrt(d) for d in HEAD_DIMS}
-_SPLIT_FROM = 512  # tokens
-_SECTIONS: dict[tuple[int, ...], ctypes.Array] = {}  # host arrays of the axis shares, by their values
+_SPLIT_FROM = 1024  # tokens
 
 
 class Kv4Cache:
@@ -146,7 +144,7 @@ def rope_kv4_append(
     if qkv.stride(1) != 1 or qkv.stride(0) % 8 or qkv.data_ptr() % 16:
         qkv = qkv.clone(memory_format=torch.contiguous_format)
     axes = table_len = ldpos = 0
-    cos_ptr = sin_ptr = pos_ptr = section_array = None
+    cos_ptr = sin_ptr = pos_ptr = None
     if cos is not None:
         if positions is None:
             raise ValueError("positions are needed with cos and sin")
@@ -155,9 +153,6 @@ def rope_kv4_append(
             raise ValueError(f"positions must be int64 [axes, {tokens}] with unit stride along the tokens")
         axes = positions.shape[0] if positions.dim() == 2 else 1
         sections = (d // 2,) if sections is None else tuple(sections)
-        section_array = _SECTIONS.get(sections)
-        if section_array is None:
-            section_array = _SECTIONS[sections] = (ctypes.c_int * len(sections))(*sections)
         if len(sections) != axes or not 1 <= axes <= 4 or sum(sections) != d // 2 or min(sections) < 0:
             raise ValueError(f"sections {sections} do not share {d // 2} pairs among {axes} axes")
         table_shape = cos.shape
@@ -186,7 +181,7 @@ def rope_kv4_append(
     nat.launch(
         "qtts_rope_kv4_append", index, qkv.data_ptr(), qkv.stride(0) if tokens > 1 else width, dtype, tokens, q_heads,
         kv_heads, d, None if q_norm is None else q_norm.data_ptr(), None if k_norm is None else k_norm.data_ptr(), eps,
-        cos_ptr, sin_ptr, table_len, pos_ptr, ldpos, axes, section_array, interleaved, slots.data_ptr(), q.data_ptr(),
+        cos_ptr, sin_ptr, table_len, pos_ptr, ldpos, axes, sections if axes else None, interleaved, slots.data_ptr(), q.data_ptr(),
         q_heads * d, *cache._ptrs, k_ptr, v_ptr, _flags())
     return (q, k_values, v_values) if values else q
 
@@ -263,7 +258,8 @@ def kv4_attention(
         raise ValueError(f"scale {scale} is not positive and finite")
     if index < 0 or cache._index != index or block_table.get_device() != index or lengths.get_device() != index:
         _require_cuda(q, cache.k_codes, block_table, lengths)
-    if q.is_contiguous():
+    dense = q.is_contiguous()
+    if dense:
         token_stride, head_stride = heads * d, d
     else:
         token_stride, head_stride = q.stride(0), q.stride(1)
@@ -275,7 +271,7 @@ def kv4_attention(
         q = q.clone(memory_format=torch.contiguous_format)
         q_ptr, token_stride, head_stride = q.data_ptr(), heads * d, d
     if out is None:
-        out = q.new_empty(shape)
+        out = torch.empty_like(q) if dense else q.new_empty(shape)
     elif out.shape != shape or out.dtype is not q.dtype or not out.is_contiguous() or out.get_device() != index:
         raise ValueError(f"out must be a contiguous {q.dtype} {tuple(shape)} on q's device")
     work_ptr = None

@@ -212,7 +212,7 @@ def add_rms_norm_quant(
             ldr = r.stride(0) if rows > 1 else width
             r_ptr = r.data_ptr()
         if residual_out is None:
-            residual_out = x.new_empty(shape)
+            residual_out = torch.empty_like(x) if flat else x.new_empty(shape)
         elif residual_out.get_device() != index:
             _require_cuda(x, residual_out)
         if residual_out.is_contiguous() and residual_out.shape == shape and residual_out.dtype is xtype:
@@ -225,7 +225,7 @@ def add_rms_norm_quant(
             ro_ptr = ro.data_ptr()
     elif residual_out is not None:
         raise ValueError("residual_out needs a residual")
-    q = x.new_empty((rows, width), dtype=dtype)
+    q = torch.empty_like(x, dtype=dtype) if flat else x.new_empty((rows, width), dtype=dtype)
     scale = x.new_empty((rows, 1), dtype=torch.float32)
     nat.launch("qtts_add_rms_norm_quant", index, a.data_ptr(), lda, r_ptr, ldr, weight.data_ptr(), eps, ro_ptr, ldro,
                nat.dtype_code(xtype), q.data_ptr(), width, nat.dtype_code(dtype), scale.data_ptr(), rows, width,
