@@ -243,7 +243,8 @@ struct Kv4AttnArgs {
 struct PromptPlan {
   int tiles;
   int64_t blocks;
-  int splits;
+  int splits;       // at most
+  int split_steps;  // 128-token steps for which another CTA joins in
 };
 PromptPlan plan_prompt(int64_t max_q, int share, int kv_heads, int batch, int64_t most_tokens);
 int launch_kv4_prompt(const Kv4AttnArgs& a, const PromptPlan& p, int dtype, int head_dim, bool pdl,

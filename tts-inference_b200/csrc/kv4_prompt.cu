@@ -114,7 +114,7 @@ __device__ __forceinline__ uint32_t tile_offset(int row, int chunk) {
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kPmThreads, 1)
-    kv4_prompt_kernel(const Kv4AttnArgs a, int tiles_a_cta, int splits, uint64_t wait_ns) {
+    kv4_prompt_kernel(const Kv4AttnArgs a, int tiles_a_cta, int max_splits, int split_steps, uint64_t wait_ns) {
   using S = PromptSmem<D>;
   constexpr int NG = D / kKv4Group;
   constexpr int kWords = D / 8;  // 32-bit words of codes a row; chunks of eight channels
@@ -167,8 +167,8 @@ __global__ void __launch_bounds__(kPmThreads, 1)
 
   // The longest blocks first, of all requests and heads: with `causal` the last rows see most.
   const int rb = static_cast<int>(gridDim.z - 1 - blockIdx.z);
-  const int split = blockIdx.x % splits;
-  const int kvh = blockIdx.x / splits;
+  const int split = blockIdx.x % max_splits;
+  const int kvh = blockIdx.x / max_splits;
   const int b = blockIdx.y;
   int start = 0, n = 0;
   bool fine = request_rows(a, b, start, n);
@@ -199,8 +199,12 @@ __global__ void __launch_bounds__(kPmThreads, 1)
   }
   // This CTA's share of the steps: `most` from step j0 on, and what each tile needs of them.
   const int all = max(steps[0], steps[1]);
-  const int j0 = static_cast<int>(static_cast<int64_t>(all) * split / splits);
-  const int most = static_cast<int>(static_cast<int64_t>(all) * (split + 1) / splits) - j0;
+  // CTAs that take part: one for every split_steps steps. The others only say that they saw
+  // nothing.
+  const int splits = max(1, min(max_splits, (all + split_steps - 1) / split_steps));
+  const bool idle = split >= splits;
+  const int j0 = idle ? 0 : static_cast<int>(static_cast<int64_t>(all) * split / splits);
+  const int most = idle ? 0 : static_cast<int>(static_cast<int64_t>(all) * (split + 1) / splits) - j0;
   steps[0] = max(0, min(steps[0] - j0, most));
   steps[1] = max(0, min(steps[1] - j0, most));
 
@@ -494,9 +498,9 @@ __global__ void __launch_bounds__(kPmThreads, 1)
       // rows are stored; lane and chunk are swizzled as in the operand tiles.
       const uint32_t qt = smem_u32(smem + S::kQ) + i * S::kTileBytes;
       const int row = tid & 127;
-      const bool part = splits > 1;
+      const bool part = max_splits > 1;
       const auto part_row = [&](int rr) {
-        return ((static_cast<int64_t>(start) + rr / share) * a.q_heads + kvh * share + rr % share) * splits + split;
+        return ((static_cast<int64_t>(start) + rr / share) * a.q_heads + kvh * share + rr % share) * max_splits + split;
       };
       if (part && r < rows) a.stats[part_row(r)] = make_float2(m, l);
 #pragma unroll
@@ -513,6 +517,7 @@ __global__ void __launch_bounds__(kPmThreads, 1)
 #pragma unroll
           for (int k = 0; k < 8 * NG; ++k) o[k] = 0u;
         }
+        if (part && steps[i] == 0) break;
         if (part) {
           // Unnormalized fp32, to be joined: 16 channels of every group are a row of this layout, so
           // the row goes in two halves.
@@ -595,7 +600,7 @@ int launch_pm(const Kv4AttnArgs& a, const PromptPlan& p, bool pdl, cudaStream_t 
     cfg.attrs = attr;
     cfg.numAttrs = 1;
   }
-  return cudaLaunchKernelEx(&cfg, kv4_prompt_kernel<T, D>, a, p.tiles, p.splits, current_wait_limit_ns()) ==
+  return cudaLaunchKernelEx(&cfg, kv4_prompt_kernel<T, D>, a, p.tiles, p.splits, p.split_steps, current_wait_limit_ns()) ==
                  cudaSuccess
              ? QTTS_OK
              : QTTS_ERR_LAUNCH;
@@ -612,11 +617,12 @@ PromptPlan plan_prompt(int64_t max_q, int share, int kv_heads, int batch, int64_
   const int64_t units = p.blocks * kv_heads * batch;
   const int64_t steps = (most_tokens + kPmTile - 1) / kPmTile;
   // Enough CTAs for three a SM, so that long ones among short ones do not hold the call up, but
-  // at least four steps each.
+  // at least four steps each of the longest request (a shorter one takes fewer CTAs).
   const int64_t want = units >= 2 * kNumSMs ? 1 : (3 * kNumSMs + units - 1) / (units > 0 ? units : 1);
   const int64_t can = steps / 4;
   const int64_t s = want < can ? want : can;
   p.splits = static_cast<int>(s < 1 ? 1 : s > 64 ? 64 : s);
+  p.split_steps = static_cast<int>((steps + p.splits - 1) / p.splits);
   return p;
 }
 
