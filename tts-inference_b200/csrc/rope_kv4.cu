@@ -48,13 +48,20 @@ __device__ __forceinline__ uint32_t quantize_group(const float (&y)[8], float lo
   const float s = __bfloat162float(sb), z = __bfloat162float(zb);
   // A scale below 2^-60 is divided by 2^64 times larger, as is what it divides, so that
   // reciprocal and remainder stay in range.
-  const float up = s < 0x1p-60f ? 0x1p64f : 1.f;
-  const float su = s * up;
+  float x[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = y[i] - z;
+  float su = s;
+  if (s < 0x1p-60f) {
+    su *= 0x1p64f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] *= 0x1p64f;
+  }
   const float r = s > 0.f ? __frcp_rn(su) : 0.f;
   float c[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float q = fminf(fmaxf(divide((y[i] - z) * up, su, r), 0.f), 15.f);
+    const float q = fminf(fmaxf(divide(x[i], su, r), 0.f), 15.f);
     c[i] = (q + 12582912.f) - 12582912.f;  // 1.5 * 2^23: to the nearest whole number, ties to even
     held[i] = fmaf(c[i], s, z);            // c * s is exact
   }
@@ -94,9 +101,8 @@ __global__ void __launch_bounds__(32, 20) rope_kv4_kernel(const RopeKv4Args a, i
 
   // A token with a position outside the tables gives zeros and is not stored.
   bool ok = true;
-  float cs[8], sn[8];
+  int64_t pos[kMaxRopeAxes] = {};
   if (a.cos != nullptr) {
-    int64_t pos[kMaxRopeAxes];
 #pragma unroll
     for (int x = 0; x < kMaxRopeAxes; ++x) {
       pos[x] = x < a.axes ? a.positions[x * a.ldpos + t] : 0;
@@ -106,16 +112,6 @@ __global__ void __launch_bounds__(32, 20) rope_kv4_kernel(const RopeKv4Args a, i
       }
     }
     if (!ok && lane == 0) record_status(QTTS_ERR_SHAPE);
-    const int j0 = 8 * (l % (kLanes / 2));  // first of this lane's pairs
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int j = j0 + i;
-      const int axis = static_cast<int>(a.axis_of[j >> 5] >> (2 * (j & 31))) & 3;
-      const int64_t at = (axis == 0 ? pos[0] : axis == 1 ? pos[1] : axis == 2 ? pos[2] : pos[3]) * (D / 2) + j;
-      cs[i] = __ldg(a.cos + at);
-      const float s = __ldg(a.sin + at);
-      sn[i] = l < kLanes / 2 ? -s : s;
-    }
   }
   const int64_t slot = a.slots[t];
   const bool inside = slot < a.cache.pages * a.cache.page_size;
@@ -124,29 +120,63 @@ __global__ void __launch_bounds__(32, 20) rope_kv4_kernel(const RopeKv4Args a, i
   const int64_t page = stored ? slot / a.cache.page_size : 0;
   const int in_page = stored ? static_cast<int>(slot - page * a.cache.page_size) : 0;
 
-  // Head (within its kind) of this lane in pass p, and the pass's kind: 0 q, 1 k, 2 v.
-  const auto kind_of = [&](int p) { return p < nq ? 0 : p < nq + nk ? 1 : 2; };
-  const auto head_of = [&](int p, int kind) { return (p - (kind == 0 ? 0 : kind == 1 ? nq : nq + nk)) * kHeads + sub; };
-
-  const auto norm = [&](float(&y)[8], const void* weight) {
-    float ss = leaf_sumsq(y);
+  // A head row through norm and rotation is y_i = inv * (x_i A_i + x_partner B_i), A and B the
+  // norm's weights times cosine and signed sine: gathered once for all heads of a kind.
+  float fa[8], fb[8];
+  const auto factors = [&](const void* weight) {
+    const int partner = l < kLanes / 2 ? l + kLanes / 2 : l - kLanes / 2;
 #pragma unroll
-    for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    const float inv = rsqrtf(ss * (1.0f / D) + a.eps);
-    const uint4 wr = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(weight) + 8 * l));
-    const T* we = reinterpret_cast<const T*>(&wr);
+    for (int i = 0; i < 8; ++i) fa[i] = 1.f, fb[i] = 0.f;
+    if (a.cos != nullptr) {
+      const int j0 = 8 * (l % (kLanes / 2));  // first of this lane's pairs
 #pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = rms_apply(y[i], inv, to_float(we[i]));
-  };
-  const auto turn = [&](float(&y)[8]) {
+      for (int i = 0; i < 8; ++i) {
+        const int j = j0 + i;
+        const int axis = static_cast<int>(a.axis_of[j >> 5] >> (2 * (j & 31))) & 3;
+        const int64_t at = (axis == 0 ? pos[0] : axis == 1 ? pos[1] : axis == 2 ? pos[2] : pos[3]) * (D / 2) + j;
+        fa[i] = __ldg(a.cos + at);
+        const float sn = __ldg(a.sin + at);
+        fb[i] = l < kLanes / 2 ? -sn : sn;
+      }
+    }
+    if (weight != nullptr) {
+      const uint4 w0 = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(weight) + 8 * l));
+      const uint4 w1 = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(weight) + 8 * partner));
+      const T* e0 = reinterpret_cast<const T*>(&w0);
+      const T* e1 = reinterpret_cast<const T*>(&w1);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float other = __shfl_xor_sync(0xffffffffu, y[i], kLanes / 2);
-      y[i] = __fadd_rn(__fmul_rn(y[i], cs[i]), __fmul_rn(other, sn[i]));
+      for (int i = 0; i < 8; ++i) fa[i] *= to_float(e0[i]), fb[i] *= to_float(e1[i]);
     }
   };
-  const auto quantize = [&](const float(&y)[8], bool live, int h, uint8_t* codes, uint32_t* all_params, void* values,
-                            auto is_value) {
+  const auto turn = [&](const uint4& raw, float(&y)[8], bool norm) {
+    uint4 other = raw;
+    if (a.cos != nullptr) {
+      other.x = __shfl_xor_sync(0xffffffffu, raw.x, kLanes / 2);
+      other.y = __shfl_xor_sync(0xffffffffu, raw.y, kLanes / 2);
+      other.z = __shfl_xor_sync(0xffffffffu, raw.z, kLanes / 2);
+      other.w = __shfl_xor_sync(0xffffffffu, raw.w, kLanes / 2);
+    }
+    const T* e = reinterpret_cast<const T*>(&raw);
+    const T* o = reinterpret_cast<const T*>(&other);
+    float inv = 1.f;
+    if (norm) {
+      float ss = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) ss = fmaf(to_float(e[i]), to_float(e[i]), ss);
+#pragma unroll
+      for (int q = kLanes / 2; q > 0; q >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, q);
+      inv = rsqrtf(ss * (1.0f / D) + a.eps);
+    }
+    if (a.cos != nullptr) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = inv * fmaf(to_float(o[i]), fb[i], to_float(e[i]) * fa[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = inv * (to_float(e[i]) * fa[i]);
+    }
+  };
+  // Codes, parameters and (where asked for) the values of a head row, through this lane's pointers.
+  const auto quantize = [&](const float(&y)[8], bool live, uint8_t* codes, uint32_t* param, T* values, auto is_value) {
     float lo = y[0], hi = y[0];
 #pragma unroll
     for (int i = 1; i < 8; ++i) lo = nan_min(lo, y[i]), hi = nan_max(hi, y[i]);
@@ -158,61 +188,82 @@ __global__ void __launch_bounds__(32, 20) rope_kv4_kernel(const RopeKv4Args a, i
     uint32_t params;
     float held[8];
     const uint32_t word = quantize_group(y, lo, hi, params, held);
-    if (values != nullptr && live) {
-      __stcs(reinterpret_cast<uint4*>(static_cast<T*>(values) + (t * kvh + h) * D + 8 * l), pack8<T>(held));
-    }
-    if (stored && live) {
-      const int64_t row = kv4_row(a.cache, page, h, in_page);
-      const int j = l / 4, c = l % 4;
+    if (!live) return;
+    if (a.k_values != nullptr) __stcs(reinterpret_cast<uint4*>(values), pack8<T>(held));
+    if (stored) {
       if constexpr (decltype(is_value)::value) {
-        uint16_t* dst = reinterpret_cast<uint16_t*>(codes + row * (D / 2));
-        dst[(2 * c) * kGroups + j] = static_cast<uint16_t>(word & 0xffffu);
-        dst[(2 * c + 1) * kGroups + j] = static_cast<uint16_t>(word >> 16);
+        *reinterpret_cast<uint16_t*>(codes) = static_cast<uint16_t>(word & 0xffffu);
+        *reinterpret_cast<uint16_t*>(codes + 2 * kGroups) = static_cast<uint16_t>(word >> 16);
       } else {
-        reinterpret_cast<uint32_t*>(codes + row * (D / 2))[c * kGroups + j] = word;
+        *reinterpret_cast<uint32_t*>(codes) = word;
       }
-      if (c == 0) all_params[row * kGroups + j] = params;
+      if (l % 4 == 0) *param = params;
     }
   };
 
-  const auto fetch = [&](int p) {
-    uint4 raw = make_uint4(0u, 0u, 0u, 0u);
-    const int kind = kind_of(p), h = head_of(p, kind);
-    if (p < p_end && ok && h < (kind == 0 ? a.q_heads : kvh)) {
-      raw = __ldcs(reinterpret_cast<const uint4*>(
-          src + (h + (kind == 0 ? 0 : kind == 1 ? a.q_heads : a.q_heads + kvh)) * D));
+  // The passes of one kind that are this warp's, kAhead rows in flight. A lane beyond the kind's heads
+  // loads the last one again and stores nothing. Everything that moves with the pass is a pointer.
+  const auto run = [&](auto kind_c, int base, int count, const void* weight) {
+    constexpr int kKind = decltype(kind_c)::value;
+    const int kind_heads = kKind == 0 ? a.q_heads : kvh;
+    const int from = max(p_first - base, 0), to = min(p_end - base, count);
+    if (from >= to) return;
+    const T* at = src + static_cast<int64_t>(kKind == 0 ? 0 : kKind == 1 ? a.q_heads : a.q_heads + kvh) * D;
+    const auto fetch = [&](int p) {
+      return __ldcs(reinterpret_cast<const uint4*>(at + min(min(p, to - 1) * kHeads + sub, kind_heads - 1) * D));
+    };
+    uint4 raw[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) raw[u] = fetch(from + u);
+    if constexpr (kKind < 2) factors(weight);
+    const int h0 = from * kHeads + sub;
+    T* out = nullptr;            // q, or the values
+    uint8_t* codes = nullptr;    // this lane's place in the head's row
+    uint32_t* params = nullptr;  // its group's
+    int64_t codes_step = 0, params_step = 0;
+    if constexpr (kKind == 0) {
+      out = static_cast<T*>(a.q_out) + t * a.ldq + h0 * D + 8 * l;
+    } else {
+      out = static_cast<T*>(kKind == 1 ? a.k_values : a.v_values) + (t * kvh + h0) * D + 8 * l;
+      const int64_t row = kv4_row(a.cache, page, h0, in_page);
+      const int j = l / 4, c = l % 4;
+      codes = (kKind == 1 ? a.cache.k_codes : a.cache.v_codes) + row * (D / 2) +
+              (kKind == 1 ? 4 * (c * kGroups + j) : 2 * (2 * c * kGroups + j));
+      params = (kKind == 1 ? a.cache.k_params : a.cache.v_params) + row * kGroups + j;
+      codes_step = static_cast<int64_t>(kHeads) * a.cache.page_size * (D / 2);
+      params_step = static_cast<int64_t>(kHeads) * a.cache.page_size * kGroups;
     }
-    return raw;
+    for (int p0 = from; p0 < to; p0 += kAhead) {
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const int p = p0 + u;
+        if (p < to) {
+          uint4 now = raw[u];
+          if (p + kAhead < to) raw[u] = fetch(p + kAhead);
+          if (!ok) now = make_uint4(0u, 0u, 0u, 0u);
+          const bool live = p * kHeads + sub < kind_heads;
+          float y[8];
+          if constexpr (kKind < 2) {
+            turn(now, y, weight != nullptr);
+          } else {
+            const T* e = reinterpret_cast<const T*>(&now);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) y[i] = to_float(e[i]);
+          }
+          if constexpr (kKind == 0) {
+            if (live) *reinterpret_cast<uint4*>(out) = pack8<T>(y);
+          } else {
+            quantize(y, live, codes, params, out, std::integral_constant<bool, kKind == 2>{});
+            codes += codes_step, params += params_step;
+          }
+          out += kHeads * D;
+        }
+      }
+    }
   };
-  uint4 raw[kAhead];
-#pragma unroll
-  for (int u = 0; u < kAhead; ++u) raw[u] = fetch(p_first + u);
-  for (int p0 = p_first; p0 < p_end; p0 += kAhead) {
-#pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      const int p = p0 + u;
-      if (p >= p_end) break;
-      const int kind = kind_of(p), h = head_of(p, kind);
-      const bool live = h < (kind == 0 ? a.q_heads : kvh);
-      const T* e = reinterpret_cast<const T*>(&raw[u]);
-      float y[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] = to_float(e[i]);
-      raw[u] = fetch(p + kAhead);
-      if (kind == 2) {
-        quantize(y, live, h, a.cache.v_codes, a.cache.v_params, a.v_values, std::true_type{});
-        continue;
-      }
-      const void* weight = kind == 0 ? a.q_norm : a.k_norm;
-      if (weight != nullptr) norm(y, weight);
-      if (a.cos != nullptr) turn(y);
-      if (kind == 1) {
-        quantize(y, live, h, a.cache.k_codes, a.cache.k_params, a.k_values, std::false_type{});
-      } else if (live) {
-        *reinterpret_cast<uint4*>(static_cast<T*>(a.q_out) + t * a.ldq + h * D + 8 * l) = pack8<T>(y);
-      }
-    }
-  }
+  run(std::integral_constant<int, 0>{}, 0, nq, a.q_norm);
+  run(std::integral_constant<int, 1>{}, nq, nk, a.k_norm);
+  run(std::integral_constant<int, 2>{}, nq + nk, nk, nullptr);
 }
 
 template <typename T, int D>
