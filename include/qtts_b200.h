@@ -424,9 +424,11 @@ QTTS_API int qtts_rope_kv4_append(const void* qkv, int64_t ldqkv, int dtype, int
  * gives zeros. What lies in the cache beyond a row's tokens is never used, be it
  * NaN.
  *   q           token and head strides in elements (multiples of 8), BF16 or FP16
- *   block_table [batch, table_cols] int32 page numbers, leading dimension ld_table
+ *   block_table [batch, table_cols] int32 page numbers, leading dimension ld_table;
+ *               table_cols * page_size is at most 2^30
  *   lengths     [batch] int32, at most table_cols * page_size
- *   q_starts    [batch + 1] int32 first rows of q; NULL: max_q rows a request
+ *   q_starts    [batch + 1] int32 first rows of q; NULL: max_q rows a request. Rows
+ *               of no request are not written
  *   max_q       the most new tokens of any request (bounds the launch)
  *   scale       positive and finite
  *   out         [total_q, q_heads, head_dim] of q's type, token stride given

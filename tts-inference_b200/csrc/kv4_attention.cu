@@ -765,9 +765,23 @@ __global__ void __launch_bounds__(32 * kJoinWarps) kv4_join_kernel(const Kv4Attn
   }
 }
 
-// Rows a request from which whole 128-row tiles are the faster.
-constexpr int64_t kPromptRows = 64;
-bool kv4_takes_prompt(int64_t max_q, int share) { return max_q * share >= kPromptRows; }
+// Which kernel: 16-row blocks that each read the cache (kv4_rows_kernel), or 128-row tiles
+// (kv4_prompt.cu), whose time hardly depends on how many of a tile's rows there are. Times
+// of the two in microseconds, 16 query and 8 key heads of 128 channels, from a request's
+// rows (new tokens x 2):
+//                                      32 rows        64 rows        128 rows
+//   1 request,   1000 tokens        9.9 |  19.5    10.4 |  19.8    12.9 |  19.4
+//   8 requests,  1000 tokens       18.8 |  21.6    19.9 |  21.7    37.6 |  22.1
+//   8 requests,  8192 tokens       72.4 | 117.6   141.8 | 118.7   270.2 | 113.7
+//   64 requests, 2048 tokens      120.4 | 169.3   222.8 | 169.8   435.4 | 152.8
+// So few rows stay here whatever the length, more than one tile's go there, and between
+// them the blocks are the faster while their work (blocks x tokens) fits about one wave.
+constexpr int64_t kPromptRows = 64, kTileRows = 128, kWaveTokens = 1 << 18;
+bool kv4_takes_prompt(int64_t max_q, int share, int kv_heads, int batch, int64_t tokens) {
+  const int64_t rows = max_q * share;
+  if (rows < kPromptRows || rows > kTileRows) return rows > kTileRows;
+  return (rows + 15) / 16 * kv_heads * batch * tokens > kWaveTokens;
+}
 
 // How a call is laid out: rows a CTA, and CTAs that share the tokens of one (request, key
 // head, row block).
@@ -778,23 +792,29 @@ struct RowsPlan {
   int warp_tiles;  // tiles a warp for which another CTA joins in
 };
 
-constexpr int kEven = 16, kEvenMax = 8;
+// Tiles that a warp of the longest request gets at most, as far as kEvenCtas CTAs (a
+// cluster) do it: a long request then holds the others of the call up less. With no
+// limit | 8 tiles | 16 tiles: 64 requests of 17 to 8192 tokens 105 | 65 | 59 us; 64 of 4096
+// tokens 87 | 96 | 82 us; 128 of 1000 to 2000 tokens 71 | 84 | 71 us.
+constexpr int kEvenTiles = 16, kEvenCtas = 8;
+
 RowsPlan plan_rows(int64_t max_q, int share, int kv_heads, int batch, int64_t most_tokens) {
   RowsPlan p;
   const int64_t rows = max_q * share;
+  // Eight rows fill an operand; more share what is made of the cache by pairs of eight
+  // (64 x 2048 tokens: 8 rows 51 us, 16 rows 67).
   p.nt = rows <= 8 ? 1 : 2;
   p.row_blocks = (rows + 8 * p.nt - 1) / (8 * p.nt);
   const int64_t units = p.row_blocks * kv_heads * batch;
-  // One wave of CTAs (three of 128 threads an SM; two with 16 rows, for their registers), at
-  // least one tile a warp; and, as far as a cluster goes, no more than 8 tiles a warp of the longest
-  // request, so that it does not hold the others up (CTAs that a shorter one has no use for
-  // leave at once).
+  // One wave of CTAs (three of 128 threads an SM at 168 registers: 77 us for 4 x 65536
+  // tokens, against 83 with four at 128 registers; two with 16 rows), at least one tile a
+  // warp, and the limit above. CTAs that a shorter request has no use for leave at once.
   const int64_t wave = static_cast<int64_t>(kNumSMs) * (p.nt == 1 ? 3 : 2);
   const int64_t tiles = (most_tokens + kTile - 1) / kTile;
   const int64_t want = wave / (units > 0 ? units : 1);
   const int64_t can = (tiles + kWarps - 1) / kWarps;
-  const int64_t even = (tiles + kEven * kWarps - 1) / (kEven * kWarps);
-  int64_t s = even < kEvenMax ? even : kEvenMax;
+  const int64_t even = (tiles + kEvenTiles * kWarps - 1) / (kEvenTiles * kWarps);
+  int64_t s = even < kEvenCtas ? even : kEvenCtas;
   if (s * units > 16 * wave) s = 16 * wave / units;
   p.warp_tiles = s > want ? 4 : 1;
   if (s < want) s = want;
@@ -863,7 +883,7 @@ template <typename T, int D>
 int launch_ka(const Kv4AttnArgs& a, int dtype, bool pdl, cudaStream_t stream) {
   const int share = a.q_heads / a.cache.kv_heads;
   const int64_t tokens = static_cast<int64_t>(a.table_cols) * a.cache.page_size;
-  if (kv4_takes_prompt(a.max_q, share)) {
+  if (kv4_takes_prompt(a.max_q, share, a.cache.kv_heads, a.batch, tokens)) {
     const PromptPlan p = plan_prompt(a.max_q, share, a.cache.kv_heads, a.batch, tokens);
     const int r = launch_kv4_prompt(a, p, dtype, D, pdl, stream);
     return r != QTTS_OK || p.splits == 1 ? r : launch_join<T, D>(a, p.splits, stream);
@@ -876,7 +896,9 @@ int launch_ka(const Kv4AttnArgs& a, int dtype, bool pdl, cudaStream_t stream) {
 
 // CTAs whose parts meet in the workspace; 1 where none do.
 int workspace_splits(int64_t max_q, int share, int kv_heads, int batch, int64_t tokens) {
-  if (kv4_takes_prompt(max_q, share)) return plan_prompt(max_q, share, kv_heads, batch, tokens).splits;
+  if (kv4_takes_prompt(max_q, share, kv_heads, batch, tokens)) {
+    return plan_prompt(max_q, share, kv_heads, batch, tokens).splits;
+  }
   const int s = plan_rows(max_q, share, kv_heads, batch, tokens).splits;
   return s > kMaxCluster ? s : 1;
 }
@@ -919,7 +941,7 @@ extern "C" int qtts_kv4_attention(const void* q, int64_t q_token_stride, int64_t
   if (dtype != QTTS_BF16 && dtype != QTTS_FP16) return QTTS_ERR_DTYPE;
   if (batch == 0 || total_q == 0 || max_q == 0) return QTTS_OK;
   if (q_starts == nullptr && static_cast<int64_t>(batch) * max_q != total_q) return QTTS_ERR_SHAPE;
-  if (static_cast<int64_t>(table_cols) * page_size > 0x7fffffff) return QTTS_ERR_SHAPE;
+  if (static_cast<int64_t>(table_cols) * page_size > (1 << 30)) return QTTS_ERR_SHAPE;
   if (q == nullptr || out == nullptr || lengths == nullptr) return QTTS_ERR_NULL;
   if (table_cols > 0 && block_table == nullptr) return QTTS_ERR_NULL;
   if (pages > 0 && (k_codes == nullptr || k_params == nullptr || v_codes == nullptr || v_params == nullptr)) {
