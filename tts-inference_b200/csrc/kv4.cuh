@@ -35,6 +35,13 @@ __device__ __forceinline__ int64_t kv4_row(const Kv4Cache& c, int64_t page, int 
 __device__ __forceinline__ float kv4_scale(uint32_t p) { return __uint_as_float(p << 16); }
 __device__ __forceinline__ float kv4_min(uint32_t p) { return __uint_as_float(p & 0xffff0000u); }
 
+// n / d for 0 <= n < 2^31 by inv = (2^32 - 1) / d, rounded down: n inv / 2^32 falls short of the
+// quotient by less than one.
+__device__ __forceinline__ int div_by(int n, int d, uint32_t inv) {
+  const int q = static_cast<int>(__umulhi(static_cast<uint32_t>(n), inv));
+  return q + (n - q * d >= d ? 1 : 0);
+}
+
 // First row and number of new tokens of request b, checked against the arguments.
 __device__ __forceinline__ bool request_rows(const Kv4AttnArgs& a, int b, int& start, int& n) {
   if (a.q_starts == nullptr) {

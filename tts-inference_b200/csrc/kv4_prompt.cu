@@ -114,7 +114,8 @@ __device__ __forceinline__ uint32_t tile_offset(int row, int chunk) {
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kPmThreads, 1)
-    kv4_prompt_kernel(const Kv4AttnArgs a, int tiles_a_cta, int max_splits, int split_steps, uint64_t wait_ns) {
+    kv4_prompt_kernel(const Kv4AttnArgs a, int tiles_a_cta, int max_splits, int split_steps, uint32_t share_inv,
+                      uint32_t page_inv, uint64_t wait_ns) {
   using S = PromptSmem<D>;
   constexpr int NG = D / kKv4Group;
   constexpr int kWords = D / 8;  // 32-bit words of codes a row; chunks of eight channels
@@ -133,8 +134,8 @@ __global__ void __launch_bounds__(kPmThreads, 1)
   uint64_t* odone = pfull + 4;           // [tile]: O has taken one more P
   uint64_t* ofull = odone + 2;           // [tile]: all of O is there
   uint64_t* mdone = ofull + 2;           // [tile]: everything issued is done
-  uint64_t* qfull = mdone + 2;           // q is there
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(qfull + 1);
+  uint64_t* qfull = mdone + 2;           // [tile]: q is there
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(qfull + 2);
 
   const int tid = threadIdx.x;
   const int warp = tid >> 5;
@@ -151,28 +152,28 @@ __global__ void __launch_bounds__(kPmThreads, 1)
       mbar_init(&pfull[i], kPmTile);
     }
     for (int i = 0; i < 6; ++i) mbar_init(&odone[i], 1);  // and ofull, mdone
-    mbar_init(qfull, 2 * kPmTile);
+    for (int i = 0; i < 2; ++i) mbar_init(&qfull[i], kPmTile);
     fence_mbarrier_init();
   }
   if (warp == kPmMmaWarp) {
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
   pdl_launch_dependents();
   pdl_wait();
 
   // The longest blocks first, of all requests and heads: with `causal` the last rows see most.
   const int rb = static_cast<int>(gridDim.z - 1 - blockIdx.z);
-  const int split = blockIdx.x % max_splits;
-  const int kvh = blockIdx.x / max_splits;
+  const int kvh = max_splits == 1 ? blockIdx.x : blockIdx.x / max_splits;
+  const int split = blockIdx.x - kvh * max_splits;
   const int b = blockIdx.y;
   int start = 0, n = 0;
-  bool fine = request_rows(a, b, start, n);
   int len = a.lengths[b];
+  bool fine = request_rows(a, b, start, n);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
   fine = fine && len >= 0 && len <= static_cast<int64_t>(a.table_cols) * a.cache.page_size &&
          (len == 0 || a.cache.pages > 0);
   if (!fine) {
@@ -191,7 +192,7 @@ __global__ void __launch_bounds__(kPmThreads, 1)
     const int first = r0 + i * kPmTile;
     steps[i] = 0;
     if (i < tiles_a_cta && first < rows) {
-      const int last = (min(rows, first + kPmTile) - 1) / share;
+      const int last = div_by(min(rows, first + kPmTile) - 1, share, share_inv);
       const int sees = max(0, a.causal ? len - n + last + 1 : len);
       steps[i] = (sees + kPmTile - 1) / kPmTile;
       kmax = max(kmax, sees);
@@ -201,10 +202,11 @@ __global__ void __launch_bounds__(kPmThreads, 1)
   const int all = max(steps[0], steps[1]);
   // CTAs that take part: one for every split_steps steps. The others only say that they saw
   // nothing.
-  const int splits = max(1, min(max_splits, (all + split_steps - 1) / split_steps));
+  const int splits = max_splits == 1 ? 1 : max(1, min(max_splits, (all + split_steps - 1) / split_steps));
   const bool idle = split >= splits;
-  const int j0 = idle ? 0 : static_cast<int>(static_cast<int64_t>(all) * split / splits);
-  const int most = idle ? 0 : static_cast<int>(static_cast<int64_t>(all) * (split + 1) / splits) - j0;
+  // At most 2^23 steps by 64 CTAs.
+  const int j0 = idle || splits == 1 ? 0 : all * split / splits;
+  const int most = idle ? 0 : splits == 1 ? all : all * (split + 1) / splits - j0;
   steps[0] = max(0, min(steps[0] - j0, most));
   steps[1] = max(0, min(steps[1] - j0, most));
 
@@ -214,10 +216,10 @@ __global__ void __launch_bounds__(kPmThreads, 1)
     const int per_page = a.cache.page_size / 16;
     const int32_t* table = a.table + b * a.ld_table;
     const int run0 = (j0 * kPmTile + t) / 16;
-    int col = run0 / per_page, off = run0 - col * per_page;
-    const int dcol = (kPmTile / 16) / per_page, doff = (kPmTile / 16) - dcol * per_page;
+    int col = div_by(run0, per_page, page_inv), off = run0 - col * per_page;
+    const int dcol = div_by(kPmTile / 16, per_page, page_inv), doff = (kPmTile / 16) - dcol * per_page;
     // What every row of the block sees from here on: below it no row is masked.
-    const int first_lim = a.causal ? len - n + r0 / share + 1 : len;
+    const int first_lim = a.causal ? len - n + div_by(r0, share, share_inv) + 1 : len;
     uint4 kc[NG], vc[NG];
     uint32_t kp[NG], vp[NG];
     int64_t row = 0;  // of this thread's token of the step being fetched; -1 beyond the tokens
@@ -251,8 +253,8 @@ __global__ void __launch_bounds__(kPmThreads, 1)
     };
     if (most > 0) {
       find(0);
-      fetch(a.cache.v_codes, a.cache.v_params, vc, vp);
       fetch(a.cache.k_codes, a.cache.k_params, kc, kp);
+      fetch(a.cache.v_codes, a.cache.v_params, vc, vp);
     }
     bool ok = true;
     for (int j = 0; ok && j < most; ++j) {
@@ -335,7 +337,7 @@ __global__ void __launch_bounds__(kPmThreads, 1)
         tc_commit(&sfull[2 * i + (u & 1)]);
       };
       const int mine = steps[i];
-      bool ok = wait(qfull, 0) && wait(&kfull[0], 0);
+      bool ok = wait(&qfull[i], 0) && wait(&kfull[0], 0);
       if (ok && elect_one()) {
         if (mine > 0) {
           scores(0);
@@ -381,44 +383,43 @@ __global__ void __launch_bounds__(kPmThreads, 1)
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t ts = tmem + lanes + kColS + i * kPmTile;
     const uint32_t to = tmem + lanes + kColO + i * D;
+    const int token = div_by(r, share, share_inv), head = kvh * share + r - token * share;
     // What the row sees, from this CTA's first token on.
-    const int lim = r < rows ? (a.causal ? len - n + r / share + 1 : len) - j0 * kPmTile : 0;
+    const int lim = r < rows ? (a.causal ? len - n + token + 1 : len) - j0 * kPmTile : 0;
     // Tokens that all rows of this tile see (they are in order).
-    const int first_lim = (a.causal ? len - n + (r0 + i * kPmTile) / share + 1 : len) - j0 * kPmTile;
+    const int first_lim = (a.causal ? len - n + div_by(r0 + i * kPmTile, share, share_inv) + 1 : len) - j0 * kPmTile;
     const bool whole = r0 + i * kPmTile + kPmTile <= rows;
     const float to_log2 = a.scale * 1.4426950408889634f;
     float m = -INFINITY, l = 0.f;
     bool ok = true;
 
-    // q, channels of a chunk in the order 0 4 1 5 2 6 3 7: kWords lanes a row, eight rows
-    // of loads at a time.
-    if (most > 0) {
-      constexpr int kRowsAPass = 2 * kPmTile / kWords;
-      const int ch = tid % kWords;
-      for (int q0 = tid / kWords; q0 < tiles_a_cta * kPmTile; q0 += 8 * kRowsAPass) {
-        uint4 u[8];
+    // Rows of a warp as it moves them: kWords lanes a row, the rows' offsets from their lanes.
+    constexpr int kRowsAPass = 32 / kWords, kPasses = 32 / kRowsAPass;
+    const int ch = lane % kWords, sub = lane / kWords;
+    const int tile_row = (warp & 3) * 32;  // the warp's first row of the tile
+    // q, channels of a chunk in the order 0 4 1 5 2 6 3 7, all loads of the warp's rows at once:
+    // rows beyond the last read the first and are cleared, since loads under a condition of
+    // their own were waited for one by one (4 prompts of 2048 tokens: 108 us, against 94).
+    if (most > 0 && i < tiles_a_cta) {
+      const int64_t mine = r < rows ? (start + token) * a.q_token_stride + head * a.q_head_stride : -1;
+      uint4 v[kPasses];
+      uint32_t keep = 0;
 #pragma unroll
-        for (int x = 0; x < 8; ++x) {
-          const int rr = r0 + q0 + x * kRowsAPass;
-          u[x] = make_uint4(0u, 0u, 0u, 0u);
-          if (q0 + x * kRowsAPass < tiles_a_cta * kPmTile && rr < rows) {
-            u[x] = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) +
-                                                   static_cast<int64_t>(start + rr / share) * a.q_token_stride +
-                                                   (kvh * share + rr % share) * a.q_head_stride + 8 * ch);
-          }
-        }
+      for (int x = 0; x < kPasses; ++x) {
+        const int64_t from = __shfl_sync(0xffffffffu, mine, x * kRowsAPass + sub);
+        v[x] = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (from >= 0 ? from : 0) + 8 * ch);
+        keep |= from >= 0 ? 1u << x : 0u;
+      }
+      const uint32_t qt = smem_u32(smem + S::kQ) + i * S::kTileBytes;
 #pragma unroll
-        for (int x = 0; x < 8; ++x) {
-          const int row = q0 + x * kRowsAPass;
-          if (row >= tiles_a_cta * kPmTile) break;
-          const uint4 v = u[x];
-          sts128(smem_u32(smem + S::kQ) + (row >> 7) * S::kTileBytes + tile_offset(row & 127, ch),
-                 __byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632), __byte_perm(v.y, v.w, 0x5410),
-                 __byte_perm(v.y, v.w, 0x7632));
-        }
+      for (int x = 0; x < kPasses; ++x) {
+        if (!(keep >> x & 1)) v[x] = make_uint4(0u, 0u, 0u, 0u);
+        sts128(qt + tile_offset(tile_row + x * kRowsAPass + sub, ch), __byte_perm(v[x].x, v[x].z, 0x5410),
+               __byte_perm(v[x].x, v[x].z, 0x7632), __byte_perm(v[x].y, v[x].w, 0x5410),
+               __byte_perm(v[x].y, v[x].w, 0x7632));
       }
       fence_proxy_async_smem();
-      mbar_arrive(qfull);
+      mbar_arrive(&qfull[i]);
     }
     auto step = [&](int u, auto masked) {
       constexpr bool kMasked = decltype(masked)::value;
@@ -428,13 +429,13 @@ __global__ void __launch_bounds__(kPmThreads, 1)
       tmem_ld<32>(tb, s[0]);
       tmem_ld<32>(tb + 32, s[1]);
       tc_wait_ld();
-      float mx = -INFINITY;
+      float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
       for (int k = 0; k < kPmSub; ++k) {
         if (kMasked && k >= left) s[k / 32][k % 32] = 0xFF800000u;  // -inf
-        mx = fmaxf(mx, __uint_as_float(s[k / 32][k % 32]));
+        mx4[k % 4] = fmaxf(mx4[k % 4], __uint_as_float(s[k / 32][k % 32]));
       }
-      mx *= to_log2;  // scale > 0
+      const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * to_log2;  // scale > 0
       if (__any_sync(0xffffffffu, mx > m + 8.f)) {
         const float up = fmaxf(m, mx);
         const float f = up > m ? ex2f(m - up) : 1.f;
@@ -499,10 +500,10 @@ __global__ void __launch_bounds__(kPmThreads, 1)
       const uint32_t qt = smem_u32(smem + S::kQ) + i * S::kTileBytes;
       const int row = tid & 127;
       const bool part = max_splits > 1;
-      const auto part_row = [&](int rr) {
-        return ((static_cast<int64_t>(start) + rr / share) * a.q_heads + kvh * share + rr % share) * max_splits + split;
-      };
-      if (part && r < rows) a.stats[part_row(r)] = make_float2(m, l);
+      // This thread's row of the output, or of the workspace.
+      const int64_t out_row = (static_cast<int64_t>(start) + token) * a.q_heads + head;
+      const int64_t part_row = out_row * max_splits + split;
+      if (part && r < rows) a.stats[part_row] = make_float2(m, l);
 #pragma unroll
       for (int c = 0; c < D / (8 * NG); ++c) {
         uint32_t o[8 * NG];
@@ -531,15 +532,14 @@ __global__ void __launch_bounds__(kPmThreads, 1)
           }
           if (c & 1) {
             __syncwarp();
-            constexpr int kChunks = 4 * NG;
-            const int ch = lane % kChunks;
+            static_assert(kWords == 4 * NG, "sixteen of a group's channels are four chunks");
 #pragma unroll 4
-            for (int x = 0; x < 32; x += 32 / kChunks) {
-              const int wrow = (warp & 3) * 32 + x + lane / kChunks;
-              const int rr = r0 + i * kPmTile + wrow;
-              if (rr < rows) {
-                *reinterpret_cast<uint4*>(a.parts + part_row(rr) * D + 32 * (ch / 4) + 8 * (c - 1) + 4 * (ch % 4)) =
-                    lds128(qt + tile_offset(wrow, ch));
+            for (int x = 0; x < kPasses; ++x) {
+              const int wrow = x * kRowsAPass + sub;
+              const int64_t to_row = __shfl_sync(0xffffffffu, part_row, wrow);
+              if (r0 + i * kPmTile + tile_row + wrow < rows) {
+                *reinterpret_cast<uint4*>(a.parts + to_row * D + 32 * (ch / 4) + 8 * (c - 1) + 4 * (ch % 4)) =
+                    lds128(qt + tile_offset(tile_row + wrow, ch));
               }
             }
             __syncwarp();
@@ -559,16 +559,21 @@ __global__ void __launch_bounds__(kPmThreads, 1)
         }
       }
       __syncwarp();
-      constexpr int kRowsAStore = 32 / kWords;
-#pragma unroll 4
-      for (int x = 0; !part && x < 32; x += kRowsAStore) {
-        const int wrow = (warp & 3) * 32 + x + lane / kWords;
-        const int rr = r0 + i * kPmTile + wrow;
-        if (rr < rows) {
-          *reinterpret_cast<uint4*>(static_cast<T*>(a.out) +
-                                    static_cast<int64_t>(start + rr / share) * a.out_token_stride +
-                                    static_cast<int64_t>(kvh * share + rr % share) * D + 8 * (lane % kWords)) =
-              lds128(qt + tile_offset(wrow, lane % kWords));
+      if (!part) {
+        const int64_t dst = (static_cast<int64_t>(start) + token) * a.out_token_stride + head * D;
+#pragma unroll
+        for (int x0 = 0; x0 < kPasses; x0 += 8) {
+          uint4 v[8];
+#pragma unroll
+          for (int x = 0; x < 8; ++x) v[x] = lds128(qt + tile_offset(tile_row + (x0 + x) * kRowsAPass + sub, ch));
+#pragma unroll
+          for (int x = 0; x < 8; ++x) {
+            const int wrow = (x0 + x) * kRowsAPass + sub;
+            const int64_t to_row = __shfl_sync(0xffffffffu, dst, wrow);
+            if (r0 + i * kPmTile + tile_row + wrow < rows) {
+              *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + to_row + 8 * ch) = v[x];
+            }
+          }
         }
       }
     }
@@ -600,7 +605,9 @@ int launch_pm(const Kv4AttnArgs& a, const PromptPlan& p, bool pdl, cudaStream_t 
     cfg.attrs = attr;
     cfg.numAttrs = 1;
   }
-  return cudaLaunchKernelEx(&cfg, kv4_prompt_kernel<T, D>, a, p.tiles, p.splits, p.split_steps, current_wait_limit_ns()) ==
+  return cudaLaunchKernelEx(&cfg, kv4_prompt_kernel<T, D>, a, p.tiles, p.splits, p.split_steps,
+                            0xffffffffu / static_cast<uint32_t>(a.q_heads / a.cache.kv_heads),
+                            0xffffffffu / static_cast<uint32_t>(a.cache.page_size / 16), current_wait_limit_ns()) ==
                  cudaSuccess
              ? QTTS_OK
              : QTTS_ERR_LAUNCH;
