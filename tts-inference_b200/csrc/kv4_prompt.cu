@@ -421,8 +421,7 @@ __global__ void __launch_bounds__(kPmThreads, 1)
       fence_proxy_async_smem();
       mbar_arrive(&qfull[i]);
     }
-    auto step = [&](int u, auto masked) {
-      constexpr bool kMasked = decltype(masked)::value;
+    auto step = [&](int u, bool masked) {
       const int left = lim - u * kPmSub;  // columns that this row sees
       const uint32_t tb = ts + (u & 1) * kPmSub;
       uint32_t s[2][32];
@@ -430,9 +429,12 @@ __global__ void __launch_bounds__(kPmThreads, 1)
       tmem_ld<32>(tb + 32, s[1]);
       tc_wait_ld();
       float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      if (masked) {
+#pragma unroll
+        for (int k = 0; k < kPmSub; ++k) s[k / 32][k % 32] = k >= left ? 0xFF800000u : s[k / 32][k % 32];  // -inf
+      }
 #pragma unroll
       for (int k = 0; k < kPmSub; ++k) {
-        if (kMasked && k >= left) s[k / 32][k % 32] = 0xFF800000u;  // -inf
         mx4[k % 4] = fmaxf(mx4[k % 4], __uint_as_float(s[k / 32][k % 32]));
       }
       const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * to_log2;  // scale > 0
@@ -445,7 +447,7 @@ __global__ void __launch_bounds__(kPmThreads, 1)
           // S(u) came after O took P(u - 2); it may be taking P(u - 1).
           ok = ok && __all_sync(0xffffffffu, mbar_wait_bounded(&odone[i], (u - 1) & 1, wait_ns));
           tc_fence_after();
-#pragma unroll
+#pragma unroll 1
           for (int c = 0; c < D / 16; ++c) {
             uint32_t o[16];
             tmem_ld<16>(to + 16 * c, o);
@@ -480,11 +482,7 @@ __global__ void __launch_bounds__(kPmThreads, 1)
       ok = __all_sync(0xffffffffu, mbar_wait_bounded(&sfull[2 * i + (u & 1)], (u / 2) & 1, wait_ns));
       if (!ok) break;
       tc_fence_after();
-      if (whole && (u + 1) * kPmSub <= first_lim) {
-        step(u, std::false_type{});
-      } else {
-        step(u, std::true_type{});
-      }
+      step(u, !whole || (u + 1) * kPmSub > first_lim);
     }
     if (ok && steps[i] > 0) {
       ok = __all_sync(0xffffffffu, mbar_wait_bounded(&ofull[i], 0, wait_ns));
@@ -504,7 +502,7 @@ __global__ void __launch_bounds__(kPmThreads, 1)
       const int64_t out_row = (static_cast<int64_t>(start) + token) * a.q_heads + head;
       const int64_t part_row = out_row * max_splits + split;
       if (part && r < rows) a.stats[part_row] = make_float2(m, l);
-#pragma unroll
+#pragma unroll 1
       for (int c = 0; c < D / (8 * NG); ++c) {
         uint32_t o[8 * NG];
         if (steps[i] > 0) {
