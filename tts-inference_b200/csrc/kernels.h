@@ -231,6 +231,8 @@ struct Kv4AttnArgs {
   const int32_t* lengths;   // [batch]
   const int32_t* q_starts;  // [batch + 1], or nullptr: max_q tokens a request
   int total_q, max_q, batch, q_heads;
+  int share, per_page;            // query heads a key head; 16-token runs a page
+  uint32_t share_inv, page_inv;   // their reciprocals for div_by
   float scale;
   int causal;
   void* out;  // [total_q, q_heads, head_dim]

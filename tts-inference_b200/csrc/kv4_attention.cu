@@ -112,7 +112,7 @@ struct RowsSmem {
 
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 3 : 2) kv4_rows_kernel(const Kv4AttnArgs a, int row_blocks,
-                                                                                int warp_tiles) {
+                                                                                int cta_tiles_log2) {
   using S = RowsSmem<D>;
   constexpr int NG = D / kKv4Group;
   constexpr int kRows = 8 * NT;
@@ -127,15 +127,25 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 3 : 2) kv4_rows_kernel(
   const int lane = threadIdx.x & 31;
   const int g = lane >> 2, c = lane & 3;
   const int rank = blockIdx.x;
-  const int rb = blockIdx.y % row_blocks;
-  const int kvh = blockIdx.y / row_blocks;
+  const int kvh = row_blocks == 1 ? blockIdx.y : blockIdx.y / row_blocks;
+  const int rb = blockIdx.y - kvh * row_blocks;
   const int b = blockIdx.z;
   pdl_launch_dependents();
+  // The first tile's place in the table does not depend on the length: both are fetched at once.
+  const int t_first = rank * warps + warp;
+  const int per_page = a.per_page;
+  const int32_t* table = a.table + b * a.ld_table;
+  int at = 2 * t_first;  // number of the tile's first run within the request
+  int col = div_by(at, per_page, a.page_inv), off = at - col * per_page;
+  const bool whole_tiles = per_page % 2 == 0;
   pdl_wait();
+  int page[2];
+  page[0] = col < a.table_cols ? table[col] : 0;
+  page[1] = !whole_tiles && off + 1 == per_page && col + 1 < a.table_cols ? table[col + 1] : page[0];
 
   int start = 0, n = 0;
-  bool fine = request_rows(a, b, start, n);
   int len = a.lengths[b];
+  bool fine = request_rows(a, b, start, n);
   fine = fine && len >= 0 && len <= static_cast<int64_t>(a.table_cols) * a.cache.page_size &&
          (len == 0 || a.cache.pages > 0);
   if (!fine) {
@@ -143,21 +153,23 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 3 : 2) kv4_rows_kernel(
     len = 0;
     if (!request_rows(a, b, start, n)) n = 0;  // rows that cannot be told are not written
   }
-  const int share = a.q_heads / a.cache.kv_heads;
+  const int share = a.share;
   const int rows = n * share;
   const int r0 = rb * kRows;
   // Tokens that any row of this block sees.
-  const int last = (min(rows, r0 + kRows) - 1) / share;  // its last new token
-  const int first_lim = a.causal ? len - n + r0 / share + 1 : len;  // what its first row sees (may be negative)
+  const int last = div_by(max(0, min(rows, r0 + kRows) - 1), share, a.share_inv);  // its last new token
+  const int first_lim = a.causal ? len - n + div_by(r0, share, a.share_inv) + 1 : len;  // what its first row sees (may be negative)
   const int kmax = r0 >= rows ? 0 : max(0, a.causal ? len - n + last + 1 : len);
+  if (at * 16 + 16 >= kmax) page[1] = 0;  // what the table holds beyond the tokens is not a page
   const int tiles = (kmax + kTile - 1) / kTile;
-  // CTAs that take part in this unit: as many as have warp_tiles tiles for each warp. The others
-  // leave (one at least stays, to answer for a unit that sees nothing).
-  const int splits = max(1, min(static_cast<int>(gridDim.x), (tiles + warps * warp_tiles - 1) / (warps * warp_tiles)));
+  // CTAs that take part in this unit: as many as have 2^cta_tiles_log2 tiles. The others leave (one
+  // at least stays, to answer for a unit that sees nothing).
+  const int splits = max(1, min(static_cast<int>(gridDim.x), (tiles + (1 << cta_tiles_log2) - 1) >> cta_tiles_log2));
   if (rank >= splits) {
     if (a.parts != nullptr && threadIdx.x < kRows && r0 + threadIdx.x < rows) {  // says that it saw nothing
       const int rr = r0 + threadIdx.x;
-      const int64_t orow = static_cast<int64_t>(start + rr / share) * a.q_heads + kvh * share + rr % share;
+      const int token = div_by(rr, share, a.share_inv);
+      const int64_t orow = static_cast<int64_t>(start + token) * a.q_heads + kvh * share + rr - token * share;
       a.stats[orow * gridDim.x + rank] = make_float2(-INFINITY, 0.f);
     }
     return;
@@ -168,19 +180,11 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 3 : 2) kv4_rows_kernel(
   // without a division, and the pages of the next tile are fetched one tile ahead.
   uint8_t* ring = smem + warp * S::kWarpRing;
   const int step = splits * warps;
-  const int t_first = rank * warps + warp;
-  const int per_page = a.cache.page_size / 16;
-  const int32_t* table = a.table + b * a.ld_table;
-  const int dcol = 2 * step / per_page, doff = 2 * step - dcol * per_page;
-  int at = 2 * t_first;  // number of the tile's first run within the request
-  int col = at / per_page, off = at - col * per_page;
-  const bool whole_tiles = per_page % 2 == 0;
-  int page[2];
+  const int dcol = div_by(2 * step, per_page, a.page_inv), doff = 2 * step - dcol * per_page;
   auto find_pages = [&]() {
     page[0] = at * 16 < kmax ? table[col] : 0;
     if (!whole_tiles) page[1] = off + 1 < per_page ? page[0] : at * 16 + 16 < kmax ? table[col + 1] : 0;
   };
-  find_pages();
   auto issue = [&](int stage) {
     const uint32_t dst = smem_u32(ring) + stage * S::kStage + 16 * lane;
     if (page[0] < 0 || page[0] >= a.cache.pages) {
@@ -248,15 +252,19 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 3 : 2) kv4_rows_kernel(
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     const int r = r0 + 8 * nt + g;
-    const T* qr = static_cast<const T*>(a.q) + static_cast<int64_t>(start + r / share) * a.q_token_stride +
-                  (kvh * share + r % share) * a.q_head_stride + 8 * c;
+    const int token = div_by(r, share, a.share_inv);
+    const T* qr = static_cast<const T*>(a.q) + static_cast<int64_t>(start + token) * a.q_token_stride +
+                  (kvh * share + r - token * share) * a.q_head_stride + 8 * c;
+    if (r >= rows) qr = static_cast<const T*>(a.q);  // read all the same (not one by one) and cleared
+    uint4 u[NG];
+#pragma unroll
+    for (int j = 0; j < NG; ++j) u[j] = *reinterpret_cast<const uint4*>(qr + 32 * j);
     float x[NG][8];
     float top = 0.f;
 #pragma unroll
     for (int j = 0; j < NG; ++j) {
-      uint4 u = make_uint4(0u, 0u, 0u, 0u);
-      if (r < rows) u = *reinterpret_cast<const uint4*>(qr + 32 * j);
-      const T* e = reinterpret_cast<const T*>(&u);
+      if (r >= rows) u[j] = make_uint4(0u, 0u, 0u, 0u);
+      const T* e = reinterpret_cast<const T*>(&u[j]);
 #pragma unroll
       for (int i = 0; i < 8; ++i) x[j][i] = to_float(e[i]), top = fmaxf(top, fabsf(x[j][i]));
     }
@@ -288,7 +296,7 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 3 : 2) kv4_rows_kernel(
   for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      const int i = (r0 + 8 * nt + 2 * c + e) / share;
+      const int i = div_by(r0 + 8 * nt + 2 * c + e, share, a.share_inv);
       lim[nt][e] = a.causal ? min(len - n + i + 1, kmax) : len;
     }
   }
@@ -609,8 +617,9 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 3 : 2) kv4_rows_kernel(
       lsum += f * stat_l[w][r];
       o.x = fmaf(f, x.x, o.x), o.y = fmaf(f, x.y, o.y), o.z = fmaf(f, x.z, o.z), o.w = fmaf(f, x.w, o.w);
     }
-    const int64_t orow = static_cast<int64_t>(start + rr / share);
-    const int head = kvh * share + rr % share;
+    const int token = div_by(rr, share, a.share_inv);
+    const int64_t orow = static_cast<int64_t>(start + token);
+    const int head = kvh * share + rr - token * share;
     if (mode == 0) {
       const float inv = lsum == 0.f ? 0.f : 1.f / lsum;
       T v[4] = {from_float<T>(o.x * inv), from_float<T>(o.y * inv), from_float<T>(o.z * inv),
@@ -639,11 +648,10 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 3 : 2) kv4_rows_kernel(
       float top = -INFINITY;
 #pragma unroll
       for (int q = 0; q < kMaxCluster; ++q) {
-        if (q < splits) {
-          pm[q] = ld_cluster_f32(mapa_shared(am, q));
-          pl[q] = ld_cluster_f32(mapa_shared(al, q));
-          po[q] = ld_cluster_f32(mapa_shared(ao, q));
-        }
+        const int peer = min(q, splits - 1);  // all at once, no branch between them
+        pm[q] = ld_cluster_f32(mapa_shared(am, peer));
+        pl[q] = ld_cluster_f32(mapa_shared(al, peer));
+        po[q] = ld_cluster_f32(mapa_shared(ao, peer));
       }
 #pragma unroll
       for (int q = 0; q < kMaxCluster; ++q) {
@@ -659,8 +667,9 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 3 : 2) kv4_rows_kernel(
           o = fmaf(f, po[q], o);
         }
       }
-      static_cast<T*>(a.out)[static_cast<int64_t>(start + rr / share) * a.out_token_stride +
-                             static_cast<int64_t>(kvh * share + rr % share) * D + ch] =
+      const int token = div_by(rr, share, a.share_inv);
+      static_cast<T*>(a.out)[static_cast<int64_t>(start + token) * a.out_token_stride +
+                             static_cast<int64_t>(kvh * share + rr - token * share) * D + ch] =
           from_float<T>(lsum == 0.f ? 0.f : o / lsum);
     }
   }
@@ -789,7 +798,7 @@ struct RowsPlan {
   int nt;
   int64_t row_blocks;
   int splits;      // CTAs at most
-  int warp_tiles;  // tiles a warp for which another CTA joins in
+  int cta_tiles_log2;  // tiles for which another CTA joins in: one a warp, or four
 };
 
 // Tiles that a warp of the longest request gets at most, as far as kEvenCtas CTAs (a
@@ -816,7 +825,8 @@ RowsPlan plan_rows(int64_t max_q, int share, int kv_heads, int batch, int64_t mo
   const int64_t even = (tiles + kEvenTiles * kWarps - 1) / (kEvenTiles * kWarps);
   int64_t s = even < kEvenCtas ? even : kEvenCtas;
   if (s * units > 16 * wave) s = 16 * wave / units;
-  p.warp_tiles = s > want ? 4 : 1;
+  static_assert(kWarps == 4, "one tile a warp, or four, as powers of two");
+  p.cta_tiles_log2 = s > want ? 4 : 2;
   if (s < want) s = want;
   if (s > can) s = can;
   p.splits = static_cast<int>(s < 1 ? 1 : s > kMaxSplits ? kMaxSplits : s);
@@ -865,7 +875,7 @@ int launch_rows(Kv4AttnArgs a, const RowsPlan& p, bool pdl, cudaStream_t stream)
   return launch(kv4_rows_kernel<T, D, NT>,
                 dim3(p.splits, static_cast<unsigned>(p.row_blocks * a.cache.kv_heads), a.batch), 32 * kWarps, kSmem,
                 workspace ? 1 : p.splits, pdl, stream, a, static_cast<int>(p.row_blocks),
-                p.warp_tiles);
+                p.cta_tiles_log2);
 }
 
 template <typename T, int D>
@@ -881,7 +891,7 @@ int launch_join(const Kv4AttnArgs& a, int splits, cudaStream_t stream) {
 
 template <typename T, int D>
 int launch_ka(const Kv4AttnArgs& a, int dtype, bool pdl, cudaStream_t stream) {
-  const int share = a.q_heads / a.cache.kv_heads;
+  const int share = a.share;
   const int64_t tokens = static_cast<int64_t>(a.table_cols) * a.cache.page_size;
   if (kv4_takes_prompt(a.max_q, share, a.cache.kv_heads, a.batch, tokens)) {
     const PromptPlan p = plan_prompt(a.max_q, share, a.cache.kv_heads, a.batch, tokens);
@@ -980,6 +990,10 @@ extern "C" int qtts_kv4_attention(const void* q, int64_t q_token_stride, int64_t
   a.max_q = max_q;
   a.batch = batch;
   a.q_heads = q_heads;
+  a.share = q_heads / kv_heads;
+  a.per_page = page_size / 16;
+  a.share_inv = 0xffffffffu / static_cast<uint32_t>(a.share);
+  a.page_inv = 0xffffffffu / static_cast<uint32_t>(a.per_page);
   a.scale = scale;
   a.causal = causal;
   a.out = out;

@@ -114,8 +114,7 @@ __device__ __forceinline__ uint32_t tile_offset(int row, int chunk) {
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kPmThreads, 1)
-    kv4_prompt_kernel(const Kv4AttnArgs a, int tiles_a_cta, int max_splits, int split_steps, uint32_t share_inv,
-                      uint32_t page_inv, uint64_t wait_ns) {
+    kv4_prompt_kernel(const Kv4AttnArgs a, int tiles_a_cta, int max_splits, int split_steps, uint64_t wait_ns) {
   using S = PromptSmem<D>;
   constexpr int NG = D / kKv4Group;
   constexpr int kWords = D / 8;  // 32-bit words of codes a row; chunks of eight channels
@@ -181,7 +180,7 @@ __global__ void __launch_bounds__(kPmThreads, 1)
     len = 0;
     if (!request_rows(a, b, start, n)) n = 0;  // rows that cannot be told are not written
   }
-  const int share = a.q_heads / a.cache.kv_heads;
+  const int share = a.share;
   const int rows = n * share;
   const int r0 = rb * tiles_a_cta * kPmTile;
   // Tiles of rows that exist, and the 128-token steps that each of them needs.
@@ -192,7 +191,7 @@ __global__ void __launch_bounds__(kPmThreads, 1)
     const int first = r0 + i * kPmTile;
     steps[i] = 0;
     if (i < tiles_a_cta && first < rows) {
-      const int last = div_by(min(rows, first + kPmTile) - 1, share, share_inv);
+      const int last = div_by(min(rows, first + kPmTile) - 1, share, a.share_inv);
       const int sees = max(0, a.causal ? len - n + last + 1 : len);
       steps[i] = (sees + kPmTile - 1) / kPmTile;
       kmax = max(kmax, sees);
@@ -213,13 +212,13 @@ __global__ void __launch_bounds__(kPmThreads, 1)
   if (warp >= kPmDqWarp && warp < kPmMmaWarp) {
     // ---------------- operands: one token a thread ----------------
     const int t = tid - kPmDqWarp * 32;
-    const int per_page = a.cache.page_size / 16;
+    const int per_page = a.per_page;
     const int32_t* table = a.table + b * a.ld_table;
     const int run0 = (j0 * kPmTile + t) / 16;
-    int col = div_by(run0, per_page, page_inv), off = run0 - col * per_page;
-    const int dcol = div_by(kPmTile / 16, per_page, page_inv), doff = (kPmTile / 16) - dcol * per_page;
+    int col = div_by(run0, per_page, a.page_inv), off = run0 - col * per_page;
+    const int dcol = div_by(kPmTile / 16, per_page, a.page_inv), doff = (kPmTile / 16) - dcol * per_page;
     // What every row of the block sees from here on: below it no row is masked.
-    const int first_lim = a.causal ? len - n + div_by(r0, share, share_inv) + 1 : len;
+    const int first_lim = a.causal ? len - n + div_by(r0, share, a.share_inv) + 1 : len;
     uint4 kc[NG], vc[NG];
     uint32_t kp[NG], vp[NG];
     int64_t row = 0;  // of this thread's token of the step being fetched; -1 beyond the tokens
@@ -383,11 +382,11 @@ __global__ void __launch_bounds__(kPmThreads, 1)
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t ts = tmem + lanes + kColS + i * kPmTile;
     const uint32_t to = tmem + lanes + kColO + i * D;
-    const int token = div_by(r, share, share_inv), head = kvh * share + r - token * share;
+    const int token = div_by(r, share, a.share_inv), head = kvh * share + r - token * share;
     // What the row sees, from this CTA's first token on.
     const int lim = r < rows ? (a.causal ? len - n + token + 1 : len) - j0 * kPmTile : 0;
     // Tokens that all rows of this tile see (they are in order).
-    const int first_lim = (a.causal ? len - n + div_by(r0 + i * kPmTile, share, share_inv) + 1 : len) - j0 * kPmTile;
+    const int first_lim = (a.causal ? len - n + div_by(r0 + i * kPmTile, share, a.share_inv) + 1 : len) - j0 * kPmTile;
     const bool whole = r0 + i * kPmTile + kPmTile <= rows;
     const float to_log2 = a.scale * 1.4426950408889634f;
     float m = -INFINITY, l = 0.f;
@@ -603,9 +602,7 @@ int launch_pm(const Kv4AttnArgs& a, const PromptPlan& p, bool pdl, cudaStream_t 
     cfg.attrs = attr;
     cfg.numAttrs = 1;
   }
-  return cudaLaunchKernelEx(&cfg, kv4_prompt_kernel<T, D>, a, p.tiles, p.splits, p.split_steps,
-                            0xffffffffu / static_cast<uint32_t>(a.q_heads / a.cache.kv_heads),
-                            0xffffffffu / static_cast<uint32_t>(a.cache.page_size / 16), current_wait_limit_ns()) ==
+  return cudaLaunchKernelEx(&cfg, kv4_prompt_kernel<T, D>, a, p.tiles, p.splits, p.split_steps, current_wait_limit_ns()) ==
                  cudaSuccess
              ? QTTS_OK
              : QTTS_ERR_LAUNCH;
