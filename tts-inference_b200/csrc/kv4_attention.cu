@@ -238,7 +238,7 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 3 : 2) kv4_rows_kernel(
     find_pages();
   };
   // One group a tile, empty ones too, so that waiting counts tiles.
-#pragma unroll
+#pragma unroll 1
   for (int s = 0; s < kStages; ++s) {
     if (t_first + s * step < tiles) issue(s);
     copy_commit();
