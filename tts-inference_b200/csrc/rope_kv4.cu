@@ -20,7 +20,7 @@
 // so a warp takes several heads of one token and gathers its cosines and sines
 // once; how many is chosen so that a short call still has a warp for every head
 // pair and a long one few gathers. 28 such warps an SM,
-// each with its next row under way, beat fewer with more (8192 tokens: 42 us; 20
+// each with its next row under way, beat fewer with more (8192 tokens: 41 us; 20
 // warps and four rows ahead 48).
 #include <type_traits>
 
@@ -83,7 +83,8 @@ __device__ __forceinline__ uint4 pack8(const float (&y)[8]) {
 }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(32, 28) rope_kv4_kernel(const RopeKv4Args a, int passes, int warps_a_token) {
+__global__ void __launch_bounds__(32, 28) rope_kv4_kernel(const RopeKv4Args a, int passes, int warps_a_token,
+                                                           uint32_t token_inv, uint32_t page_inv) {
   constexpr int kLanes = D / 8;          // lanes a head row
   constexpr int kHeads = 32 / kLanes;    // head rows a pass of a warp
   constexpr int kGroups = D / kKv4Group;
@@ -91,23 +92,27 @@ __global__ void __launch_bounds__(32, 28) rope_kv4_kernel(const RopeKv4Args a, i
   pdl_wait();
   // One warp a CTA: token, passes and kinds are the CTA's, so every branch is uniform.
   const int lane = threadIdx.x;
-  const int64_t t = blockIdx.x / warps_a_token;
+  const int token = div_by(blockIdx.x, warps_a_token, token_inv);
+  const int64_t t = token;
   const int l = lane % kLanes;
   const int sub = lane / kLanes;  // which of the pass's heads
   const int kvh = a.cache.kv_heads;
   // A pass takes kHeads heads of one kind: the q passes first, then k, then v.
   const int nq = (a.q_heads + kHeads - 1) / kHeads, nk = (kvh + kHeads - 1) / kHeads;
-  const int p_first = static_cast<int>(blockIdx.x % warps_a_token) * passes;
+  const int p_first = (static_cast<int>(blockIdx.x) - token * warps_a_token) * passes;
   const int p_end = min(p_first + passes, nq + 2 * nk);
   const T* src = static_cast<const T*>(a.qkv) + t * a.ldqkv + 8 * l;
 
   // A token with a position outside the tables gives zeros and is not stored.
   bool ok = true;
+  const int64_t slot = a.slots[t];
   int64_t pos[kMaxRopeAxes] = {};
   if (a.cos != nullptr) {
+    // Axes that are not there read the last one: all loads at once, none under a condition.
+#pragma unroll
+    for (int x = 0; x < kMaxRopeAxes; ++x) pos[x] = a.positions[min(x, a.axes - 1) * a.ldpos + t];
 #pragma unroll
     for (int x = 0; x < kMaxRopeAxes; ++x) {
-      pos[x] = x < a.axes ? a.positions[x * a.ldpos + t] : 0;
       if (pos[x] < 0 || pos[x] >= a.table_len) {
         pos[x] = 0;
         ok = false;
@@ -115,11 +120,12 @@ __global__ void __launch_bounds__(32, 28) rope_kv4_kernel(const RopeKv4Args a, i
     }
     if (!ok && lane == 0) record_status(QTTS_ERR_SHAPE);
   }
-  const int64_t slot = a.slots[t];
   const bool inside = slot < a.cache.pages * a.cache.page_size;
   if (!inside && lane == 0) record_status(QTTS_ERR_SHAPE);
   const bool stored = ok && inside && slot >= 0;
-  const int64_t page = stored ? slot / a.cache.page_size : 0;
+  const int64_t page = !stored ? 0
+                       : slot <= 0x7fffffff ? div_by(static_cast<int>(slot), a.cache.page_size, page_inv)
+                                            : slot / a.cache.page_size;
   const int in_page = stored ? static_cast<int>(slot - page * a.cache.page_size) : 0;
 
   // A head row through norm and rotation is y_i = inv * (x_i A_i + x_partner B_i), A and B the
@@ -291,8 +297,11 @@ int launch_rk(const RopeKv4Args& a, bool pdl, cudaStream_t stream) {
     cfg.attrs = attr;
     cfg.numAttrs = 1;
   }
-  return cudaLaunchKernelEx(&cfg, rope_kv4_kernel<T, D>, a, passes, warps_a_token) == cudaSuccess ? QTTS_OK
-                                                                                                 : QTTS_ERR_LAUNCH;
+  return cudaLaunchKernelEx(&cfg, rope_kv4_kernel<T, D>, a, passes, warps_a_token,
+                            0xffffffffu / static_cast<uint32_t>(warps_a_token),
+                            0xffffffffu / static_cast<uint32_t>(a.cache.page_size)) == cudaSuccess
+             ? QTTS_OK
+             : QTTS_ERR_LAUNCH;
 }
 
 }  // namespace
