@@ -30,6 +30,10 @@
 //     CTAs splits one of them and meets in distributed shared memory, or, where
 //     that is not enough to fill the machine, any number of CTAs through a
 //     workspace that a second kernel joins. Sums are in a fixed order.
+// 2 requests over 131071 tokens, 32 + 2 x 8 heads of 128 channels: 336 MB of cache in
+// 75.6 us, 4.4 TB/s, issue slots 63 % busy: the nibbles' instructions and the waits
+// between them bound it, the copies are ahead. 8 requests over 513 tokens: 7.1 us, a
+// launch and the chain lengths -> page -> codes -> scores -> meeting of the CTAs.
 #include <type_traits>
 
 #include "kernels.h"
@@ -110,9 +114,9 @@ struct RowsSmem {
   static constexpr int kPitch = D + 4;  // floats a partial output row: lanes of one store hit different banks
 };
 
-template <typename T, int D, int NT>
-__global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 3 : 2) kv4_rows_kernel(const Kv4AttnArgs a, int row_blocks,
-                                                                                int cta_tiles_log2) {
+template <typename T, int D, int NT, int kCtas>
+__global__ void __launch_bounds__(32 * kWarps, kCtas) kv4_rows_kernel(const Kv4AttnArgs a, int row_blocks,
+                                                                      int cta_tiles_log2) {
   using S = RowsSmem<D>;
   constexpr int NG = D / kKv4Group;
   constexpr int kRows = 8 * NT;
@@ -779,13 +783,13 @@ __global__ void __launch_bounds__(32 * kJoinWarps) kv4_join_kernel(const Kv4Attn
 // of the two in microseconds, 16 query and 8 key heads of 128 channels, from a request's
 // rows (new tokens x 2):
 //                                      32 rows        64 rows        128 rows
-//   1 request,   1000 tokens        9.9 |  19.5    10.4 |  19.8    12.9 |  19.4
-//   8 requests,  1000 tokens       18.8 |  21.6    19.9 |  21.7    37.6 |  22.1
-//   8 requests,  8192 tokens       72.4 | 117.6   141.8 | 118.7   270.2 | 113.7
-//   64 requests, 2048 tokens      120.4 | 169.3   222.8 | 169.8   435.4 | 152.8
+//   1 request,   1000 tokens        9.1 |  16.5    10.2 |  16.4    13.1 |  15.8
+//   8 requests,  1000 tokens       17.5 |  18.0    19.9 |  18.2    37.6 |  18.9
+//   8 requests,  8192 tokens       73.6 |  98.4   144.1 |  99.9   278.8 | 100.1
+//   64 requests, 2048 tokens      128.9 | 142.0   224.9 | 142.5   441.5 | 140.1
 // So few rows stay here whatever the length, more than one tile's go there, and between
-// them the blocks are the faster while their work (blocks x tokens) fits about one wave.
-constexpr int64_t kPromptRows = 64, kTileRows = 128, kWaveTokens = 1 << 18;
+// them the blocks are the faster while their work (blocks x tokens) is well below one wave's.
+constexpr int64_t kPromptRows = 64, kTileRows = 128, kWaveTokens = 1 << 17;
 bool kv4_takes_prompt(int64_t max_q, int share, int kv_heads, int batch, int64_t tokens) {
   const int64_t rows = max_q * share;
   if (rows < kPromptRows || rows > kTileRows) return rows > kTileRows;
@@ -796,6 +800,7 @@ bool kv4_takes_prompt(int64_t max_q, int share, int kv_heads, int batch, int64_t
 // head, row block).
 struct RowsPlan {
   int nt;
+  int ctas;  // an SM
   int64_t row_blocks;
   int splits;      // CTAs at most
   int cta_tiles_log2;  // tiles for which another CTA joins in: one a warp, or four
@@ -803,22 +808,27 @@ struct RowsPlan {
 
 // Tiles that a warp of the longest request gets at most, as far as kEvenCtas CTAs (a
 // cluster) do it: a long request then holds the others of the call up less. With no
-// limit | 8 tiles | 16 tiles: 64 requests of 17 to 8192 tokens 105 | 65 | 59 us; 64 of 4096
-// tokens 87 | 96 | 82 us; 128 of 1000 to 2000 tokens 71 | 84 | 71 us.
+// limit | 8 tiles | 16 tiles, at three CTAs an SM: 64 requests of 17 to 8192 tokens 104 | 61 | 56 us; 64 of 4096
+// tokens 87 | 93 | 79 us; 128 of 1000 to 2000 tokens 66 | 80 | 66 us.
 constexpr int kEvenTiles = 16, kEvenCtas = 8;
 
 RowsPlan plan_rows(int64_t max_q, int share, int kv_heads, int batch, int64_t most_tokens) {
   RowsPlan p;
   const int64_t rows = max_q * share;
   // Eight rows fill an operand; more share what is made of the cache by pairs of eight
-  // (64 x 2048 tokens: 8 rows 51 us, 16 rows 67).
+  // (64 x 2048 tokens: 8 rows 50 us, 16 rows 67).
   p.nt = rows <= 8 ? 1 : 2;
   p.row_blocks = (rows + 8 * p.nt - 1) / (8 * p.nt);
   const int64_t units = p.row_blocks * kv_heads * batch;
-  // One wave of CTAs (three of 128 threads an SM at 168 registers: 77 us for 4 x 65536
-  // tokens, against 83 with four at 128 registers; two with 16 rows), at least one tile a
-  // warp, and the limit above. CTAs that a shorter request has no use for leave at once.
-  const int64_t wave = static_cast<int64_t>(kNumSMs) * (p.nt == 1 ? 3 : 2);
+  // CTAs an SM: two with 16 rows. With 8, three at 168 registers where units are split anyway, the
+  // quicker code (8 x 513 tokens 7.1 us, four at 128 registers 8.3; 8 x 2048: 10.9, 12.3), four
+  // where there is a unit for every SM, more of which then fit at once (32 x 2048: 27.6 us, three
+  // 32.9; 64 x 2000..4000 of 64 channels 25.8, 32.7; 64 x 4096
+  // 77.9, 79.4; but 64 x 17..8192 57.2, 56.3).
+  p.ctas = p.nt == 2 ? 2 : units > kNumSMs ? 4 : 3;
+  // One wave of them, at least one tile a warp, and the limit above. CTAs that a shorter request
+  // has no use for leave at once.
+  const int64_t wave = static_cast<int64_t>(kNumSMs) * p.ctas;
   const int64_t tiles = (most_tokens + kTile - 1) / kTile;
   const int64_t want = wave / (units > 0 ? units : 1);
   const int64_t can = (tiles + kWarps - 1) / kWarps;
@@ -859,20 +869,20 @@ int launch(KernT kern, dim3 grid, int threads, size_t smem, int cluster, bool pd
   return cudaLaunchKernelEx(&cfg, kern, args...) == cudaSuccess ? QTTS_OK : QTTS_ERR_LAUNCH;
 }
 
-template <typename T, int D, int NT>
+template <typename T, int D, int NT, int kCtas>
 int launch_rows(Kv4AttnArgs a, const RowsPlan& p, bool pdl, cudaStream_t stream) {
   using S = RowsSmem<D>;
   constexpr size_t kRing = static_cast<size_t>(kWarps) * S::kWarpRing;
   constexpr size_t kPart = static_cast<size_t>(kWarps) * 8 * NT * S::kPitch * 4;
   constexpr size_t kSmem = kRing > kPart ? kRing : kPart;
-  if (kSmem > 48 * 1024 && cudaFuncSetAttribute(kv4_rows_kernel<T, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                static_cast<int>(kSmem)) != cudaSuccess) {
+  if (kSmem > 48 * 1024 && cudaFuncSetAttribute(kv4_rows_kernel<T, D, NT, kCtas>,
+                                                cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmem)) != cudaSuccess) {
     (void)cudaGetLastError();
     return QTTS_ERR_LAUNCH;
   }
   const bool workspace = p.splits > kMaxCluster;
   if (!workspace) a.parts = nullptr, a.stats = nullptr;
-  return launch(kv4_rows_kernel<T, D, NT>,
+  return launch(kv4_rows_kernel<T, D, NT, kCtas>,
                 dim3(p.splits, static_cast<unsigned>(p.row_blocks * a.cache.kv_heads), a.batch), 32 * kWarps, kSmem,
                 workspace ? 1 : p.splits, pdl, stream, a, static_cast<int>(p.row_blocks),
                 p.cta_tiles_log2);
@@ -900,7 +910,9 @@ int launch_ka(const Kv4AttnArgs& a, int dtype, bool pdl, cudaStream_t stream) {
   }
   const RowsPlan p = plan_rows(a.max_q, share, a.cache.kv_heads, a.batch, tokens);
   if (p.row_blocks * a.cache.kv_heads > 65535) return QTTS_ERR_SHAPE;
-  const int r = p.nt == 1 ? launch_rows<T, D, 1>(a, p, pdl, stream) : launch_rows<T, D, 2>(a, p, pdl, stream);
+  const int r = p.ctas == 4   ? launch_rows<T, D, 1, 4>(a, p, pdl, stream)
+                : p.ctas == 3 ? launch_rows<T, D, 1, 3>(a, p, pdl, stream)
+                              : launch_rows<T, D, 2, 2>(a, p, pdl, stream);
   return r != QTTS_OK || p.splits <= kMaxCluster ? r : launch_join<T, D>(a, p.splits, stream);
 }
 

@@ -4,23 +4,31 @@
 //
 // A CTA takes one or two tiles of rows of one (request, key head) and walks over
 // the tokens, 128 at a time:
-//   * warps 8-11 turn the tile's codes into the activations' type in shared memory,
-//     one token a thread, a key or value rounded once. Keys and values
-//     have the same layout there, 128-byte rows of 64 channels a token,
-//     swizzled: the keys are the K-major B operand of S = Q K^T, the values the
-//     transposed (N-contiguous) B operand of O += P V. The order of channels
-//     within a row is the order in which masks give pairs; q is stored to match, and
-//     the outputs are put back in order at the end;
-//   * warps 12 and 13 issue the products of a tile each, 64 tokens of S at a time into one of two buffers
-//     a tile, so that S(u + 1) is made while the probabilities of S(u) are. P
-//     replaces S in tensor memory. The products of one tile run in the order
-//     issued, so S(u + 2) may overwrite P(u);
-//   * warps 0-3 and 4-7 (a thread a row, no exchange between threads) take the
-//     running maximum and sum in fp32 and write P in the operands' type. The reference maximum
-//     follows only when the maximum has grown by more than 2^8, so O is rescaled
-//     rarely (and then waits for the product before); the row's sum divides at the end.
-// Bound by the two products (2 x 512 cycles a tile of 128 x 128 x 128) and, as
-// much, by 16384 exponentials a tile at 16 a cycle.
+//   * warps 8-11 turn the tile's codes into the activations' type in shared memory, one
+//     token a thread, a key or value rounded once. Keys and values have the same
+//     layout there, 128-byte rows of 64 channels a token, swizzled: the keys are the
+//     K-major B operand of S = Q K^T, the values the transposed (N-contiguous) B
+//     operand of O += P V. The order of channels within a row is the order in which
+//     masks give pairs; q is stored to match, and the outputs are put back in order
+//     at the end;
+//   * warps 12 and 13 issue the products of a tile each, 64 tokens of S at a time into
+//     one of two buffers a tile, so that S(u + 1) is made while the probabilities of
+//     S(u) are. P replaces S in tensor memory. The products of one tile run in the
+//     order issued, so S(u + 2) may overwrite P(u);
+//   * warps 0-3 and 4-7 (a thread a row, no exchange between threads) take the running
+//     maximum and sum in fp32 and write P in the operands' type, rounded to nearest
+//     (the sum takes it unrounded). The reference maximum follows only when the
+//     maximum has grown by more than 2^8, so O is rescaled rarely (and then waits for
+//     the product before); the row's sum divides at the end;
+//   * where there are few (request, key head, block) units, up to 64 CTAs share the
+//     tokens of one and leave fp32 parts in a workspace, which kv4_join_kernel joins.
+// Floor: the two products. 4 prompts of 2048 tokens, 16 + 2 x 8 heads of 128 channels,
+// causal: 90 us, 0.76 PFLOP/s. What bounds it is latency: some 3900 clocks for 128
+// tokens of two tiles, where the tensor cores need 2600 and the exponentials 2050, as
+// the chain S -> maximum -> exponentials -> P -> products has only the other tile to
+// hide behind (two tiles fill the tensor memory), and 12000 clocks a CTA before its
+// first S and after its last P, for cold code and first loads. Rolled loops where they
+// are rare and one body for masked and whole steps took 4 us off by fetching less.
 #include <type_traits>
 
 #include "kernels.h"
@@ -613,13 +621,16 @@ int launch_pm(const Kv4AttnArgs& a, const PromptPlan& p, bool pdl, cudaStream_t 
 PromptPlan plan_prompt(int64_t max_q, int share, int kv_heads, int batch, int64_t most_tokens) {
   PromptPlan p;
   const int64_t rows = max_q * share;
-  // Two tiles a CTA share the operands and hide each other's softmax.
+  // Two tiles a CTA share the operands and hide each other's softmax (4 prompts of 2048 tokens,
+  // 16 + 2 x 8 heads of 128 channels: 90 us, one tile a CTA 133).
   p.tiles = rows > kPmTile ? 2 : 1;
   p.blocks = (rows + p.tiles * kPmTile - 1) / (p.tiles * kPmTile);
   const int64_t units = p.blocks * kv_heads * batch;
   const int64_t steps = (most_tokens + kPmTile - 1) / kPmTile;
   // Enough CTAs for three a SM, so that long ones among short ones do not hold the call up, but
-  // at least four steps each of the longest request (a shorter one takes fewer CTAs).
+  // at least four steps each of the longest request (a shorter one takes fewer CTAs). 193 new
+  // tokens over 1500 to 5001 earlier ones, three requests of 32 + 2 x 4 heads of 64 channels: 47 us,
+  // one CTA an SM 52, at least eight steps 48, two steps 47.
   const int64_t want = units >= 2 * kNumSMs ? 1 : (3 * kNumSMs + units - 1) / (units > 0 ? units : 1);
   const int64_t can = steps / 4;
   const int64_t s = want < can ? want : can;
