@@ -152,6 +152,17 @@ def test_prompt_edges(q_len, length):
     check_attention([length], [q_len], 4, 2, 128, 64, "bf16", seed=q_len)
 
 
+@pytest.mark.parametrize("page,length", [(48, 912), (16, 890), (64, 1000), (64, 900)])
+def test_prompts_over_tables_about_as_long_as_a_split(page, length):
+    check_attention([length], [300], 4, 2, 128, page, "bf16", seed=length)
+
+
+@pytest.mark.parametrize("rows", [63, 64, 65, 127, 128, 129])
+@pytest.mark.parametrize("batch,length", [(1, 200), (3, 1500), (9, 1100)])
+def test_rows_about_the_choice_of_kernel(rows, batch, length):
+    check_attention([length - 5 * b for b in range(batch)], [rows] * batch, 4, 4, 64, 16, "fp16", seed=rows)
+
+
 def test_ragged_chunks_with_empty_requests():
     check_attention([70, 0, 300, 9], [70, 0, 129, 1], 16, 8, 128, 16, "bf16", ragged=True)
 

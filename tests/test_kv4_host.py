@@ -196,3 +196,15 @@ def test_fast_calls_convert_as_ctypes_does(lib):
         fast.qtts_rope_kv4_append(*write_args[:16], (1, 2, 3, 4, 5), *write_args[17:])
     with pytest.raises(TypeError):
         fast.bind(1, 2)
+
+
+def test_no_workspace_below_the_split():
+    # The Python entry does not ask for a workspace below this many tokens, so none may be needed.
+    for heads, kv_heads in [(1, 1), (16, 8), (32, 4), (5, 1)]:
+        for max_q in (1, 3, 20, 64, 300, 2000):
+            for batch in (1, 2, 9, 64):
+                for d in (64, 128):
+                    args = (batch * max_q, max_q, batch, heads, kv_heads, d)
+                    for tokens in (16, 500, kv4._SPLIT_FROM - 1):
+                        assert nat.lib().qtts_kv4_attention_workspace(*args, tokens) == 0
+    assert nat.lib().qtts_kv4_attention_workspace(300, 300, 1, 4, 2, 128, kv4._SPLIT_FROM) > 0

@@ -30,7 +30,7 @@ HEAD_DIMS = (64, 128)
 _HALVES = (32, 64)
 _DTYPES = {torch.bfloat16: nat.BF16, torch.float16: nat.FP16}
 _SCALES = {d: 1.0 / math.sqrt(d) for d in HEAD_DIMS}
-_SPLIT_FROM = 1024  # tokens
+_SPLIT_FROM = 897  # tokens: eight steps of 128, which two CTAs may share
 
 
 class Kv4Cache:
