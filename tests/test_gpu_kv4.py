@@ -163,6 +163,28 @@ def test_rows_about_the_choice_of_kernel(rows, batch, length):
     check_attention([length - 5 * b for b in range(batch)], [rows] * batch, 4, 4, 64, 16, "fp16", seed=rows)
 
 
+@pytest.mark.parametrize("k_lift,v_lift", [(0, 0), (60, -40), (-30, 90)])
+@pytest.mark.parametrize("q_len", [1, 300])
+def test_bf16_beyond_the_range_of_fp16(q_len, k_lift, v_lift):
+    # Keys and values far outside fp16's range, values that differ by 2^24 from page to page and a page
+    # of zeros, against the formula with the bound of check_attention.
+    g = torch.Generator().manual_seed(9)
+    cache = filled_cache(40, 2, 16, 128, g)
+    by_page = 2.0 ** torch.randint(-12, 13, (40, 1, 1, 1, 1), generator=g).cuda()
+    by_page[7] = 0.0
+    cache.k_params.copy_(cache.k_params.float() * 2.0**k_lift)
+    cache.v_params.copy_(cache.v_params.float() * by_page * 2.0**v_lift)
+    q = torch.randn(q_len, 4, 128, generator=g).to(torch.bfloat16).cuda()
+    table = torch.arange(40, dtype=torch.int32).cuda()[None]
+    n, sc = 633, 128**-0.5 * 2.0**-k_lift
+    out = kv4.kv4_attention(q, cache, table, torch.tensor([n], dtype=torch.int32).cuda(), scale=sc).double()
+    k, v = request_rows(cache, table[0], n)
+    sees = n - q_len + torch.arange(q_len, device="cuda") + 1
+    want, mag, most = ref.attention(q.double(), k, v, sees, sc)
+    bound = (2 * 2.0**-8 + 4 * 2.0**-8 * sc * most[..., None] + 1e-4) * mag + UNIT["bf16"] * want.abs()
+    assert ((out - want).abs() <= bound).all()
+
+
 def test_ragged_chunks_with_empty_requests():
     check_attention([70, 0, 300, 9], [70, 0, 129, 1], 16, 8, 128, 16, "bf16", ragged=True)
 

@@ -162,7 +162,8 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas) kv4_rows_kernel(const Kv4A
   const int r0 = rb * kRows;
   // Tokens that any row of this block sees.
   const int last = div_by(max(0, min(rows, r0 + kRows) - 1), share, a.share_inv);  // its last new token
-  const int first_lim = a.causal ? len - n + div_by(r0, share, a.share_inv) + 1 : len;  // what its first row sees (may be negative)
+  // What its first row sees (may be negative).
+  const int first_lim = a.causal ? len - n + div_by(r0, share, a.share_inv) + 1 : len;
   const int kmax = r0 >= rows ? 0 : max(0, a.causal ? len - n + last + 1 : len);
   if (at * 16 + 16 >= kmax) page[1] = 0;  // what the table holds beyond the tokens is not a page
   const int tiles = (kmax + kTile - 1) / kTile;
@@ -783,10 +784,10 @@ __global__ void __launch_bounds__(32 * kJoinWarps) kv4_join_kernel(const Kv4Attn
 // of the two in microseconds, 16 query and 8 key heads of 128 channels, from a request's
 // rows (new tokens x 2):
 //                                      32 rows        64 rows        128 rows
-//   1 request,   1000 tokens        9.1 |  16.5    10.2 |  16.4    13.1 |  15.8
-//   8 requests,  1000 tokens       17.5 |  18.0    19.9 |  18.2    37.6 |  18.9
-//   8 requests,  8192 tokens       73.6 |  98.4   144.1 |  99.9   278.8 | 100.1
-//   64 requests, 2048 tokens      128.9 | 142.0   224.9 | 142.5   441.5 | 140.1
+//   1 request,   1000 tokens        9.1 |  18.5    10.2 |  18.4    13.1 |  17.5
+//   8 requests,  1000 tokens       17.5 |  19.6    19.9 |  19.9    37.6 |  20.5
+//   8 requests,  8192 tokens       73.6 | 110.3   144.1 | 112.5   278.8 | 111.6
+//   64 requests, 2048 tokens      128.9 | 163.7   224.9 | 164.0   441.5 | 160.5
 // So few rows stay here whatever the length, more than one tile's go there, and between
 // them the blocks are the faster while their work (blocks x tokens) is well below one wave's.
 constexpr int64_t kPromptRows = 64, kTileRows = 128, kWaveTokens = 1 << 17;
@@ -875,8 +876,9 @@ int launch_rows(Kv4AttnArgs a, const RowsPlan& p, bool pdl, cudaStream_t stream)
   constexpr size_t kRing = static_cast<size_t>(kWarps) * S::kWarpRing;
   constexpr size_t kPart = static_cast<size_t>(kWarps) * 8 * NT * S::kPitch * 4;
   constexpr size_t kSmem = kRing > kPart ? kRing : kPart;
-  if (kSmem > 48 * 1024 && cudaFuncSetAttribute(kv4_rows_kernel<T, D, NT, kCtas>,
-                                                cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmem)) != cudaSuccess) {
+  if (kSmem > 48 * 1024 &&
+      cudaFuncSetAttribute(kv4_rows_kernel<T, D, NT, kCtas>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           static_cast<int>(kSmem)) != cudaSuccess) {
     (void)cudaGetLastError();
     return QTTS_ERR_LAUNCH;
   }

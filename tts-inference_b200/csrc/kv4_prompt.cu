@@ -4,8 +4,8 @@
 //
 // A CTA takes one or two tiles of rows of one (request, key head) and walks over
 // the tokens, 128 at a time:
-//   * warps 8-11 turn the tile's codes into the activations' type in shared memory, one
-//     token a thread, a key or value rounded once. Keys and values have the same
+//   * warps 8-11 turn the tile's codes into fp16 in shared memory, one token a thread, a
+//     key or value rounded once (bf16 activations: in units of their own, below). Keys and values have the same
 //     layout there, 128-byte rows of 64 channels a token, swizzled: the keys are the
 //     K-major B operand of S = Q K^T, the values the transposed (N-contiguous) B
 //     operand of O += P V. The order of channels within a row is the order in which
@@ -16,14 +16,15 @@
 //     S(u) are. P replaces S in tensor memory. The products of one tile run in the
 //     order issued, so S(u + 2) may overwrite P(u);
 //   * warps 0-3 and 4-7 (a thread a row, no exchange between threads) take the running
-//     maximum and sum in fp32 and write P in the operands' type, rounded to nearest
+//     maximum and sum in fp32 and write P in fp16, rounded to nearest
 //     (the sum takes it unrounded). The reference maximum follows only when the
 //     maximum has grown by more than 2^8, so O is rescaled rarely (and then waits for
 //     the product before); the row's sum divides at the end;
 //   * where there are few (request, key head, block) units, up to 64 CTAs share the
 //     tokens of one and leave fp32 parts in a workspace, which kv4_join_kernel joins.
 // Floor: the two products. 4 prompts of 2048 tokens, 16 + 2 x 8 heads of 128 channels,
-// causal: 90 us, 0.76 PFLOP/s. What bounds it is latency: some 3900 clocks for 128
+// causal: 103 us, 0.67 PFLOP/s (fp16 operands in units: 13 us more than bf16 operands
+// took, for half the error). What bounds it is latency: some 4000 clocks for 128
 // tokens of two tiles, where the tensor cores need 2600 and the exponentials 2050, as
 // the chain S -> maximum -> exponentials -> P -> products has only the other tile to
 // hide behind (two tiles fill the tensor memory), and 12000 clocks a CTA before its
@@ -52,17 +53,13 @@ struct PromptSmem {
   static constexpr int kK = 2 * kTileBytes;
   static constexpr int kV = kK + kPmStages * kTileBytes;
   static constexpr int kBars = kV + kPmStages * kTileBytes;
-  static constexpr int kBytes = kBars + 256 + 1024;  // barriers; slack to align the base to 1024
+  static constexpr int kUnits = kBars + 256;             // [step % 4]: of the keys, of the values, four each
+  static constexpr int kBytes = kUnits + 128 + 1024;     // slack to align the base to 1024
 };
 
 __device__ __forceinline__ float ex2f(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
-__device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
-  uint32_t r;
-  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
 __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
@@ -71,50 +68,33 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
   return r;
 }
 
-// The operands' type is the activations': q as it came, keys, values and probabilities rounded once
-// to it, sums in fp32. Against 64 bits (2-norm): bf16 3.2e-3, of which the output's own rounding is
-// 1.7e-3; fp16 4e-4 and 2e-4. fp16 operands for bf16 activations would need a unit for every
-// tile's keys and values, as their range is wider. bf16: a group's scale and minimum as they are held.
-// fp16: both brought to fp16, where they fit because the keys and values were fp16 (the
-// largest finite ones rounded up to 2^16 by bf16 come back to 65504).
-template <typename T>
-struct Operand;
-template <>
-struct Operand<__nv_bfloat16> {
-  static constexpr uint32_t kFormat = 1u;
-  static constexpr float kLift = 0.f;  // exponent that probabilities are lifted by
-  static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return pack_bf16x2(lo, hi); }
-  // Scales (z = false) or minima (z = true) of two groups as a pair.
-  static __device__ __forceinline__ uint32_t params(uint32_t a, uint32_t b, bool z) {
-    return __byte_perm(a, b, z ? 0x7632 : 0x5410);
-  }
-  // code * s + z of nibbles n and n + 4 of a word: 128 + code by a mask, less 128 (exact), and one
+__device__ __forceinline__ float exp2_int(int e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
+
+// The operands are fp16, rounded once from what the codes stand for; sums are fp32. fp16 activations
+// as they are: their keys and values fit. bf16 ones reach further, so they are brought to units of
+// a power of two: q a row (largest magnitude 2^14 to 2^15), keys and values every 32 tokens, a warp of
+// those that make them (2^7 to 2^15, in steps of 2^8 so that units seldom differ); what is below
+// 2^-21 of the largest loses bits. The units of q and keys
+// go into the scores' factor, that of the values into P where it is not the output's own, which
+// follows the largest. Against 64 bits (2-norm) bf16 operands had 3.2e-3, of which the output's own
+// rounding is 1.7e-3; fp16 activations have 4e-4 and 2e-4.
+__device__ __forceinline__ uint32_t values(uint32_t w, int n, uint32_t s, uint32_t z) {
+  // code * s + z of nibbles n and n + 4 of a word: 1024 + code by a mask, less 1024 (exact), and one
   // rounding in the multiply-add.
-  static __device__ __forceinline__ uint32_t values(uint32_t w, int n, uint32_t s, uint32_t z) {
-    uint32_t x = ((w >> (4 * n)) & 0x000F000Fu) | 0x43004300u;
-    asm("sub.rn.bf16x2 %0, %0, %1;" : "+r"(x) : "r"(0x43004300u));
-    asm("fma.rn.bf16x2 %0, %0, %1, %2;" : "+r"(x) : "r"(s), "r"(z));
-    return x;
-  }
-};
-template <>
-struct Operand<__half> {
-  static constexpr uint32_t kFormat = 0u;
-  static constexpr float kLift = 7.f;  // at most 2^15 while the maximum lags by 2^8; normal down to 2^-21
-  static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return pack_f16x2(lo, hi); }
-  static __device__ __forceinline__ float fit(float x) {
-    return fabsf(x) <= 65536.f ? fminf(fmaxf(x, -65504.f), 65504.f) : x;
-  }
-  static __device__ __forceinline__ uint32_t params(uint32_t a, uint32_t b, bool z) {
-    return z ? pack_f16x2(fit(kv4_min(a)), fit(kv4_min(b))) : pack_f16x2(kv4_scale(a), kv4_scale(b));
-  }
-  static __device__ __forceinline__ uint32_t values(uint32_t w, int n, uint32_t s, uint32_t z) {
-    uint32_t x = ((w >> (4 * n)) & 0x000F000Fu) | 0x64006400u;  // 1024 + code
-    asm("sub.rn.f16x2 %0, %0, %1;" : "+r"(x) : "r"(0x64006400u));
-    asm("fma.rn.f16x2 %0, %0, %1, %2;" : "+r"(x) : "r"(s), "r"(z));
-    return x;
-  }
-};
+  uint32_t x = ((w >> (4 * n)) & 0x000F000Fu) | 0x64006400u;
+  asm("sub.rn.f16x2 %0, %0, %1;" : "+r"(x) : "r"(0x64006400u));
+  asm("fma.rn.f16x2 %0, %0, %1, %2;" : "+r"(x) : "r"(s), "r"(z));
+  return x;
+}
+// The largest finite magnitude that a group's codes can stand for, as ordered bits.
+__device__ __forceinline__ uint32_t group_top(uint32_t p) {
+  const float z = fabsf(kv4_min(p)), y = fabsf(fmaf(15.f, kv4_scale(p), kv4_min(p)));
+  return __float_as_uint(fmaxf(z < INFINITY ? z : 0.f, y < INFINITY ? y : 0.f));
+}
+// The larger magnitude of a bf16 pair's, as floats.
+__device__ __forceinline__ float pair_top(uint32_t w) {
+  return fmaxf(fabsf(__uint_as_float(w << 16)), fabsf(__uint_as_float(w & 0xffff0000u)));
+}
 __device__ __forceinline__ void sts128(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
@@ -129,10 +109,12 @@ __global__ void __launch_bounds__(kPmThreads, 1)
   using S = PromptSmem<D>;
   constexpr int NG = D / kKv4Group;
   constexpr int kWords = D / 8;  // 32-bit words of codes a row; chunks of eight channels
-  constexpr uint32_t kIdescS = umma_idesc(Operand<T>::kFormat, Operand<T>::kFormat, kPmTile, kPmSub);
+  constexpr uint32_t kIdescS = umma_idesc(0u, 0u, kPmTile, kPmSub);
   constexpr uint32_t kIdescO = 
-      umma_idesc(Operand<T>::kFormat, Operand<T>::kFormat, kPmTile, D) | kUmmaBTransposed;
+      umma_idesc(0u, 0u, kPmTile, D) | kUmmaBTransposed;
   constexpr uint32_t kColS = 0, kColO = 2 * kPmTile;
+  constexpr bool kUnits = std::is_same_v<T, __nv_bfloat16>;
+  constexpr float kLift = 7.f;  // of P: at most 2^15 while the maximum lags by 2^8; normal down to 2^-21
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* kfull = reinterpret_cast<uint64_t*>(smem + S::kBars);
@@ -146,6 +128,7 @@ __global__ void __launch_bounds__(kPmThreads, 1)
   uint64_t* mdone = ofull + 2;           // [tile]: everything issued is done
   uint64_t* qfull = mdone + 2;           // [tile]: q is there
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(qfull + 2);
+  volatile int* units = reinterpret_cast<volatile int*>(smem + S::kUnits);  // as exponents of two
 
   const int tid = threadIdx.x;
   const int warp = tid >> 5;
@@ -231,7 +214,7 @@ __global__ void __launch_bounds__(kPmThreads, 1)
     // What every row of the block sees from here on: below it no row is masked.
     const int first_lim = a.causal ? len - n + div_by(r0, share, a.share_inv) + 1 : len;
     uint4 kc[NG], vc[NG];
-    uint32_t kp[NG], vp[NG];
+    uint32_t kp[NG], vp[NG], vq[NG];  // vq: the next step's vp
     int64_t row = 0;  // of this thread's token of the step being fetched; -1 beyond the tokens
     auto find = [&](int j) {
       row = -1;
@@ -246,25 +229,43 @@ __global__ void __launch_bounds__(kPmThreads, 1)
       col += dcol, off += doff;
       if (off >= per_page) off -= per_page, ++col;
     };
-    auto fetch = [&](const uint8_t* codes, const uint32_t* params, uint4(&c)[NG], uint32_t(&p)[NG]) {
+    auto fetch_params = [&](const uint32_t* params, uint32_t(&p)[NG]) {
 #pragma unroll
-      for (int i = 0; i < NG; ++i) c[i] = make_uint4(0u, 0u, 0u, 0u), p[i] = 0u;
+      for (int i = 0; i < NG; ++i) p[i] = 0u;
       if (row >= 0) {
-        const uint4* c4 = reinterpret_cast<const uint4*>(codes + row * (D / 2));
         const uint2* p2 = reinterpret_cast<const uint2*>(params + row * NG);
 #pragma unroll
         for (int i = 0; i < NG / 2; ++i) {
           const uint2 x = __ldg(p2 + i);
           p[2 * i] = x.x, p[2 * i + 1] = x.y;
         }
+      }
+    };
+    auto fetch = [&](const uint8_t* codes, uint4(&c)[NG]) {
+#pragma unroll
+      for (int i = 0; i < NG; ++i) c[i] = make_uint4(0u, 0u, 0u, 0u);
+      if (row >= 0) {
+        const uint4* c4 = reinterpret_cast<const uint4*>(codes + row * (D / 2));
 #pragma unroll
         for (int i = 0; i < D / 32; ++i) c[i] = __ldg(c4 + i);
       }
     };
+    // Scales (z = false) or minima (z = true) of two groups as a pair in fp16.
+    const auto pair = [&](uint32_t x, uint32_t y, bool z, float up) {
+      if constexpr (kUnits) {
+        return z ? pack_f16x2(kv4_min(x) * up, kv4_min(y) * up) : pack_f16x2(kv4_scale(x) * up, kv4_scale(y) * up);
+      } else {
+        // The largest finite minimum that bf16 rounded up to 2^16 comes back to 65504.
+        const auto fit = [](float v) { return fabsf(v) <= 65536.f ? fminf(fmaxf(v, -65504.f), 65504.f) : v; };
+        return z ? pack_f16x2(fit(kv4_min(x)), fit(kv4_min(y))) : pack_f16x2(kv4_scale(x), kv4_scale(y));
+      }
+    };
     if (most > 0) {
       find(0);
-      fetch(a.cache.k_codes, a.cache.k_params, kc, kp);
-      fetch(a.cache.v_codes, a.cache.v_params, vc, vp);
+      fetch_params(a.cache.k_params, kp);
+      fetch_params(a.cache.v_params, vp);
+      fetch(a.cache.k_codes, kc);
+      fetch(a.cache.v_codes, vc);
     }
     bool ok = true;
     for (int j = 0; ok && j < most; ++j) {
@@ -282,44 +283,65 @@ __global__ void __launch_bounds__(kPmThreads, 1)
           for (int i = 0; i < NG; ++i) vp[i] = 0u, kp[i] = 0x7FC07FC0u;
         }
       }
+      float kup = 1.f, vup = 1.f;
+      if constexpr (kUnits) {
+        uint32_t kt = 0u, vt = 0u;
+#pragma unroll
+        for (int i = 0; i < NG; ++i) kt = max(kt, group_top(kp[i])), vt = max(vt, group_top(vp[i]));
+        const int ke = max(16, static_cast<int>(__reduce_max_sync(0xffffffffu, kt) >> 23) | 7) - 141;
+        const int ve = max(16, static_cast<int>(__reduce_max_sync(0xffffffffu, vt) >> 23) | 7) - 141;
+        kup = exp2_int(-ke), vup = exp2_int(-ve);
+        // Both tiles have read this slot: vempty of step j - 3 was waited for, and it is handed back
+        // after P of that step, which is after what this slot held (step j - 4).
+        if (lane == 0) {
+          units[(j & 3) * 8 + warp - kPmDqWarp] = ke;
+          units[(j & 3) * 8 + 4 + warp - kPmDqWarp] = ve;
+        }
+      }
       if (j >= kPmStages) ok = mbar_wait_bounded(&kempty[s], ((j / kPmStages) - 1) & 1, wait_ns);
       const uint32_t kt = smem_u32(smem + S::kK) + s * S::kTileBytes;
       const uint32_t vt = smem_u32(smem + S::kV) + s * S::kTileBytes;
       // Keys: word c * NG + g holds channels 32 g + 8 c .. + 7, one group; chunk 4 g + c.
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
-        const uint32_t sc = Operand<T>::params(kp[g], kp[g], false), z = Operand<T>::params(kp[g], kp[g], true);
+        const uint32_t sc = pair(kp[g], kp[g], false, kup), z = pair(kp[g], kp[g], true, kup);
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           const int wi = c * NG + g;
           const uint32_t w = reinterpret_cast<const uint32_t*>(kc)[wi];
-          sts128(kt + tile_offset(t, 4 * g + c), Operand<T>::values(w, 0, sc, z), Operand<T>::values(w, 1, sc, z),
-                 Operand<T>::values(w, 2, sc, z), Operand<T>::values(w, 3, sc, z));
+          sts128(kt + tile_offset(t, 4 * g + c), values(w, 0, sc, z), values(w, 1, sc, z),
+                 values(w, 2, sc, z), values(w, 3, sc, z));
         }
       }
       fence_proxy_async_smem();
       mbar_arrive(&kfull[s]);
       if (j + 1 < most) {  // the next keys are on their way while the values are made
         find(j + 1);
-        fetch(a.cache.k_codes, a.cache.k_params, kc, kp);
+        fetch_params(a.cache.k_params, kp);
+        fetch_params(a.cache.v_params, vq);
+        fetch(a.cache.k_codes, kc);
       }
       if (ok && j >= kPmStages) ok = mbar_wait_bounded(&vempty[s], ((j / kPmStages) - 1) & 1, wait_ns);
       // Values: word wi holds four channels each of two neighbouring groups in its halves.
 #pragma unroll
       for (int h = 0; h < NG / 2; ++h) {
-        const uint32_t sc = Operand<T>::params(vp[2 * h], vp[2 * h + 1], false);
-        const uint32_t z = Operand<T>::params(vp[2 * h], vp[2 * h + 1], true);
+        const uint32_t sc = pair(vp[2 * h], vp[2 * h + 1], false, vup);
+        const uint32_t z = pair(vp[2 * h], vp[2 * h + 1], true, vup);
 #pragma unroll
         for (int c = 0; c < 8; ++c) {
           const int wi = c * (NG / 2) + h;
           const uint32_t w = reinterpret_cast<const uint32_t*>(vc)[wi];
-          sts128(vt + tile_offset(t, wi), Operand<T>::values(w, 0, sc, z), Operand<T>::values(w, 1, sc, z),
-                 Operand<T>::values(w, 2, sc, z), Operand<T>::values(w, 3, sc, z));
+          sts128(vt + tile_offset(t, wi), values(w, 0, sc, z), values(w, 1, sc, z),
+                 values(w, 2, sc, z), values(w, 3, sc, z));
         }
       }
       fence_proxy_async_smem();
       mbar_arrive(&vfull[s]);
-      if (j + 1 < most) fetch(a.cache.v_codes, a.cache.v_params, vc, vp);
+      if (j + 1 < most) {
+        fetch(a.cache.v_codes, vc);
+#pragma unroll
+        for (int i = 0; i < NG; ++i) vp[i] = vq[i];
+      }
     }
     if (!ok) record_status(QTTS_ERR_TIMEOUT);
   } else if (warp >= kPmMmaWarp) {
@@ -399,8 +421,9 @@ __global__ void __launch_bounds__(kPmThreads, 1)
     // Tokens that all rows of this tile see (they are in order).
     const int first_lim = (a.causal ? len - n + div_by(r0 + i * kPmTile, share, a.share_inv) + 1 : len) - j0 * kPmTile;
     const bool whole = r0 + i * kPmTile + kPmTile <= rows;
-    const float to_log2 = a.scale * 1.4426950408889634f;
+    float to_log2 = a.scale * 1.4426950408889634f;  // with bf16, from the units of the row's q
     float m = -INFINITY, l = 0.f;
+    int vunit = -1000;  // of O, an exponent of two; none yet
     bool ok = true;
 
     // Rows of a warp as it moves them: kWords lanes a row, the rows' offsets from their lanes.
@@ -409,7 +432,7 @@ __global__ void __launch_bounds__(kPmThreads, 1)
     const int tile_row = (warp & 3) * 32;  // the warp's first row of the tile
     // q, channels of a chunk in the order 0 4 1 5 2 6 3 7, all loads of the warp's rows at once:
     // rows beyond the last read the first and are cleared, since loads under a condition of
-    // their own were waited for one by one (4 prompts of 2048 tokens: 108 us, against 94).
+    // their own were waited for one by one (4 prompts of 2048 tokens: 108 us, against 94 at that step).
     if (most > 0 && i < tiles_a_cta) {
       const int64_t mine = r < rows ? (start + token) * a.q_token_stride + head * a.q_head_stride : -1;
       uint4 v[kPasses];
@@ -424,9 +447,36 @@ __global__ void __launch_bounds__(kPmThreads, 1)
 #pragma unroll
       for (int x = 0; x < kPasses; ++x) {
         if (!(keep >> x & 1)) v[x] = make_uint4(0u, 0u, 0u, 0u);
-        sts128(qt + tile_offset(tile_row + x * kRowsAPass + sub, ch), __byte_perm(v[x].x, v[x].z, 0x5410),
-               __byte_perm(v[x].x, v[x].z, 0x7632), __byte_perm(v[x].y, v[x].w, 0x5410),
-               __byte_perm(v[x].y, v[x].w, 0x7632));
+        const uint32_t at = qt + tile_offset(tile_row + x * kRowsAPass + sub, ch);
+        if constexpr (kUnits) {
+          sts128(at, v[x].x, v[x].y, v[x].z, v[x].w);
+        } else {
+          sts128(at, __byte_perm(v[x].x, v[x].z, 0x5410), __byte_perm(v[x].x, v[x].z, 0x7632),
+                 __byte_perm(v[x].y, v[x].w, 0x5410), __byte_perm(v[x].y, v[x].w, 0x7632));
+        }
+      }
+      if constexpr (kUnits) {
+        // Each thread brings its own row to its unit.
+        __syncwarp();
+        float top = 0.f;
+#pragma unroll 4
+        for (int k = 0; k < kWords; ++k) {
+          const uint4 e = lds128(qt + tile_offset(tid & 127, k));
+          top = fmaxf(fmaxf(top, fmaxf(pair_top(e.x), pair_top(e.y))), fmaxf(pair_top(e.z), pair_top(e.w)));
+        }
+        const int e = min(100, max(-100, 141 - static_cast<int>(__float_as_uint(top) >> 23)));
+        const float up = exp2_int(e);
+        to_log2 *= exp2_int(-e);
+#pragma unroll 4
+        for (int k = 0; k < kWords; ++k) {
+          const uint32_t at = qt + tile_offset(tid & 127, k);
+          const uint4 x = lds128(at);
+          const auto two = [&](uint32_t p, uint32_t q, bool hi) {
+            return pack_f16x2(__uint_as_float(hi ? p & 0xffff0000u : p << 16) * up,
+                              __uint_as_float(hi ? q & 0xffff0000u : q << 16) * up);
+          };
+          sts128(at, two(x.x, x.z, false), two(x.x, x.z, true), two(x.y, x.w, false), two(x.y, x.w, true));
+        }
       }
       fence_proxy_async_smem();
       mbar_arrive(&qfull[i]);
@@ -434,6 +484,15 @@ __global__ void __launch_bounds__(kPmThreads, 1)
     auto step = [&](int u, bool masked) {
       const int left = lim - u * kPmSub;  // columns that this row sees
       const uint32_t tb = ts + (u & 1) * kPmSub;
+      // Factors of the scores of the two halves, and units of their values.
+      float to0 = to_log2, to1 = to_log2;
+      int v0 = 0, v1 = 0;
+      if constexpr (kUnits) {
+        const volatile int* un = units + (u >> 1 & 3) * 8 + 2 * (u & 1);
+        to0 = fminf(fmaxf(to_log2 * exp2_int(un[0]), 1e-37f), 1e37f);
+        to1 = fminf(fmaxf(to_log2 * exp2_int(un[1]), 1e-37f), 1e37f);
+        v0 = un[4], v1 = un[5];
+      }
       uint32_t s[2][32];
       tmem_ld<32>(tb, s[0]);
       tmem_ld<32>(tb + 32, s[1]);
@@ -445,14 +504,20 @@ __global__ void __launch_bounds__(kPmThreads, 1)
       }
 #pragma unroll
       for (int k = 0; k < kPmSub; ++k) {
-        mx4[k % 4] = fmaxf(mx4[k % 4], __uint_as_float(s[k / 32][k % 32]));
+        float& top = mx4[2 * (k / 32) + k % 2];
+        top = fmaxf(top, __uint_as_float(s[k / 32][k % 32]));
       }
-      const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * to_log2;  // scale > 0
-      if (__any_sync(0xffffffffu, mx > m + 8.f)) {
+      const float mx = fmaxf(fmaxf(mx4[0], mx4[1]) * to0, fmaxf(mx4[2], mx4[3]) * to1);  // scale > 0
+      const int vmost = max(v0, v1);
+      if (__any_sync(0xffffffffu, mx > m + 8.f) || (kUnits && vmost > vunit)) {
         const float up = fmaxf(m, mx);
-        const float f = up > m ? ex2f(m - up) : 1.f;
+        float f = up > m ? ex2f(m - up) : 1.f;
         m = up;
         l *= f;
+        if (kUnits && vmost > vunit) {
+          if (u > 0) f *= exp2_int(max(-126, vunit - vmost));
+          vunit = vmost;
+        }
         if (u > 0) {
           // S(u) came after O took P(u - 2); it may be taking P(u - 1).
           ok = ok && __all_sync(0xffffffffu, mbar_wait_bounded(&odone[i], (u - 1) & 1, wait_ns));
@@ -468,18 +533,26 @@ __global__ void __launch_bounds__(kPmThreads, 1)
           }
         }
       }
-      const float off = Operand<T>::kLift - (m == -INFINITY ? 0.f : m);
+      const float off = kLift - (m == -INFINITY ? 0.f : m);
       float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         uint32_t p[16];
 #pragma unroll
         for (int k = 0; k < 32; k += 2) {
-          const float x = ex2f(fmaf(__uint_as_float(s[c][k]), to_log2, off));
-          const float y = ex2f(fmaf(__uint_as_float(s[c][k + 1]), to_log2, off));
+          const float x = ex2f(fmaf(__uint_as_float(s[c][k]), c ? to1 : to0, off));
+          const float y = ex2f(fmaf(__uint_as_float(s[c][k + 1]), c ? to1 : to0, off));
           sum[k / 2 % 2] += x;
           sum[2 + k / 2 % 2] += y;
-          p[k / 2] = Operand<T>::pack(x, y);
+          p[k / 2] = pack_f16x2(x, y);
+        }
+        if constexpr (kUnits) {
+          const int d = vunit - (c ? v1 : v0);
+          if (d != 0) {  // 2^-d as an fp16 pair, 0 below 2^-24
+            const uint32_t g = (d < 15 ? (15 - d) << 10 : d <= 24 ? 1 << (24 - d) : 0) * 0x10001u;
+#pragma unroll
+            for (int k = 0; k < 16; ++k) asm("mul.rn.f16x2 %0, %0, %1;" : "+r"(p[k]) : "r"(g));
+          }
         }
         tmem_st_x16(tb + 16 * c, p);
       }
@@ -500,7 +573,8 @@ __global__ void __launch_bounds__(kPmThreads, 1)
     }
     if (!ok && lane == 0) record_status(QTTS_ERR_TIMEOUT);
     if (i < tiles_a_cta && r0 + i * kPmTile < rows) {
-      const float inv = l == 0.f ? 0.f : 1.f / l;
+      const float unit = kUnits && steps[i] > 0 ? exp2_int(vunit) : 1.f;
+      const float inv = l == 0.f ? 0.f : unit / l;
       // Column 8 wi + 2 x + e of O is channel 32 (2 (wi % (NG/2)) + e) + 4 (wi / (NG/2)) + x: the
       // columns of NG words together are eight channels of every group. A warp's 32 rows go through
       // shared memory (its part of q's tile, which no product reads any more), so that whole
@@ -535,7 +609,9 @@ __global__ void __launch_bounds__(kPmThreads, 1)
 #pragma unroll
             for (int q = 0; q < 2; ++q) {
               const int k = 8 * (q * (NG / 2) + g / 2) + (g & 1);
-              sts128(qt + tile_offset(row, 4 * g + 2 * (c & 1) + q), o[k], o[k + 2], o[k + 4], o[k + 6]);
+              const auto out = [&](uint32_t x) { return __float_as_uint(__uint_as_float(x) * unit); };
+              sts128(qt + tile_offset(row, 4 * g + 2 * (c & 1) + q), out(o[k]), out(o[k + 2]), out(o[k + 4]),
+                     out(o[k + 6]));
             }
           }
           if (c & 1) {
@@ -613,8 +689,8 @@ int launch_pm(const Kv4AttnArgs& a, const PromptPlan& p, bool pdl, cudaStream_t 
     cfg.attrs = attr;
     cfg.numAttrs = 1;
   }
-  return cudaLaunchKernelEx(&cfg, kv4_prompt_kernel<T, D>, a, p.tiles, p.splits, p.split_steps, current_wait_limit_ns()) ==
-                 cudaSuccess
+  return cudaLaunchKernelEx(&cfg, kv4_prompt_kernel<T, D>, a, p.tiles, p.splits, p.split_steps,
+                            current_wait_limit_ns()) == cudaSuccess
              ? QTTS_OK
              : QTTS_ERR_LAUNCH;
 }
@@ -625,7 +701,7 @@ PromptPlan plan_prompt(int64_t max_q, int share, int kv_heads, int batch, int64_
   PromptPlan p;
   const int64_t rows = max_q * share;
   // Two tiles a CTA share the operands and hide each other's softmax (4 prompts of 2048 tokens,
-  // 16 + 2 x 8 heads of 128 channels: 90 us, one tile a CTA 133).
+  // 16 + 2 x 8 heads of 128 channels: 103 us, one tile a CTA 156).
   p.tiles = rows > kPmTile ? 2 : 1;
   p.blocks = (rows + p.tiles * kPmTile - 1) / (p.tiles * kPmTile);
   const int64_t units = p.blocks * kv_heads * batch;
