@@ -8,7 +8,11 @@
 // where the angle is the table's row for the position of the token along the axis
 // that pair j belongs to (time, height, width for images and video; one axis for
 // text). q is written in its own type, k and v as 4-bit groups (kv4.cuh). All of
-// it in fp32 between the load and the one rounding of each output.
+// it in fp32 between the load and the one rounding of each output, each step of the
+// formula rounded by itself (square root and divisions as IEEE has them, no product
+// contracted with the sum that takes it) and the sum of squares in one fixed order:
+// near the boundary between two codes a last bit decides, so the codes are those
+// of the same steps as separate fp32 operations, bit for bit.
 //
 // D / 8 lanes hold one head row, eight neighbouring channels each: one 16-byte
 // load, a pair's partner D / 16 lanes away, a group of 32 channels on four
@@ -17,13 +21,14 @@
 //
 // The projection's row is read once, q, codes and (where asked for) the stored
 // values are written once: 8192 tokens of 16 + 2 x 8 heads of 128 channels, 145 MB,
-// in 41 us (3.5 TB/s), which the instructions of norm, rotation and quantizer bound
-// more than the memory does. A lane's channels are the same in every head,
-// so a warp takes several heads of one token and gathers its cosines and sines
-// once; how many is chosen so that a short call still has a warp for every head
-// pair and a long one few gathers. 28 such warps an SM,
-// each with its next row under way, beat fewer with more (8192 tokens: 41 us; 20
-// warps and four rows ahead 48).
+// in 45 us (3.2 TB/s), which the instructions of norm, rotation and quantizer bound
+// more than the memory does. (With an approximate root and weight, cosine and root
+// folded into one factor it was 41 us, and codes near a boundary differed.) A lane's
+// channels are the same in every head, so a warp takes several heads of one token and
+// gathers its cosines and sines once; how many is chosen so that a short call still
+// has a warp for every head pair and a long one few gathers. 28 such warps an SM, each
+// with its next row under way, beat fewer with more registers (8192 tokens: 45 us; 24
+// warps 47).
 #include <type_traits>
 
 #include "kernels.h"
@@ -40,6 +45,43 @@ constexpr int kAhead = 1;  // passes whose rows are loaded ahead
 __device__ __forceinline__ float divide(float a, float s, float r) {
   const float q = a * r;
   return fmaf(fmaf(-q, s, a), r, q);
+}
+
+// Sum of squares of a head row, eight channels a lane; every lane of the row returns the same bits.
+// One order, that of torch's mean over fp32: 128 channels as 32 sums of four neighbours, one after
+// the other, 64 as they are; then the upper half is added to the lower until one sum is left. A
+// step across lanes also shares out the sums that a lane holds, so that later steps have fewer.
+template <int D>
+__device__ __forceinline__ float row_sumsq(const float (&x)[8], int l) {
+  const auto across = [](float v, int o) { return __fadd_rn(v, __shfl_xor_sync(0xffffffffu, v, o)); };
+  float p[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) p[i] = __fmul_rn(x[i], x[i]);
+  if constexpr (D == 128) {
+    const float s0 = __fadd_rn(__fadd_rn(__fadd_rn(p[0], p[1]), p[2]), p[3]);
+    const float s1 = __fadd_rn(__fadd_rn(__fadd_rn(p[4], p[5]), p[6]), p[7]);
+    const bool up = (l & 8) != 0;
+    float s = __fadd_rn(up ? s1 : s0, __shfl_xor_sync(0xffffffffu, up ? s0 : s1, 8));
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) s = across(s, o);
+    return across(s, 8);
+  } else {
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) {
+      const bool up = (l & o) != 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (i < o) {
+          const float keep = up ? p[i + o] : p[i];
+          p[i] = __fadd_rn(keep, __shfl_xor_sync(0xffffffffu, up ? p[i] : p[i + o], o));
+        }
+      }
+    }
+    float s = p[0];
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) s = across(s, o);
+    return s;
+  }
 }
 
 // The eight codes of a lane's channels; returns them one a nibble and gives the
@@ -130,13 +172,11 @@ __global__ void __launch_bounds__(32, 28) rope_kv4_kernel(const RopeKv4Args a, i
                                             : slot / a.cache.page_size;
   const int in_page = stored ? static_cast<int>(slot - page * a.cache.page_size) : 0;
 
-  // A head row through norm and rotation is y_i = inv * (x_i A_i + x_partner B_i), A and B the
-  // norm's weights times cosine and signed sine: gathered once for all heads of a kind.
+  // Norm weights, cosines and signed sines of this lane's channels: gathered once for all heads of a
+  // kind.
+  uint4 fw = make_uint4(0u, 0u, 0u, 0u);
   float fa[8], fb[8];
   const auto factors = [&](const void* weight) {
-    const int partner = l < kLanes / 2 ? l + kLanes / 2 : l - kLanes / 2;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) fa[i] = 1.f, fb[i] = 0.f;
     if (a.cos != nullptr) {
       const int j0 = 8 * (l % (kLanes / 2));  // first of this lane's pairs
 #pragma unroll
@@ -150,39 +190,25 @@ __global__ void __launch_bounds__(32, 28) rope_kv4_kernel(const RopeKv4Args a, i
       }
     }
     if (weight != nullptr) {
-      const uint4 w0 = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(weight) + 8 * l));
-      const uint4 w1 = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(weight) + 8 * partner));
-      const T* e0 = reinterpret_cast<const T*>(&w0);
-      const T* e1 = reinterpret_cast<const T*>(&w1);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) fa[i] *= to_float(e0[i]), fb[i] *= to_float(e1[i]);
+      fw = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(weight) + 8 * l));
     }
   };
+  // Each step of the formula rounded once, none contracted with the next.
   const auto turn = [&](const uint4& raw, float(&y)[8], bool norm) {
-    uint4 other = raw;
-    if (a.cos != nullptr) {
-      other.x = __shfl_xor_sync(0xffffffffu, raw.x, kLanes / 2);
-      other.y = __shfl_xor_sync(0xffffffffu, raw.y, kLanes / 2);
-      other.z = __shfl_xor_sync(0xffffffffu, raw.z, kLanes / 2);
-      other.w = __shfl_xor_sync(0xffffffffu, raw.w, kLanes / 2);
-    }
     const T* e = reinterpret_cast<const T*>(&raw);
-    const T* o = reinterpret_cast<const T*>(&other);
-    float inv = 1.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = to_float(e[i]);
     if (norm) {
-      float ss = 0.f;
+      const float inv = rms_inv(row_sumsq<D>(y, l), D, a.eps);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) ss = fmaf(to_float(e[i]), to_float(e[i]), ss);
-#pragma unroll
-      for (int q = kLanes / 2; q > 0; q >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, q);
-      inv = rsqrtf(ss * (1.0f / D) + a.eps);
+      for (int i = 0; i < 8; ++i) y[i] = rms_apply(y[i], inv, to_float(reinterpret_cast<const T*>(&fw)[i]));
     }
     if (a.cos != nullptr) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] = inv * fmaf(to_float(o[i]), fb[i], to_float(e[i]) * fa[i]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] = inv * (to_float(e[i]) * fa[i]);
+      for (int i = 0; i < 8; ++i) {
+        const float other = __shfl_xor_sync(0xffffffffu, y[i], kLanes / 2);
+        y[i] = __fadd_rn(__fmul_rn(y[i], fa[i]), __fmul_rn(other, fb[i]));
+      }
     }
   };
   // Codes, parameters and (where asked for) the values of a head row, through this lane's pointers.
@@ -248,9 +274,8 @@ __global__ void __launch_bounds__(32, 28) rope_kv4_kernel(const RopeKv4Args a, i
       for (int u = 0; u < kAhead; ++u) {
         const int p = p0 + u;
         if (p < to) {
-          uint4 now = raw[u];
+          const uint4 now = raw[u];
           if (p + kAhead < to) raw[u] = fetch(p + kAhead);
-          if (!ok) now = make_uint4(0u, 0u, 0u, 0u);
           const bool live = p * kHeads + sub < kind_heads;
           float y[8];
           if constexpr (kKind < 2) {
@@ -259,6 +284,10 @@ __global__ void __launch_bounds__(32, 28) rope_kv4_kernel(const RopeKv4Args a, i
             const T* e = reinterpret_cast<const T*>(&now);
 #pragma unroll
             for (int i = 0; i < 8; ++i) y[i] = to_float(e[i]);
+          }
+          if (!ok) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) y[i] = 0.f;
           }
           if constexpr (kKind == 0) {
             if (live) *reinterpret_cast<uint4*>(out) = pack8<T>(y);
@@ -281,12 +310,13 @@ int launch_rk(const RopeKv4Args& a, bool pdl, cudaStream_t stream) {
   constexpr int kHeads = 32 / (D / 8);
   // Passes a token needs.
   const int total = (a.q_heads + kHeads - 1) / kHeads + 2 * ((a.cache.kv_heads + kHeads - 1) / kHeads);
-  // A warp for every pass while that is less than some four warps an SM; then longer warps, which
-  // gather their angles once, up to 16 passes (8192 tokens of 16 + 2 x 8 heads: 41 us, with up to
-  // four passes 50, with up to 64 the same). 333 tokens of 32 + 2 x 4 heads of 64 channels: 4.8 us,
-  // and 5.2 where only sixteen or more warps an SM are made longer; one token is 2.8 us either way.
+  // A warp for every pass while that is less than 32 warps an SM, about as many as are resident;
+  // then longer warps, which gather their angles once, up to 16 passes. A warp's passes follow
+  // one another, so longer ones before the SMs are full only wait (from 4 | 16 | 32 warps an SM on:
+  // 333 tokens of 16 + 2 x 8 heads of 128 channels 10.9 | 6.5 | 6.1 us, 1000 tokens 15.7 | 11.4 | 9.4,
+  // 333 of 32 + 2 x 4 heads of 64 channels 6.2 | 5.6 | 5.3; 8192 tokens 45 each way).
   int passes = 1;
-  while (passes < 16 && passes < total && static_cast<int64_t>(a.tokens) * total >= 4ll * kNumSMs * passes) passes *= 2;
+  while (passes < 16 && passes < total && static_cast<int64_t>(a.tokens) * total >= 32ll * kNumSMs * passes) passes *= 2;
   const int warps_a_token = (total + passes - 1) / passes;
   const int64_t warps = static_cast<int64_t>(a.tokens) * warps_a_token;
   cudaLaunchConfig_t cfg = {};
