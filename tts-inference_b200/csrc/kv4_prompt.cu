@@ -152,7 +152,6 @@ __global__ void __launch_bounds__(kPmThreads, 1)
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
-  pdl_launch_dependents();
   pdl_wait();
 
   // The longest blocks first, of all requests and heads: with `causal` the last rows see most.
@@ -167,6 +166,9 @@ __global__ void __launch_bounds__(kPmThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
+  // Only now that the columns are this CTA's: the next kernel may want some on this SM and, holding
+  // them, waits for this one to end.
+  pdl_launch_dependents();
   fine = fine && len >= 0 && len <= static_cast<int64_t>(a.table_cols) * a.cache.page_size &&
          (len == 0 || a.cache.pages > 0);
   if (!fine) {
