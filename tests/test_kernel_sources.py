@@ -36,3 +36,13 @@ def test_dependents_are_released_once_tensor_memory_is_held(path, name, text):
     published = text.index("__syncthreads()", alloc)
     released = [m.start() for m in re.finditer(r"pdl_launch_dependents\(\)", text)]
     assert released and min(released) > published, f"{path.name}: {name}"
+
+
+def test_a_wait_that_runs_out_is_the_whole_warps():
+    # The prompt kernel's roles go on with warp-wide reductions, ballots and tensor-memory accesses after
+    # a wait: lanes that gave up one by one would leave the others of their warp waiting without a limit.
+    text = kernels(SRC_DIR / "kv4_prompt.cu")["kv4_prompt_kernel"]
+    waits = [m.start() for m in re.finditer(r"mbar_wait_bounded\(", text)]
+    assert waits
+    for at in waits:
+        assert re.search(r"__all_sync\(\s*0xffffffffu,\s*$", text[:at]), text[max(0, at - 90):at + 60]

@@ -269,8 +269,12 @@ __global__ void __launch_bounds__(kPmThreads, 1)
       fetch(a.cache.k_codes, kc);
       fetch(a.cache.v_codes, vc);
     }
+    // A wait that runs out ends the loop for the whole warp: its reductions and ballots need all lanes.
+    const auto wait = [&](uint64_t* bar, int phase) {
+      return __all_sync(0xffffffffu, mbar_wait_bounded(bar, phase & 1, wait_ns));
+    };
     bool ok = true;
-    for (int j = 0; ok && j < most; ++j) {
+    for (int j = 0; j < most; ++j) {
       const int s = j % kPmStages;
       if ((j0 + j + 1) * kPmTile > first_lim) {
         // Rows that do not see a token must not meet its NaN or infinity (0 * NaN): a token with
@@ -300,7 +304,8 @@ __global__ void __launch_bounds__(kPmThreads, 1)
           units[(j & 3) * 8 + 4 + warp - kPmDqWarp] = ve;
         }
       }
-      if (j >= kPmStages) ok = mbar_wait_bounded(&kempty[s], ((j / kPmStages) - 1) & 1, wait_ns);
+      ok = j < kPmStages || wait(&kempty[s], j / kPmStages - 1);
+      if (!ok) break;
       const uint32_t kt = smem_u32(smem + S::kK) + s * S::kTileBytes;
       const uint32_t vt = smem_u32(smem + S::kV) + s * S::kTileBytes;
       // Keys: word c * NG + g holds channels 32 g + 8 c .. + 7, one group; chunk 4 g + c.
@@ -323,7 +328,8 @@ __global__ void __launch_bounds__(kPmThreads, 1)
         fetch_params(a.cache.v_params, vq);
         fetch(a.cache.k_codes, kc);
       }
-      if (ok && j >= kPmStages) ok = mbar_wait_bounded(&vempty[s], ((j / kPmStages) - 1) & 1, wait_ns);
+      ok = j < kPmStages || wait(&vempty[s], j / kPmStages - 1);
+      if (!ok) break;
       // Values: word wi holds four channels each of two neighbouring groups in its halves.
 #pragma unroll
       for (int h = 0; h < NG / 2; ++h) {
@@ -345,7 +351,7 @@ __global__ void __launch_bounds__(kPmThreads, 1)
         for (int i = 0; i < NG; ++i) vp[i] = vq[i];
       }
     }
-    if (!ok) record_status(QTTS_ERR_TIMEOUT);
+    if (!ok && lane == 0) record_status(QTTS_ERR_TIMEOUT);
   } else if (warp >= kPmMmaWarp) {
     // ---------------- the products of tile i ----------------
     // The whole warp runs along, so that operands and branches are uniform; one elected lane issues.
