@@ -683,7 +683,8 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas) kv4_rows_kernel(const Kv4A
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-// The parts of a (token, head) row from the workspace. Bound by latency: all statistics are read
+// The parts of a (token, head) row from the workspace, request by request: rows of no request have
+// none and are not written. Bound by latency: all statistics are read
 // at once, and four parts a warp are in flight. Eight warps a row where there are many parts (one
 // long cache: 256 parts in 4 us instead of 28 with one warp), one where there are many rows.
 constexpr int kJoinWarps = 8;  // a CTA
@@ -702,8 +703,13 @@ __global__ void __launch_bounds__(32 * kJoinWarps) kv4_join_kernel(const Kv4Attn
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int sub = warp / kRowWarps, rw = warp % kRowWarps;
   const int tid = rw * 32 + lane;  // within the row
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + sub;
-  const bool there = row < static_cast<int64_t>(a.total_q) * a.q_heads;
+  int start = 0, n = 0;
+  if (!request_rows(a, blockIdx.y, start, n)) n = 0;
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * kRows;
+  const int64_t rows = static_cast<int64_t>(n) * a.q_heads;  // of this request
+  if (first >= rows) return;
+  const bool there = first + sub < rows;
+  const int64_t row = static_cast<int64_t>(start) * a.q_heads + first + sub;
   const float2* st = a.stats + row * splits;
   float2 s[kSlots];
   float top = -INFINITY;
@@ -892,13 +898,13 @@ int launch_rows(Kv4AttnArgs a, const RowsPlan& p, bool pdl, cudaStream_t stream)
 
 template <typename T, int D>
 int launch_join(const Kv4AttnArgs& a, int splits, cudaStream_t stream) {
-  const int64_t rows = static_cast<int64_t>(a.total_q) * a.q_heads;
+  const int64_t rows = static_cast<int64_t>(a.max_q) * a.q_heads;  // of a request, at most
   if (splits <= kFewSplits) {
-    return launch(kv4_join_kernel<T, D, 1>, dim3(static_cast<unsigned>((rows + kJoinWarps - 1) / kJoinWarps)),
+    return launch(kv4_join_kernel<T, D, 1>, dim3(static_cast<unsigned>((rows + kJoinWarps - 1) / kJoinWarps), a.batch),
                   32 * kJoinWarps, 0, 1, true, stream, a, splits);
   }
-  return launch(kv4_join_kernel<T, D, kJoinWarps>, dim3(static_cast<unsigned>(rows)), 32 * kJoinWarps, 0, 1, true,
-                stream, a, splits);
+  return launch(kv4_join_kernel<T, D, kJoinWarps>, dim3(static_cast<unsigned>(rows), a.batch), 32 * kJoinWarps, 0, 1,
+                true, stream, a, splits);
 }
 
 template <typename T, int D>

@@ -215,7 +215,8 @@ def kv4_attention(
     the cached tokens of each request, new ones included. Without ``q_starts`` every
     request brings ``total / batch`` new tokens (one, in a decode step); with it, ``[batch +
     1]`` int32, request b brings rows ``q_starts[b]`` to ``q_starts[b + 1]`` and ``max_q``
-    says how many at most. The new tokens are the last ones of their request: with
+    says how many at most (rows of no request keep what ``out`` held: in a new ``out``,
+    anything). The new tokens are the last ones of their request: with
     ``causal`` each sees the tokens up to itself, without it every cached token (cross
     attention to an encoder's states, for instance). ``q_heads`` is a multiple of the
     cache's heads. A row that sees nothing gives zeros. ``scale`` defaults to
