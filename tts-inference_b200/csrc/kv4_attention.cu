@@ -15,12 +15,16 @@
 //     (largest magnitude in [2^14, 2^15): exact for bf16 down to 2^-24 of it) and
 //     the channels of the higher nibbles by 2^-4 more. The group's scale and
 //     minimum enter once per (token, row, group), in fp32;
-//   * out^T = V^T P^T: two tokens' half-words are interleaved by a byte permute, so
-//     the same masks again give operand pairs, and one fp16 fused multiply-add
-//     makes a pair the value itself, rounded once: code * scale + minimum, in units
-//     of a power of two that follows the largest scale the warp has met (that scale
-//     becomes 2^14..2^15 against the code's 2^-24, so a value keeps 11 bits, or 2^-15
-//     of that scale where it is smaller). Scale and minimum of a tile are
+//   * out^T = V^T P^T: two tokens' half-words are interleaved by bytes, so that a mask
+//     leaves two codes of one channel in neighbouring bytes. Read as e4m3 these are
+//     code * 2^-9, and one conversion makes them an fp16 pair, one fused multiply-add
+//     the value itself, rounded once: code * scale + minimum, in units of a power of two
+//     that follows the largest scale or minimum the warp has met (values then reach
+//     2^10 and keep their 11 bits down to 2^-14, 2^-24 of the largest). Used as the
+//     subnormals that they are, the codes would save the conversions (2 x 131071 tokens
+//     75.5 us instead of 79.6, 64 x 4096 tokens 78 instead of 84; no less for 16 rows), but
+//     a value would keep no more than 2^-15 of the largest scale in any group and token,
+//     too little for groups of unlike size. Scale and minimum of a tile are
 //     brought to those units once, a word a lane, through shared memory.
 //     Probabilities are fp16 too, times 2^7: up to 2^15 while the running maximum
 //     may lag by 2^8, and the small ones normal down to 2^-21;
@@ -31,7 +35,7 @@
 //     that is not enough to fill the machine, any number of CTAs through a
 //     workspace that a second kernel joins. Sums are in a fixed order.
 // 2 requests over 131071 tokens, 32 + 2 x 8 heads of 128 channels: 336 MB of cache in
-// 75.6 us, 4.4 TB/s, issue slots 63 % busy: the nibbles' instructions and the waits
+// 79.6 us, 4.2 TB/s: the nibbles' instructions and the waits
 // between them bound it, the copies are ahead. 8 requests over 513 tokens: 7.1 us, a
 // launch and the chain lengths -> page -> codes -> scores -> meeting of the CTAs.
 #include <type_traits>
@@ -53,6 +57,14 @@ constexpr int kFewSplits = 32;   // up to which one warp joins a row
 // n = 0, code * 2^-20 for n = 1; nibbles n + 2 and n + 6 from the word shifted by eight.
 __device__ __forceinline__ uint32_t nib_pair(uint32_t w, int n) { return w & (n ? 0x00F000F0u : 0x000F000Fu); }
 
+// Two 4-bit codes, a byte each, as fp16 numbers code * 2^-9, exactly: read as e4m3 a byte below 16 is
+// that many steps of 2^-9 (subnormals, and the first eight normal numbers).
+__device__ __forceinline__ uint32_t codes_f16x2(uint32_t two) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(static_cast<uint16_t>(two)));
+  return r;
+}
+
 __device__ __forceinline__ float ex2(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -67,11 +79,6 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
 __device__ __forceinline__ uint32_t fma_f16x2(uint32_t a, uint32_t b, uint32_t c) {
   uint32_t r;
   asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
-  return r;
-}
-__device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
-  uint32_t r;
-  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
 // D = A x B (no accumulator to be zeroed first), m16n8k16 fp16 -> fp32.
@@ -307,7 +314,7 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas) kv4_rows_kernel(const Kv4A
   }
 
   float m[NT][2], l[NT][2];
-  float acc[NT][NG][2][4];  // [group][channel pair] of out^T, fp32, in units of 2^(vexp - 127 + 10)
+  float acc[NT][NG][2][4];  // [group][channel pair] of out^T, fp32, in units of 2^(vexp - 127 - 5)
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -321,12 +328,12 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas) kv4_rows_kernel(const Kv4A
       }
     }
   }
-  // Unit of the values: 2^(vexp - 127 + 10), vexp the exponent field of the largest value scale
-  // so far (or of the largest minimum / 2^20, where that is more: both have to stay in fp16's
-  // range). What reaches vlimit moves it.
+  // Unit of the values: 2^(vexp - 127 - 5), vexp the exponent field of the largest value scale
+  // so far (or of the largest minimum / 16, where that is more): 15 scale + |minimum| < 2^15 units.
+  // What reaches vlimit moves it.
   int vexp = 0;
   float vlimit = 0.f;
-  float vs_to = 0.f, vz_to = 0.f;  // 2^14 and 2^-10 in units of 2^(vexp - 127)
+  float vs_to = 0.f, vz_to = 0.f;  // 2^9 and 1 in those units
 
   // Token of row slot s of a 16-token operand: s with the last bit turned in every other
   // pair, so that neither the key nor the value loads below hit one bank with more than two rows.
@@ -377,22 +384,22 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas) kv4_rows_kernel(const Kv4A
       }
     }
 #pragma unroll
-    for (int k = 0; k < NG; ++k) top = fmaxf(top, fmaxf(vs[k], fabsf(vz[k]) * 0x1p-20f));
+    for (int k = 0; k < NG; ++k) top = fmaxf(top, fmaxf(vs[k], fabsf(vz[k]) * 0x1p-4f));
     if (__any_sync(0xffffffffu, !(top < vlimit))) {
       float most = 0.f;  // of the finite ones; others reach the output as they are
 #pragma unroll
       for (int k = 0; k < NG; ++k) {
-        const float x = fmaxf(vs[k], fabsf(vz[k]) * 0x1p-20f);
+        const float x = fmaxf(vs[k], fabsf(vz[k]) * 0x1p-4f);
         most = fmaxf(most, x < INFINITY ? x : 0.f);
       }
       most = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most)));
       if (!(most < vlimit)) {
-        const int to = min(243, max(16, static_cast<int>(__float_as_uint(most) >> 23)));
+        const int to = min(253, max(16, static_cast<int>(__float_as_uint(most) >> 23)));
         const float f = vlimit == 0.f ? 1.f : exp2_int(max(-126, vexp - to));
         vexp = to;
         vlimit = exp2_int(to - 126);
         vs_to = exp2_int(127 - to) * 0x1p14f;
-        vz_to = exp2_int(127 - to) * 0x1p-10f;
+        vz_to = exp2_int(127 - to) * 0x1p5f;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -537,16 +544,16 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas) kv4_rows_kernel(const Kv4A
       }
 #pragma unroll
       for (int j = 0; j < NG; ++j) {
-        // Tokens (2c, 2c + 1) and (2c + 8, 2c + 9) of group j, interleaved by half-words.
-        const uint32_t xa = __byte_perm(vw[0][j / 2], vw[1][j / 2], (j & 1) ? 0x7632 : 0x5410);
-        const uint32_t xb = __byte_perm(vw[2][j / 2], vw[3][j / 2], (j & 1) ? 0x7632 : 0x5410);
-        const uint32_t ya = xa >> 8, yb = xb >> 8;
+        // Tokens (2c, 2c + 1) and (2c + 8, 2c + 9) of group j, interleaved by bytes.
+        const uint32_t xa = __byte_perm(vw[0][j / 2], vw[1][j / 2], (j & 1) ? 0x7362 : 0x5140);
+        const uint32_t xb = __byte_perm(vw[2][j / 2], vw[3][j / 2], (j & 1) ? 0x7362 : 0x5140);
+        const uint32_t la = xa & 0x0F0F0F0Fu, ha = xa >> 4 & 0x0F0F0F0Fu;
+        const uint32_t lb = xb & 0x0F0F0F0Fu, hb = xb >> 4 & 0x0F0F0F0Fu;
         const uint32_t sa = sw[0][j], za = zw[0][j], sb = sw[1][j], zb = zw[1][j];
-        const uint32_t sa4 = mul_f16x2(sa, 0x2C002C00u), sb4 = mul_f16x2(sb, 0x2C002C00u);  // / 16
-        const uint32_t a0[4] = {fma_f16x2(nib_pair(xa, 0), sa, za), fma_f16x2(nib_pair(xa, 1), sa4, za),
-                                fma_f16x2(nib_pair(xb, 0), sb, zb), fma_f16x2(nib_pair(xb, 1), sb4, zb)};
-        const uint32_t a1[4] = {fma_f16x2(nib_pair(ya, 0), sa, za), fma_f16x2(nib_pair(ya, 1), sa4, za),
-                                fma_f16x2(nib_pair(yb, 0), sb, zb), fma_f16x2(nib_pair(yb, 1), sb4, zb)};
+        const uint32_t a0[4] = {fma_f16x2(codes_f16x2(la), sa, za), fma_f16x2(codes_f16x2(ha), sa, za),
+                                fma_f16x2(codes_f16x2(lb), sb, zb), fma_f16x2(codes_f16x2(hb), sb, zb)};
+        const uint32_t a1[4] = {fma_f16x2(codes_f16x2(la >> 16), sa, za), fma_f16x2(codes_f16x2(ha >> 16), sa, za),
+                                fma_f16x2(codes_f16x2(lb >> 16), sb, zb), fma_f16x2(codes_f16x2(hb >> 16), sb, zb)};
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           Mma16816<__half>::run(acc[nt][j][0], a0, b0[nt], b1[nt]);
@@ -583,7 +590,7 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas) kv4_rows_kernel(const Kv4A
   }
   __syncthreads();  // every warp is done with its ring: the partial outputs take its place
   float* part = reinterpret_cast<float*>(smem) + warp * kRows * S::kPitch;
-  const float vref = vlimit == 0.f ? 0.f : exp2_int(vexp - 127);  // no tile: no values
+  const float vref = vlimit == 0.f ? 0.f : exp2_int(vexp - 127) * 0x1p-5f;  // no tile: no values
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -592,8 +599,8 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas) kv4_rows_kernel(const Kv4A
 #pragma unroll
       for (int j = 0; j < NG; ++j) {
         *reinterpret_cast<float4*>(part + r * S::kPitch + 32 * j + 4 * g) = make_float4(
-            acc[nt][j][0][e] * 0x1p10f * vref, acc[nt][j][0][e + 2] * 0x1p10f * vref,
-            acc[nt][j][1][e] * 0x1p10f * vref, acc[nt][j][1][e + 2] * 0x1p10f * vref);
+            acc[nt][j][0][e] * vref, acc[nt][j][0][e + 2] * vref,
+            acc[nt][j][1][e] * vref, acc[nt][j][1][e + 2] * vref);
       }
       if (g == 0) stat_m[warp][r] = m[nt][e], stat_l[warp][r] = l[nt][e];
     }
@@ -819,7 +826,7 @@ struct RowsPlan {
 // tokens 87 | 93 | 79 us; 128 of 1000 to 2000 tokens 66 | 80 | 66 us.
 constexpr int kEvenTiles = 16, kEvenCtas = 8;
 
-RowsPlan plan_rows(int64_t max_q, int share, int kv_heads, int batch, int64_t most_tokens) {
+RowsPlan plan_rows(int64_t max_q, int share, int kv_heads, int batch, int64_t most_tokens, int head_dim) {
   RowsPlan p;
   const int64_t rows = max_q * share;
   // Eight rows fill an operand; more share what is made of the cache by pairs of eight
@@ -827,12 +834,14 @@ RowsPlan plan_rows(int64_t max_q, int share, int kv_heads, int batch, int64_t mo
   p.nt = rows <= 8 ? 1 : 2;
   p.row_blocks = (rows + 8 * p.nt - 1) / (8 * p.nt);
   const int64_t units = p.row_blocks * kv_heads * batch;
-  // CTAs an SM: two with 16 rows. With 8, three at 168 registers where units are split anyway, the
-  // quicker code (8 x 513 tokens 7.1 us, four at 128 registers 8.3; 8 x 2048: 10.9, 12.3), four
-  // where there is a unit for every SM, more of which then fit at once (32 x 2048: 27.6 us, three
-  // 32.9; 64 x 2000..4000 of 64 channels 25.8, 32.7; 64 x 4096
-  // 77.9, 79.4; but 64 x 17..8192 57.2, 56.3).
-  p.ctas = p.nt == 2 ? 2 : units > kNumSMs ? 4 : 3;
+  // CTAs an SM: two with 16 rows. With 8, three at 168 registers where units are split anyway (8 x 513
+  // tokens 7.1 us, four at 128 registers 8.3; 8 x 2048: 10.9, 12.3). Four where there is a unit for
+  // every SM and three would not hold two CTAs of each (32 x 2048 tokens: 29.8 us, three 34.0); beyond
+  // that the few values that 128 channels spill at 128 registers cost more than the fourth CTA gives
+  // (64 x 4096 tokens: 84.4, three 81.4; 64 x 17..8192: 60.8, 57.7; 128 x 1000..2000: 63.3, 62.2), and
+  // 64 channels spill none (64 x 2000..4000: 44.8, 48.6).
+  const bool four = units > kNumSMs && (head_dim == 64 || units <= 3 * kNumSMs);
+  p.ctas = p.nt == 2 ? 2 : four ? 4 : 3;
   // One wave of them, at least one tile a warp, and the limit above. CTAs that a shorter request
   // has no use for leave at once.
   const int64_t wave = static_cast<int64_t>(kNumSMs) * p.ctas;
@@ -916,7 +925,7 @@ int launch_ka(const Kv4AttnArgs& a, int dtype, bool pdl, cudaStream_t stream) {
     const int r = launch_kv4_prompt(a, p, dtype, D, pdl, stream);
     return r != QTTS_OK || p.splits == 1 ? r : launch_join<T, D>(a, p.splits, stream);
   }
-  const RowsPlan p = plan_rows(a.max_q, share, a.cache.kv_heads, a.batch, tokens);
+  const RowsPlan p = plan_rows(a.max_q, share, a.cache.kv_heads, a.batch, tokens, D);
   if (p.row_blocks * a.cache.kv_heads > 65535) return QTTS_ERR_SHAPE;
   const int r = p.ctas == 4   ? launch_rows<T, D, 1, 4>(a, p, pdl, stream)
                 : p.ctas == 3 ? launch_rows<T, D, 1, 3>(a, p, pdl, stream)
@@ -925,11 +934,11 @@ int launch_ka(const Kv4AttnArgs& a, int dtype, bool pdl, cudaStream_t stream) {
 }
 
 // CTAs whose parts meet in the workspace; 1 where none do.
-int workspace_splits(int64_t max_q, int share, int kv_heads, int batch, int64_t tokens) {
+int workspace_splits(int64_t max_q, int share, int kv_heads, int batch, int64_t tokens, int head_dim) {
   if (kv4_takes_prompt(max_q, share, kv_heads, batch, tokens)) {
     return plan_prompt(max_q, share, kv_heads, batch, tokens).splits;
   }
-  const int s = plan_rows(max_q, share, kv_heads, batch, tokens).splits;
+  const int s = plan_rows(max_q, share, kv_heads, batch, tokens, head_dim).splits;
   return s > kMaxCluster ? s : 1;
 }
 
@@ -950,7 +959,7 @@ extern "C" int64_t qtts_kv4_attention_workspace(int total_q, int max_q, int batc
                                                 int head_dim, int64_t max_tokens) {
   using namespace qtts;
   if (total_q < 1 || max_q < 1 || batch < 1 || kv_heads < 1 || q_heads < 1 || q_heads % kv_heads != 0) return 0;
-  const int splits = workspace_splits(max_q, q_heads / kv_heads, kv_heads, batch, max_tokens);
+  const int splits = workspace_splits(max_q, q_heads / kv_heads, kv_heads, batch, max_tokens, head_dim);
   return splits == 1 ? 0 : static_cast<int64_t>(total_q) * q_heads * splits * (head_dim + 2) * 4;
 }
 
