@@ -116,3 +116,22 @@ def test_groups_of_unlike_size_where_nothing_averages(name, d, q_len, small):
     cache.v_params.copy_(cache.v_params.float() * lift * (1.0 if name == "bf16" else 2.0**7))
     q = torch.randn(q_len, 4, d, generator=g).to(DTYPES[name]).cuda()
     check(cache, q, q_len, name)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("q_len", [1, 300])
+@pytest.mark.parametrize("lift", [-20, -16, -12])
+def test_fp16_activations_over_keys_below_the_range_of_fp16(d, q_len, lift):
+    # Scales of keys that fp16 only has as subnormals, with a softmax scale that makes up for them.
+    g = torch.Generator().manual_seed(60 + lift)
+    cache = filled_cache(8, 2, 64, d, g)
+    cache.k_params.mul_(2.0**lift)
+    q = torch.randn(q_len, 4, d, generator=g).to(torch.float16).cuda()
+    table = torch.arange(8, dtype=torch.int32).cuda()[None]
+    sc = d**-0.5 * 2.0**-lift
+    out = kv4.kv4_attention(q, cache, table, torch.tensor([500], dtype=torch.int32).cuda(), scale=sc).double()
+    k, v = request_rows(cache, table[0], 500)
+    sees = 500 - q_len + torch.arange(q_len, device="cuda") + 1
+    want, mag, most = ref.attention(q.double(), k, v, sees, sc)
+    bound = (2 * 2.0**-11 + 2 * 2.0**-11 * sc * most[..., None] + 1e-4) * mag + UNIT["fp16"] * want.abs()
+    assert ((out - want).abs() <= bound).all(), ((out - want).abs() / bound).max()

@@ -5,7 +5,7 @@
 // A CTA takes one or two tiles of rows of one (request, key head) and walks over
 // the tokens, 128 at a time:
 //   * warps 8-11 turn the tile's codes into fp16 in shared memory, one token a thread, a
-//     key or value rounded once (bf16 activations: in units of their own, below). Keys and values have the same
+//     key or value rounded once (in units of their own, below). Keys and values have the same
 //     layout there, 128-byte rows of 64 channels a token, swizzled: the keys are the
 //     K-major B operand of S = Q K^T, the values the transposed (N-contiguous) B
 //     operand of O += P V. The order of channels within a row is the order in which
@@ -23,8 +23,8 @@
 //   * where there are few (request, key head, block) units, up to 64 CTAs share the
 //     tokens of one and leave fp32 parts in a workspace, which kv4_join_kernel joins.
 // Floor: the two products. 4 prompts of 2048 tokens, 16 + 2 x 8 heads of 128 channels,
-// causal: 103 us, 0.67 PFLOP/s (fp16 operands in units: 13 us more than bf16 operands
-// took, for half the error). What bounds it is latency: some 4000 clocks for 128
+// causal: 105 us, 0.65 PFLOP/s in bf16 (fp16 operands in units: 13 us more than bf16 operands
+// took, for half the error) and 100 us in fp16, whose q needs no units. What bounds it is latency: some 4000 clocks for 128
 // tokens of two tiles, where the tensor cores need 2600 and the exponentials 2050, as
 // the chain S -> maximum -> exponentials -> P -> products has only the other tile to
 // hide behind (two tiles fill the tensor memory), and 12000 clocks a CTA before its
@@ -70,14 +70,16 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
 
 __device__ __forceinline__ float exp2_int(int e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
 
-// The operands are fp16, rounded once from what the codes stand for; sums are fp32. fp16 activations
-// as they are: their keys and values fit. bf16 ones reach further, so they are brought to units of
-// a power of two: q a row (largest magnitude 2^14 to 2^15), keys and values every 32 tokens, a warp of
-// those that make them (2^7 to 2^15, in steps of 2^8 so that units seldom differ); what is below
-// 2^-21 of the largest loses bits. The units of q and keys
-// go into the scores' factor, that of the values into P where it is not the output's own, which
-// follows the largest. Against 64 bits (2-norm) bf16 operands had 3.2e-3, of which the output's own
-// rounding is 1.7e-3; fp16 activations have 4e-4 and 2e-4.
+// The operands are fp16, rounded once from what the codes stand for; sums are fp32. Keys, values and
+// bf16 activations reach further than fp16, and their scales further down, so they are brought to
+// units of a power of two: q a row (largest magnitude 2^14 to 2^15; fp16 ones stay as they are), keys
+// and values every 32 tokens, a warp of those that make them (2^7 to 2^15, in steps of 2^8 so that units
+// seldom differ); what is below 2^-21 of the largest of those 32 tokens loses bits. The units of q and
+// keys go into the scores' factor, that of the values into P where it is not the output's own, which
+// follows the largest. Against 64 bits (2-norm) bf16 operands had 3.2e-3, these have 1.7e-3, the
+// output's own rounding; fp16 activations have 3e-4 to 4e-4, of which that is 2e-4. (fp16 activations
+// over keys and values as they are: 92 us instead of 100 for 4 x 2048 tokens, but scales below 2^-14
+// are subnormals then, and keys with a scale of 2^-18 gave scores off by 2^-8.)
 __device__ __forceinline__ uint32_t values(uint32_t w, int n, uint32_t s, uint32_t z) {
   // code * s + z of nibbles n and n + 4 of a word: 1024 + code by a mask, less 1024 (exact), and one
   // rounding in the multiply-add.
@@ -110,10 +112,9 @@ __global__ void __launch_bounds__(kPmThreads, 1)
   constexpr int NG = D / kKv4Group;
   constexpr int kWords = D / 8;  // 32-bit words of codes a row; chunks of eight channels
   constexpr uint32_t kIdescS = umma_idesc(0u, 0u, kPmTile, kPmSub);
-  constexpr uint32_t kIdescO = 
-      umma_idesc(0u, 0u, kPmTile, D) | kUmmaBTransposed;
+  constexpr uint32_t kIdescO = umma_idesc(0u, 0u, kPmTile, D) | kUmmaBTransposed;
   constexpr uint32_t kColS = 0, kColO = 2 * kPmTile;
-  constexpr bool kUnits = std::is_same_v<T, __nv_bfloat16>;
+  constexpr bool kQUnits = std::is_same_v<T, __nv_bfloat16>;
   constexpr float kLift = 7.f;  // of P: at most 2^15 while the maximum lags by 2^8; normal down to 2^-21
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -254,13 +255,7 @@ __global__ void __launch_bounds__(kPmThreads, 1)
     };
     // Scales (z = false) or minima (z = true) of two groups as a pair in fp16.
     const auto pair = [&](uint32_t x, uint32_t y, bool z, float up) {
-      if constexpr (kUnits) {
-        return z ? pack_f16x2(kv4_min(x) * up, kv4_min(y) * up) : pack_f16x2(kv4_scale(x) * up, kv4_scale(y) * up);
-      } else {
-        // The largest finite minimum that bf16 rounded up to 2^16 comes back to 65504.
-        const auto fit = [](float v) { return fabsf(v) <= 65536.f ? fminf(fmaxf(v, -65504.f), 65504.f) : v; };
-        return z ? pack_f16x2(fit(kv4_min(x)), fit(kv4_min(y))) : pack_f16x2(kv4_scale(x), kv4_scale(y));
-      }
+      return z ? pack_f16x2(kv4_min(x) * up, kv4_min(y) * up) : pack_f16x2(kv4_scale(x) * up, kv4_scale(y) * up);
     };
     if (most > 0) {
       find(0);
@@ -289,20 +284,17 @@ __global__ void __launch_bounds__(kPmThreads, 1)
           for (int i = 0; i < NG; ++i) vp[i] = 0u, kp[i] = 0x7FC07FC0u;
         }
       }
-      float kup = 1.f, vup = 1.f;
-      if constexpr (kUnits) {
-        uint32_t kt = 0u, vt = 0u;
+      uint32_t ktop = 0u, vtop = 0u;
 #pragma unroll
-        for (int i = 0; i < NG; ++i) kt = max(kt, group_top(kp[i])), vt = max(vt, group_top(vp[i]));
-        const int ke = max(16, static_cast<int>(__reduce_max_sync(0xffffffffu, kt) >> 23) | 7) - 141;
-        const int ve = max(16, static_cast<int>(__reduce_max_sync(0xffffffffu, vt) >> 23) | 7) - 141;
-        kup = exp2_int(-ke), vup = exp2_int(-ve);
-        // Both tiles have read this slot: vempty of step j - 3 was waited for, and it is handed back
-        // after P of that step, which is after what this slot held (step j - 4).
-        if (lane == 0) {
-          units[(j & 3) * 8 + warp - kPmDqWarp] = ke;
-          units[(j & 3) * 8 + 4 + warp - kPmDqWarp] = ve;
-        }
+      for (int i = 0; i < NG; ++i) ktop = max(ktop, group_top(kp[i])), vtop = max(vtop, group_top(vp[i]));
+      const int ke = max(16, static_cast<int>(__reduce_max_sync(0xffffffffu, ktop) >> 23) | 7) - 141;
+      const int ve = max(16, static_cast<int>(__reduce_max_sync(0xffffffffu, vtop) >> 23) | 7) - 141;
+      const float kup = exp2_int(-ke), vup = exp2_int(-ve);
+      // Both tiles have read this slot: vempty of step j - 3 was waited for, and it is handed back
+      // after P of that step, which is after what this slot held (step j - 4).
+      if (lane == 0) {
+        units[(j & 3) * 8 + warp - kPmDqWarp] = ke;
+        units[(j & 3) * 8 + 4 + warp - kPmDqWarp] = ve;
       }
       ok = j < kPmStages || wait(&kempty[s], j / kPmStages - 1);
       if (!ok) break;
@@ -429,7 +421,7 @@ __global__ void __launch_bounds__(kPmThreads, 1)
     // Tokens that all rows of this tile see (they are in order).
     const int first_lim = (a.causal ? len - n + div_by(r0 + i * kPmTile, share, a.share_inv) + 1 : len) - j0 * kPmTile;
     const bool whole = r0 + i * kPmTile + kPmTile <= rows;
-    float to_log2 = a.scale * 1.4426950408889634f;  // with bf16, from the units of the row's q
+    float to_log2 = a.scale * 1.4426950408889634f;  // from the units of the row's q
     float m = -INFINITY, l = 0.f;
     int vunit = -1000;  // of O, an exponent of two; none yet
     bool ok = true;
@@ -456,14 +448,14 @@ __global__ void __launch_bounds__(kPmThreads, 1)
       for (int x = 0; x < kPasses; ++x) {
         if (!(keep >> x & 1)) v[x] = make_uint4(0u, 0u, 0u, 0u);
         const uint32_t at = qt + tile_offset(tile_row + x * kRowsAPass + sub, ch);
-        if constexpr (kUnits) {
+        if constexpr (kQUnits) {
           sts128(at, v[x].x, v[x].y, v[x].z, v[x].w);
         } else {
           sts128(at, __byte_perm(v[x].x, v[x].z, 0x5410), __byte_perm(v[x].x, v[x].z, 0x7632),
                  __byte_perm(v[x].y, v[x].w, 0x5410), __byte_perm(v[x].y, v[x].w, 0x7632));
         }
       }
-      if constexpr (kUnits) {
+      if constexpr (kQUnits) {
         // Each thread brings its own row to its unit.
         __syncwarp();
         float top = 0.f;
@@ -493,14 +485,10 @@ __global__ void __launch_bounds__(kPmThreads, 1)
       const int left = lim - u * kPmSub;  // columns that this row sees
       const uint32_t tb = ts + (u & 1) * kPmSub;
       // Factors of the scores of the two halves, and units of their values.
-      float to0 = to_log2, to1 = to_log2;
-      int v0 = 0, v1 = 0;
-      if constexpr (kUnits) {
-        const volatile int* un = units + (u >> 1 & 3) * 8 + 2 * (u & 1);
-        to0 = fminf(fmaxf(to_log2 * exp2_int(un[0]), 1e-37f), 1e37f);
-        to1 = fminf(fmaxf(to_log2 * exp2_int(un[1]), 1e-37f), 1e37f);
-        v0 = un[4], v1 = un[5];
-      }
+      const volatile int* un = units + (u >> 1 & 3) * 8 + 2 * (u & 1);
+      const float to0 = fminf(fmaxf(to_log2 * exp2_int(un[0]), 1e-37f), 1e37f);
+      const float to1 = fminf(fmaxf(to_log2 * exp2_int(un[1]), 1e-37f), 1e37f);
+      const int v0 = un[4], v1 = un[5];
       uint32_t s[2][32];
       tmem_ld<32>(tb, s[0]);
       tmem_ld<32>(tb + 32, s[1]);
@@ -517,12 +505,12 @@ __global__ void __launch_bounds__(kPmThreads, 1)
       }
       const float mx = fmaxf(fmaxf(mx4[0], mx4[1]) * to0, fmaxf(mx4[2], mx4[3]) * to1);  // scale > 0
       const int vmost = max(v0, v1);
-      if (__any_sync(0xffffffffu, mx > m + 8.f) || (kUnits && vmost > vunit)) {
+      if (__any_sync(0xffffffffu, mx > m + 8.f) || vmost > vunit) {
         const float up = fmaxf(m, mx);
         float f = up > m ? ex2f(m - up) : 1.f;
         m = up;
         l *= f;
-        if (kUnits && vmost > vunit) {
+        if (vmost > vunit) {
           if (u > 0) f *= exp2_int(max(-126, vunit - vmost));
           vunit = vmost;
         }
@@ -554,13 +542,11 @@ __global__ void __launch_bounds__(kPmThreads, 1)
           sum[2 + k / 2 % 2] += y;
           p[k / 2] = pack_f16x2(x, y);
         }
-        if constexpr (kUnits) {
-          const int d = vunit - (c ? v1 : v0);
-          if (d != 0) {  // 2^-d as an fp16 pair, 0 below 2^-24
-            const uint32_t g = (d < 15 ? (15 - d) << 10 : d <= 24 ? 1 << (24 - d) : 0) * 0x10001u;
+        const int d = vunit - (c ? v1 : v0);
+        if (d != 0) {  // 2^-d as an fp16 pair, 0 below 2^-24
+          const uint32_t g = (d < 15 ? (15 - d) << 10 : d <= 24 ? 1 << (24 - d) : 0) * 0x10001u;
 #pragma unroll
-            for (int k = 0; k < 16; ++k) asm("mul.rn.f16x2 %0, %0, %1;" : "+r"(p[k]) : "r"(g));
-          }
+          for (int k = 0; k < 16; ++k) asm("mul.rn.f16x2 %0, %0, %1;" : "+r"(p[k]) : "r"(g));
         }
         tmem_st_x16(tb + 16 * c, p);
       }
@@ -581,7 +567,7 @@ __global__ void __launch_bounds__(kPmThreads, 1)
     }
     if (!ok && lane == 0) record_status(QTTS_ERR_TIMEOUT);
     if (i < tiles_a_cta && r0 + i * kPmTile < rows) {
-      const float unit = kUnits && steps[i] > 0 ? exp2_int(vunit) : 1.f;
+      const float unit = steps[i] > 0 ? exp2_int(vunit) : 1.f;
       const float inv = l == 0.f ? 0.f : unit / l;
       // Column 8 wi + 2 x + e of O is channel 32 (2 (wi % (NG/2)) + e) + 4 (wi / (NG/2)) + x: the
       // columns of NG words together are eight channels of every group. A warp's 32 rows go through
@@ -709,15 +695,16 @@ PromptPlan plan_prompt(int64_t max_q, int share, int kv_heads, int batch, int64_
   PromptPlan p;
   const int64_t rows = max_q * share;
   // Two tiles a CTA share the operands and hide each other's softmax (4 prompts of 2048 tokens,
-  // 16 + 2 x 8 heads of 128 channels: 103 us, one tile a CTA 156).
+  // 16 + 2 x 8 heads of 128 channels: 105 us, one tile a CTA 156).
   p.tiles = rows > kPmTile ? 2 : 1;
   p.blocks = (rows + p.tiles * kPmTile - 1) / (p.tiles * kPmTile);
   const int64_t units = p.blocks * kv_heads * batch;
   const int64_t steps = (most_tokens + kPmTile - 1) / kPmTile;
   // Enough CTAs for three a SM, so that long ones among short ones do not hold the call up, but
   // at least four steps each of the longest request (a shorter one takes fewer CTAs). 193 new
-  // tokens over 1500 to 5001 earlier ones, three requests of 32 + 2 x 4 heads of 64 channels: 47 us,
-  // one CTA an SM 52, at least eight steps 48, two steps 47.
+  // tokens over 1500 to 5001 earlier ones, three requests of 32 + 2 x 4 heads of 64 channels: 52 us;
+  // measured before its operands had units: 47 us, one CTA an SM 52, at least eight steps 48, two
+  // steps 47.
   const int64_t want = units >= 2 * kNumSMs ? 1 : (3 * kNumSMs + units - 1) / (units > 0 ? units : 1);
   const int64_t can = steps / 4;
   const int64_t s = want < can ? want : can;
