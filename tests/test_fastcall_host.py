@@ -1,0 +1,48 @@
+"""The argument-conversion module of the hot entry points among threads, and its build: on the host."""
+
+from __future__ import annotations
+
+import ctypes
+import threading
+import time
+
+import pytest
+
+from qtts_b200 import _native as nat
+
+NORM = [16, 64, 16, 64, 16, 1e-6, 16, 64, nat.BF16, 16, 64, nat.E4M3, 16, 4, 64, 0, None]
+
+
+def addresses():
+    return [ctypes.cast(getattr(nat.lib(), name), ctypes.c_void_p).value for name in nat._LAUNCHED]
+
+
+def test_other_threads_run_during_a_call():
+    # A launch may block (a full queue, a module's first load). Threads that run Python must not stand
+    # still for it: the work that it waits for may need one of them.
+    fast = nat._fastcall()
+    if fast is None:
+        pytest.skip("csrc/fastcall.c is not built here")
+    libc = ctypes.CDLL(None)
+    seen, stop = [], threading.Event()
+
+    def other():
+        while not stop.is_set():
+            seen.append(time.monotonic())
+            time.sleep(0.002)
+
+    thread = threading.Thread(target=other)
+    thread.start()
+    try:
+        # usleep in the place of an entry point: its first argument is the time.
+        fast.bind(ctypes.cast(libc.usleep, ctypes.c_void_p).value, *addresses()[1:])
+        time.sleep(0.02)
+        began = time.monotonic()
+        fast.qtts_add_rms_norm_quant(400_000, *NORM[1:])
+        ended = time.monotonic()
+    finally:
+        fast.bind(*addresses())
+        stop.set()
+        thread.join()
+    assert ended - began >= 0.35
+    assert sum(began + 0.05 < t < ended - 0.05 for t in seen) >= 10

@@ -35,11 +35,16 @@ static int ready(int which, Py_ssize_t got, Py_ssize_t want) {
   return 0;
 }
 
-/* The converted arguments are locals so that a failed conversion is seen before the call. */
-#define CALL(type, ...)                                           \
-  do {                                                            \
-    if (PyErr_Occurred()) return NULL;                            \
-    return PyLong_FromLong(((type)entry[which])(__VA_ARGS__));    \
+/* The converted arguments are locals, so that a failed conversion is seen before the call and the call
+ * holds no Python object: other threads run during it (a launch blocks while its queue is full). */
+#define CALL(type, ...)                                    \
+  do {                                                     \
+    int code;                                              \
+    if (PyErr_Occurred()) return NULL;                     \
+    Py_BEGIN_ALLOW_THREADS;                                \
+    code = ((type)entry[which])(__VA_ARGS__);              \
+    Py_END_ALLOW_THREADS;                                  \
+    return PyLong_FromLong(code);                          \
   } while (0)
 
 static PyObject* add_rms_norm_quant(PyObject* self, PyObject* const* a, Py_ssize_t n) {
