@@ -46,3 +46,37 @@ def test_other_threads_run_during_a_call():
         thread.join()
     assert ended - began >= 0.35
     assert sum(began + 0.05 < t < ended - 0.05 for t in seen) >= 10
+
+
+def test_first_calls_of_two_threads(monkeypatch):
+    # The second thread arrives while the first is still looking entry points up.
+    half_done, go_on = threading.Event(), threading.Event()
+
+    class Slow:
+        def __getattr__(self, name):
+            if name == nat._LAUNCHED[-1]:
+                half_done.set()
+                assert go_on.wait(10)
+            return lambda *args: nat.OK
+
+    monkeypatch.setattr(nat, "_calls", {})
+    monkeypatch.setattr(nat, "_fastcall", Slow)
+    monkeypatch.setattr(nat, "_raw_device", lambda: 0)
+    monkeypatch.setattr(nat, "_raw_stream", lambda index: None)
+    failed = []
+
+    def call(name):
+        try:
+            nat.launch(name, 0)
+        except BaseException as e:  # noqa: BLE001 - the test's result
+            failed.append(e)
+
+    threads = [threading.Thread(target=call, args=(name,)) for name in (nat._LAUNCHED[0], nat._LAUNCHED[-1])]
+    threads[0].start()
+    assert half_done.wait(10)
+    threads[1].start()
+    time.sleep(0.1)
+    go_on.set()
+    for t in threads:
+        t.join(10)
+    assert not failed and set(nat._calls) == set(nat._LAUNCHED)

@@ -224,6 +224,7 @@ _raw_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_d
 #: Entry points that ``launch`` calls; csrc/fastcall.c converts their arguments where it is built.
 _LAUNCHED = ("qtts_add_rms_norm_quant", "qtts_rope_kv4_append", "qtts_kv4_attention")
 _calls: dict[str, object] = {}
+_calls_lock = threading.Lock()
 
 
 def _fastcall():
@@ -256,9 +257,11 @@ def _through_ctypes(name: str):
 
 
 def _bind_calls() -> None:
-    fast = _fastcall()
-    for name in _LAUNCHED:
-        _calls[name] = getattr(fast, name) if fast is not None else _through_ctypes(name)
+    with _calls_lock:
+        if not _calls:  # all at once: other threads see none or all
+            fast = _fastcall()
+            _calls.update({name: getattr(fast, name) if fast is not None else _through_ctypes(name)
+                           for name in _LAUNCHED})
 
 
 def launch(name: str, index: int, *args) -> None:
