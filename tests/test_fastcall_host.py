@@ -80,3 +80,67 @@ def test_first_calls_of_two_threads(monkeypatch):
     for t in threads:
         t.join(10)
     assert not failed and set(nat._calls) == set(nat._LAUNCHED)
+
+
+@pytest.fixture
+def build_dir(monkeypatch, tmp_path):
+    from qtts_b200 import build
+
+    monkeypatch.setattr(build, "LIB_DIR", tmp_path)
+    monkeypatch.setattr(build, "LIB_PATH", tmp_path / "libqtts_b200.so")
+    monkeypatch.setattr(build, "FAST_PATH", tmp_path / "_qtts_fastcall.so")
+    monkeypatch.setattr(build, "nvcc_path", lambda: "nvcc")
+    monkeypatch.setattr(build, "PKG_DIR", tmp_path / "pkg")
+    return build
+
+
+def runs(monkeypatch, build, fails):
+    """Commands as build._run sees them: the output file appears, or the command fails."""
+    seen = []
+
+    def run(cmd, verbose):
+        what = "nvcc" if cmd[0] == "nvcc" else "cc"
+        seen.append(what)
+        if what in fails:
+            raise RuntimeError(f"{what} failed")
+        out = cmd[cmd.index("-o") + 1]
+        with open(out, "w") as f:
+            f.write("new")
+
+    monkeypatch.setattr(build, "_run", run)
+    return seen
+
+
+def test_a_failed_compile_of_the_module_leaves_the_library(build_dir, monkeypatch):
+    # The module is optional: without it the calls go through ctypes.
+    build_dir.FAST_PATH.write_text("old")
+    runs(monkeypatch, build_dir, {"cc"})
+    assert build_dir.build(force=True) == build_dir.LIB_PATH and build_dir.LIB_PATH.read_text() == "new"
+    assert not build_dir.FAST_PATH.exists()  # one of an earlier library would pass its old argument lists
+
+
+@pytest.mark.parametrize("gone", ["cc", "header"])
+def test_no_compiler_leaves_no_old_module(build_dir, monkeypatch, gone):
+    build_dir.FAST_PATH.write_text("old")
+    runs(monkeypatch, build_dir, set())
+    if gone == "cc":
+        monkeypatch.setattr(build_dir.shutil, "which", lambda name: None)
+    else:
+        monkeypatch.setattr(build_dir.sysconfig, "get_paths", lambda: {"include": "/nowhere"})
+    build_dir.build(force=True)
+    assert build_dir.LIB_PATH.read_text() == "new" and not build_dir.FAST_PATH.exists()
+
+
+def test_a_failed_library_leaves_library_and_module_as_they_were(build_dir, monkeypatch):
+    build_dir.LIB_PATH.write_text("old")
+    build_dir.FAST_PATH.write_text("old")
+    runs(monkeypatch, build_dir, {"nvcc"})
+    with pytest.raises(RuntimeError):
+        build_dir.build(force=True)
+    assert build_dir.LIB_PATH.read_text() == build_dir.FAST_PATH.read_text() == "old"
+
+
+def test_the_module_is_built_behind_the_library(build_dir, monkeypatch):
+    seen = runs(monkeypatch, build_dir, set())
+    build_dir.build(force=True)
+    assert seen[-2:] == ["nvcc", "cc"] and build_dir.FAST_PATH.read_text() == "new"

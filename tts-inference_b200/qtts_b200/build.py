@@ -69,7 +69,7 @@ def _run(cmd: list[str], verbose: bool) -> None:
         print(" ".join(cmd), file=sys.stderr)
     proc = subprocess.run(cmd, capture_output=True, text=True)
     if proc.returncode != 0:
-        raise RuntimeError(f"nvcc failed ({proc.returncode}):\n{proc.stdout}\n{proc.stderr}")
+        raise RuntimeError(f"{Path(cmd[0]).name} failed ({proc.returncode}):\n{proc.stdout}\n{proc.stderr}")
     if verbose and (proc.stdout or proc.stderr):
         print(proc.stdout + proc.stderr, file=sys.stderr)
 
@@ -99,21 +99,26 @@ def build(force: bool = False, verbose: bool = False, extra_flags: list[str] | N
     tmp = LIB_PATH.with_suffix(".so.tmp")
     _run([nvcc_path()] + ARCH_FLAGS + ["-shared", "-Xcompiler", "-fPIC", "-o", str(tmp)] + [str(o) for o in objs],
          verbose)
+    FAST_PATH.unlink(missing_ok=True)  # its argument lists are the old library's
     os.replace(tmp, LIB_PATH)
     build_fastcall(verbose)
     return LIB_PATH
 
 
 def build_fastcall(verbose: bool = False) -> Path | None:
-    """Compile the fast argument conversion; None where there is no C compiler or no Python.h
-    (the binding then goes through ctypes)."""
+    """Compile the fast argument conversion; None where there is no C compiler or no Python.h, or
+    where they fail (the binding then goes through ctypes)."""
     include = Path(sysconfig.get_paths()["include"])
     cc = shutil.which("gcc") or shutil.which("cc")
     if cc is None or not (include / "Python.h").exists():
         return None
     LIB_DIR.mkdir(parents=True, exist_ok=True)
     tmp = FAST_PATH.with_suffix(".so.tmp")
-    _run([cc, "-O2", "-fPIC", "-shared", "-I", str(include), "-o", str(tmp), str(SRC_DIR / "fastcall.c")], verbose)
+    try:
+        _run([cc, "-O2", "-fPIC", "-shared", "-I", str(include), "-o", str(tmp), str(SRC_DIR / "fastcall.c")], verbose)
+    except RuntimeError as e:
+        print(f"csrc/fastcall.c was not built, calls go through ctypes: {e}", file=sys.stderr)
+        return None
     os.replace(tmp, FAST_PATH)
     return FAST_PATH
 
