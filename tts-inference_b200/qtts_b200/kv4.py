@@ -54,6 +54,8 @@ class Kv4Cache:
         pages, kv_heads, page_size, half = shape
         if half not in _HALVES:
             raise ValueError(f"head_dim {2 * half}: the 4-bit cache takes {HEAD_DIMS}")
+        if kv_heads < 1:
+            raise ValueError("kv_heads is at least 1")
         if page_size < 16 or page_size % 16:
             raise ValueError(f"page_size {page_size} is not a multiple of 16")
         want = (pages, kv_heads, page_size, half * 2 // GROUP, 2)
