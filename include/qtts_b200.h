@@ -402,7 +402,10 @@ QTTS_API int qtts_add_rms_norm_quant(const void* x, int64_t ldx, const void* res
  *   q_out     [tokens, q_heads * head_dim] of qkv's type, leading dimension ldq
  *   k_values, v_values  [tokens, kv_heads, head_dim] of qkv's type, or both NULL:
  *             what the cache will give back for these tokens
- * fp32 from the load to the one rounding of each output. A position outside the
+ * fp32 from the load to the one rounding of each output, each step of the formulas
+ * rounded by itself (w * (x * inv), inv = 1 / sqrt(mean + eps) with IEEE root and
+ * division, a * cos - b * sin without contraction): the codes are those of the same
+ * steps as separate fp32 operations. A position outside the
  * tables or a slot outside the cache records QTTS_ERR_SHAPE on the device; such a
  * token is not stored (and with a bad position its outputs are zeros). 16-byte
  * aligned rows. Replaces: q/k norm, apply_rope and the cache write of
@@ -428,12 +431,15 @@ QTTS_API int qtts_rope_kv4_append(const void* qkv, int64_t ldqkv, int dtype, int
  *               table_cols * page_size is at most 2^30
  *   lengths     [batch] int32, at most table_cols * page_size
  *   q_starts    [batch + 1] int32 first rows of q; NULL: max_q rows a request. Rows
- *               of no request are not written
+ *               of no request, and of one with more rows than max_q, are not written
  *   max_q       the most new tokens of any request (bounds the launch)
  *   scale       positive and finite
  *   out         [total_q, q_heads, head_dim] of q's type, token stride given
  *   workspace   qtts_kv4_attention_workspace() bytes, 16-byte aligned; NULL when 0
- * page_size is a multiple of 16. Scores, softmax statistics and sums are fp32. A
+ * page_size is a multiple of 16. Scores, softmax statistics and sums are fp32;
+ * probabilities, values and (for many rows) keys are rounded once to fp16's 11 bits, in
+ * units of a power of two: a value keeps them down to 2^-21 of the largest of the 32
+ * tokens beside it (many rows) or 2^-24 of the largest met (few rows). A
  * length, row range or page number out of its bounds records QTTS_ERR_SHAPE on the
  * device; nothing outside the arrays is read, and that request's output means
  * nothing. Replaces: the SDPA backend over the

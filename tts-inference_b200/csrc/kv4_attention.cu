@@ -795,7 +795,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) kv4_join_kernel(const Kv4Attn
 // Which kernel: 16-row blocks that each read the cache (kv4_rows_kernel), or 128-row tiles
 // (kv4_prompt.cu), whose time hardly depends on how many of a tile's rows there are. Times
 // of the two in microseconds, 16 query and 8 key heads of 128 channels, from a request's
-// rows (new tokens x 2):
+// rows (new tokens x 2; both within 8 % of this since their operands keep more bits):
 //                                      32 rows        64 rows        128 rows
 //   1 request,   1000 tokens        9.1 |  18.5    10.2 |  18.4    13.1 |  17.5
 //   8 requests,  1000 tokens       17.5 |  19.6    19.9 |  19.9    37.6 |  20.5

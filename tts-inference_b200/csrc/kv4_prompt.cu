@@ -24,7 +24,11 @@
 //     tokens of one and leave fp32 parts in a workspace, which kv4_join_kernel joins.
 // Floor: the two products. 4 prompts of 2048 tokens, 16 + 2 x 8 heads of 128 channels,
 // causal: 105 us, 0.65 PFLOP/s in bf16 (fp16 operands in units: 13 us more than bf16 operands
-// took, for half the error) and 100 us in fp16, whose q needs no units. What bounds it is latency: some 4000 clocks for 128
+// took, for half the error) and 100 us in fp16, whose q needs no units; not causal, twice
+// the work, 184 us. fp16 operands are the choice because the products run at half that
+// rate from 32-bit ones, which would need twice the shared memory that two tiles fill
+// already; with fp16 activations they make 4e-4 of error (2-norm) where the output's own
+// rounding makes 2e-4. What bounds it is latency: some 4000 clocks for 128
 // tokens of two tiles, where the tensor cores need 2600 and the exponentials 2050, as
 // the chain S -> maximum -> exponentials -> P -> products has only the other tile to
 // hide behind (two tiles fill the tensor memory), and 12000 clocks a CTA before its

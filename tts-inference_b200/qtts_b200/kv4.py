@@ -9,8 +9,10 @@ qtts/attention/backends/torch_sdpa.py:16-69) as two launches:
 * :func:`kv4_attention` -- attention of one or many new tokens a request over that cache.
 
 :class:`Kv4Cache` holds the four tensors; ``include/qtts_b200.h`` gives their layout.
-Both functions launch on ``torch.cuda.current_stream()``, allocate only their outputs
-and never synchronize, so a decode step with them can be captured in a CUDA graph.
+Both functions launch on ``torch.cuda.current_stream()`` and never synchronize, so a decode
+step with them can be captured in a CUDA graph. They allocate their outputs, a workspace
+where a long cache is split among many CTAs, and copies of inputs whose rows are not
+16-byte aligned or whose strides the kernels do not take.
 There is no CPU path. Indices that live on the device (slots, positions, page numbers,
 lengths) are checked by the kernels: one out of range is left out and recorded
 (``_native.device_status()``).
@@ -123,7 +125,8 @@ def rope_kv4_append(
     a q or k head is turned by the tables' row ``positions[axis of j]``; ``positions`` is
     ``[tokens]`` or ``[axes, tokens]`` int64, ``sections`` says how many pairs each axis has
     (in order, or taking turns when ``interleaved``). ``q_norm`` / ``k_norm`` ``[head_dim]``
-    are the weights of the per-head RMSNorm.
+    are the weights of the per-head RMSNorm. The codes stored are those of the same steps as
+    separate fp32 torch operations, bit for bit.
 
     Returns q ``[tokens, q_heads, head_dim]``; with ``values`` also the keys and values
     ``[tokens, kv_heads, head_dim]`` as the cache will give them back.
