@@ -439,7 +439,8 @@ QTTS_API int qtts_rope_kv4_append(const void* qkv, int64_t ldqkv, int dtype, int
  * page_size is a multiple of 16. Scores, softmax statistics and sums are fp32;
  * probabilities, values and (for many rows) keys are rounded once to fp16's 11 bits, in
  * units of a power of two: a value keeps them down to 2^-21 of the largest of the 32
- * tokens beside it (many rows) or 2^-24 of the largest met (few rows). A
+ * cached tokens beside it (many rows; whether the row sees that one or not) or 2^-24 of
+ * the largest met (few rows). A
  * length, row range or page number out of its bounds records QTTS_ERR_SHAPE on the
  * device; nothing outside the arrays is read, and that request's output means
  * nothing. Replaces: the SDPA backend over the
